@@ -376,6 +376,139 @@ typedef struct mlvc_hip_y1_tail_desc {
 } mlvc_hip_y1_tail_desc;
 int mlvc_hip_y1_tail(const mlvc_hip_y1_tail_desc* desc, mlvc_hip_stream s);
 
+/* ---- attention over latent tokens ----
+ * Tokens are rows of FP16 heads, [token][head][head_dim], with a stride of
+ * their own (in halves, so a tensor may be a slice of a wider projection).
+ * No counterpart in the reference, whose only memory of earlier frames is the
+ * recurrent feature: these are for predictors that look at the latents of
+ * earlier frames themselves. Sums, norms and softmax statistics are FP32;
+ * every output is rounded to FP16 once (RNE). Strides are at least a row
+ * (heads * head_dim). Rows need no alignment beyond a half's; 16-byte aligned
+ * rows (pointers and strides) of heads of 64 or 128 run the fast kernels. */
+
+/* Norm and rotation of queries and keys, in one pass:
+ *   x' = x / sqrt(mean(x^2) + eps) * weight    per head (weight NULL: x' = x)
+ *   (a, b) -> (a c - b s, b c + a s),  c = m cos(p f_i), s = m sin(p f_i)
+ * for the pairs i < rot_dim / 2 of a head's first rot_dim values: (i, i +
+ * rot_dim / 2), or adjacent ones (2i, 2i + 1) when interleaved. p is the
+ * token's position, f_i = freqs[i] radians a position, m = rot_scale. The
+ * phase is reduced to one turn in FP64, so far positions lose nothing. The
+ * outputs may be the inputs (same pointer and stride), not overlap otherwise. */
+typedef struct mlvc_hip_qk_norm_rope_desc {
+    int tokens, q_heads, k_heads, head_dim; /* head_dim 1..512; one of the head counts may be 0 */
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    int64_t q_stride, k_stride, q_out_stride, k_out_stride; /* halves from token to token */
+    const void* q_weight;                   /* FP16 [head_dim], or NULL */
+    const void* k_weight;
+    float eps;
+    const int32_t* positions;               /* [tokens] */
+    const double* freqs;                    /* [rot_dim / 2], device memory */
+    int rot_dim;                            /* even, 0..head_dim; 0: no rotation */
+    int interleaved;
+    float rot_scale;
+} mlvc_hip_qk_norm_rope_desc;
+int mlvc_hip_qk_norm_rope(const mlvc_hip_qk_norm_rope_desc* desc, mlvc_hip_stream s);
+
+/* Frequencies of the rotation, freqs[i] = base^(-2i / rot_dim) for i <
+ * rot_dim / 2, stretched for contexts `factor` times as long as `trained`
+ * positions (factor >= 1):
+ *   MLVC_ROPE_PLAIN   unchanged;
+ *   MLVC_ROPE_LINEAR  every frequency divided by factor;
+ *   MLVC_ROPE_BASE    base * factor^(rot_dim / (rot_dim - 2)): the lowest
+ *                     frequency is divided by factor, the highest stays;
+ *   MLVC_ROPE_BANDS   by the turns t = trained * f / 2 pi a pair makes over the
+ *                     trained context: kept from 32 turns up, divided by factor
+ *                     up to 1 turn, mixed linearly in t between; *rot_scale =
+ *                     0.1 ln(factor) + 1 (1 for the others).
+ * Computed on the host in FP64; freqs_host holds rot_dim / 2 values. */
+enum { MLVC_ROPE_PLAIN = 0, MLVC_ROPE_LINEAR = 1, MLVC_ROPE_BASE = 2, MLVC_ROPE_BANDS = 3 };
+int mlvc_hip_rope_frequencies(int rot_dim, double base, int scaling, double factor, double trained,
+                              double* freqs_host, float* rot_scale);
+
+/* A paged cache of keys and values. Values are kept as
+ * [pages][heads][page_size][head_dim], the scales of quantised rows as FP32
+ * [pages][heads][page_size]. A slot is page * page_size + place in the page.
+ * A row x of one head is quantised on its own: a = max |x|, A = 448 (E4M3) or
+ * 127 (INT8), scale = a / A in FP32, stored = round(x A / a) (nearest, ties to
+ * even), and stands for stored * scale. A zero row has scale 0; a row with an
+ * infinity or NaN reads back as NaN throughout. */
+enum { MLVC_KV_F16 = 0, MLVC_KV_E4M3 = 1, MLVC_KV_INT8 = 2 };
+typedef struct mlvc_hip_kv_cache {
+    int kind;                /* MLVC_KV_* */
+    int pages, page_size;    /* page_size a multiple of 16; pages * page_size < 2^31 */
+    int heads, head_dim;     /* head_dim a multiple of 8 up to 512 */
+    void* k;                 /* 16-byte aligned */
+    void* v;
+    float* k_scale;          /* 16-byte aligned; unused with MLVC_KV_F16 */
+    float* v_scale;
+} mlvc_hip_kv_cache;
+/* Bytes of k or v, and of k_scale or v_scale (0 with MLVC_KV_F16). */
+size_t mlvc_hip_kv_cache_bytes(const mlvc_hip_kv_cache* cache);
+size_t mlvc_hip_kv_cache_scale_bytes(const mlvc_hip_kv_cache* cache);
+
+/* Rows to write or read: token t of k and v goes to or comes from slots[t].
+ * Writing skips a slot outside the cache (-1: a padding token), reading one
+ * gives zeros. A slot is written at most once a call. */
+typedef struct mlvc_hip_kv_rows {
+    int tokens;
+    void* k;                    /* FP16 rows; not changed by a write */
+    void* v;
+    int64_t k_stride, v_stride; /* halves from token to token */
+    const int32_t* slots;       /* [tokens] */
+} mlvc_hip_kv_rows;
+int mlvc_hip_kv_write(const mlvc_hip_kv_cache* cache, const mlvc_hip_kv_rows* rows, mlvc_hip_stream s);
+int mlvc_hip_kv_read(const mlvc_hip_kv_cache* cache, const mlvc_hip_kv_rows* rows, mlvc_hip_stream s);
+
+/* Attention of packed sequences:
+ *   out_i = sum_j p_ij v_j,  p_ij = softmax_j(scale q_i . k_j)
+ * Sequence n has the queries q_starts[n] .. q_starts[n + 1] and the keys
+ * k_starts[n] .. k_starts[n + 1]; its last query stands at its last key, and
+ * with causal a query sees the keys up to its own place only. A query that
+ * sees no key gives zeros. Query head h reads key head h * kv_heads / q_heads.
+ * What a query does not see (keys past its place, other sequences' rows) never
+ * reaches its output, infinities and NaN included. */
+typedef struct mlvc_hip_attention_prompt_desc {
+    int sequences, q_heads, kv_heads, head_dim; /* q_heads a multiple of kv_heads; head_dim 1..512 */
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    int64_t q_stride, k_stride, v_stride, out_stride; /* halves from token to token */
+    const int32_t* q_starts;   /* [sequences + 1], ascending, device memory */
+    const int32_t* k_starts;
+    int q_tokens, k_tokens;    /* rows of q / out and of k / v: starts beyond are cut to them */
+    int longest_q;             /* at least the longest sequence's queries; later ones are not computed */
+    int causal;
+    float scale;
+} mlvc_hip_attention_prompt_desc;
+int mlvc_hip_attention_prompt(const mlvc_hip_attention_prompt_desc* desc, mlvc_hip_stream s);
+
+/* Attention of one query per stream on the stream's cached context: stream n
+ * sees lengths[n] tokens, token j in page table[n][j / page_size]. A length of
+ * zero gives zeros; tokens of pages outside the cache are not seen. Long
+ * contexts are split over workgroups, which leave FP32 partials in the
+ * workspace that a second kernel joins in a fixed order. */
+typedef struct mlvc_hip_attention_token_desc {
+    const mlvc_hip_kv_cache* cache;
+    int streams, q_heads;          /* q_heads a multiple of the cache's heads */
+    const void* q;                 /* [streams][q_heads][head_dim] FP16 */
+    void* out;
+    int64_t q_stride, out_stride;  /* halves from stream to stream */
+    const int32_t* table;          /* [streams][table_stride], device memory */
+    int table_stride;              /* pages of a table row */
+    const int32_t* lengths;        /* [streams], device memory */
+    int longest;                   /* at least the longest context; later tokens are not seen */
+    float scale;
+    void* workspace;               /* 16-byte aligned; mlvc_hip_attention_token_workspace_bytes */
+    size_t workspace_bytes;
+} mlvc_hip_attention_token_desc;
+/* Depends on streams, q_heads, longest and the cache's layout only (0: none needed). */
+size_t mlvc_hip_attention_token_workspace_bytes(const mlvc_hip_attention_token_desc* desc);
+int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip_stream s);
+
 #ifdef __cplusplus
 }
 #endif

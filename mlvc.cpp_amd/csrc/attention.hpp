@@ -1,0 +1,65 @@
+// Shared parts of the attention kernels: argument checks, wave reductions and
+// the rows of the paged cache.
+#pragma once
+
+#include "common.hpp"
+#include "mlvc_hip_device.h"
+
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+namespace mlvc_hip {
+
+inline void require(bool ok, const char* op, const char* what)
+{
+    if (!ok) throw std::runtime_error(std::string(op) + ": " + what);
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0; }
+inline bool aligned2(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 1u) == 0; }
+
+// 16-byte aligned rows of halves.
+inline bool vector_rows(const void* p, std::int64_t stride) { return aligned16(p) && stride % 8 == 0; }
+
+constexpr int kMaxHeadDim = 512;
+
+// Checks a cache descriptor; `op` names the caller in the message.
+void check_cache(const mlvc_hip_kv_cache* cache, const char* op);
+
+// Opaque to the optimiser: keeps the narrowing of an FP32 result a rounding
+// of its own.
+__device__ __forceinline__ float opaque(float x)
+{
+    asm("" : "+v"(x));
+    return x;
+}
+
+__device__ __forceinline__ std::uint32_t pack_rounded(float a, float b) { return pack_f16(opaque(a), opaque(b)); }
+
+// Reductions over groups of LANES adjacent lanes; every lane gets the result.
+template <int LANES>
+__device__ __forceinline__ float group_sum(float x)
+{
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+template <int LANES>
+__device__ __forceinline__ float group_max(float x)
+{
+#pragma unroll
+    for (int o = LANES / 2; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
+
+// 8-bit values of a cached row, widened. INT8 is two's complement.
+__device__ __forceinline__ float from_byte(int kind, std::uint8_t b)
+{
+    if (kind == MLVC_KV_INT8) return static_cast<float>(static_cast<std::int8_t>(b));
+    return __builtin_amdgcn_cvt_f32_fp8(b, 0);
+}
+
+}  // namespace mlvc_hip

@@ -97,6 +97,7 @@ def device_lib() -> C.CDLL:
     if _dev is None:
         _dev = _load(DEVICE_LIB)
         _dev.mlvc_hip_last_error.restype = C.c_char_p
+        _bind_attention(_dev)
     return _dev
 
 
@@ -411,3 +412,108 @@ def default_model_location() -> str:
     buf = C.create_string_buffer(4096)
     _check(backend_lib().mlvc_model_default_location(buf, len(buf)))
     return buf.value.decode()
+
+
+# ---- attention over latent tokens (device C ABI) ----------------------------
+# Tensors are device addresses (integers), as the device functions take them;
+# streams are hipStream_t handles, None for the default stream. Descriptors are
+# filled once for buffers that stay and passed to every call.
+
+KV_F16, KV_E4M3, KV_INT8 = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BANDS = 0, 1, 2, 3
+
+
+class QkNormRope(C.Structure):
+    """mlvc_hip_qk_norm_rope_desc"""
+    _fields_ = [(f, C.c_int) for f in ("tokens", "q_heads", "k_heads", "head_dim")] + [
+        (f, C.c_void_p) for f in ("q", "k", "q_out", "k_out")] + [
+        (f, C.c_int64) for f in ("q_stride", "k_stride", "q_out_stride", "k_out_stride")] + [
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("eps", C.c_float), ("positions", C.c_void_p),
+        ("freqs", C.c_void_p), ("rot_dim", C.c_int), ("interleaved", C.c_int), ("rot_scale", C.c_float)]
+
+
+class KvCache(C.Structure):
+    """mlvc_hip_kv_cache"""
+    _fields_ = [(f, C.c_int) for f in ("kind", "pages", "page_size", "heads", "head_dim")] + [
+        (f, C.c_void_p) for f in ("k", "v", "k_scale", "v_scale")]
+
+
+class KvRows(C.Structure):
+    """mlvc_hip_kv_rows"""
+    _fields_ = [("tokens", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64),
+                ("v_stride", C.c_int64), ("slots", C.c_void_p)]
+
+
+class PromptAttention(C.Structure):
+    """mlvc_hip_attention_prompt_desc"""
+    _fields_ = [(f, C.c_int) for f in ("sequences", "q_heads", "kv_heads", "head_dim")] + [
+        (f, C.c_void_p) for f in ("q", "k", "v", "out")] + [
+        (f, C.c_int64) for f in ("q_stride", "k_stride", "v_stride", "out_stride")] + [
+        ("q_starts", C.c_void_p), ("k_starts", C.c_void_p)] + [
+        (f, C.c_int) for f in ("q_tokens", "k_tokens", "longest_q", "causal")] + [("scale", C.c_float)]
+
+
+class TokenAttention(C.Structure):
+    """mlvc_hip_attention_token_desc; keep the KvCache that `cache` points to."""
+    _fields_ = [("cache", C.POINTER(KvCache)), ("streams", C.c_int), ("q_heads", C.c_int), ("q", C.c_void_p),
+                ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("table", C.c_void_p),
+                ("table_stride", C.c_int), ("lengths", C.c_void_p), ("longest", C.c_int), ("scale", C.c_float),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+def _bind_attention(lib) -> None:
+    lib.mlvc_hip_qk_norm_rope.argtypes = [C.POINTER(QkNormRope), C.c_void_p]
+    lib.mlvc_hip_rope_frequencies.argtypes = [C.c_int, C.c_double, C.c_int, C.c_double, C.c_double, C.c_void_p,
+                                              C.POINTER(C.c_float)]
+    for fn in (lib.mlvc_hip_kv_cache_bytes, lib.mlvc_hip_kv_cache_scale_bytes):
+        fn.argtypes, fn.restype = [C.POINTER(KvCache)], C.c_size_t
+    for fn in (lib.mlvc_hip_kv_write, lib.mlvc_hip_kv_read):
+        fn.argtypes = [C.POINTER(KvCache), C.POINTER(KvRows), C.c_void_p]
+    lib.mlvc_hip_attention_prompt.argtypes = [C.POINTER(PromptAttention), C.c_void_p]
+    lib.mlvc_hip_attention_token_workspace_bytes.argtypes = [C.POINTER(TokenAttention)]
+    lib.mlvc_hip_attention_token_workspace_bytes.restype = C.c_size_t
+    lib.mlvc_hip_attention_token.argtypes = [C.POINTER(TokenAttention), C.c_void_p]
+
+
+def _device_check(rc: int) -> None:
+    if rc != 0:
+        raise MlvcError(device_lib().mlvc_hip_last_error().decode())
+
+
+def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: int = ROPE_PLAIN, factor: float = 1.0,
+                     trained: float = 0.0) -> tuple[np.ndarray, float]:
+    """(radians a position of each pair, rot_scale) for QkNormRope.freqs and .rot_scale; host memory, FP64."""
+    freqs, scale = np.empty(max(rot_dim, 0) // 2, np.float64), C.c_float()
+    _device_check(device_lib().mlvc_hip_rope_frequencies(rot_dim, base, scaling, factor, trained, freqs.ctypes.data,
+                                                         C.byref(scale)))
+    return freqs, scale.value
+
+
+def qk_norm_rope(desc: QkNormRope, stream=None) -> None:
+    _device_check(device_lib().mlvc_hip_qk_norm_rope(desc, stream))
+
+
+def kv_cache_bytes(cache: KvCache) -> tuple[int, int]:
+    """Bytes of k (or v) and of k_scale (or v_scale)."""
+    lib = device_lib()
+    return lib.mlvc_hip_kv_cache_bytes(cache), lib.mlvc_hip_kv_cache_scale_bytes(cache)
+
+
+def kv_write(cache: KvCache, rows: KvRows, stream=None) -> None:
+    _device_check(device_lib().mlvc_hip_kv_write(cache, rows, stream))
+
+
+def kv_read(cache: KvCache, rows: KvRows, stream=None) -> None:
+    _device_check(device_lib().mlvc_hip_kv_read(cache, rows, stream))
+
+
+def attention_prompt(desc: PromptAttention, stream=None) -> None:
+    _device_check(device_lib().mlvc_hip_attention_prompt(desc, stream))
+
+
+def attention_token_workspace_bytes(desc: TokenAttention) -> int:
+    return device_lib().mlvc_hip_attention_token_workspace_bytes(desc)
+
+
+def attention_token(desc: TokenAttention, stream=None) -> None:
+    _device_check(device_lib().mlvc_hip_attention_token(desc, stream))
