@@ -9,6 +9,8 @@
 
 #include "attention.hpp"
 
+#include <type_traits>
+
 namespace mlvc_hip {
 namespace {
 
@@ -20,8 +22,8 @@ struct PromptArgs {
     std::int64_t q_stride, k_stride, v_stride, out_stride;
     const std::int32_t* q_starts;
     const std::int32_t* k_starts;
-    int sequences, q_heads, group, dim, q_tokens, k_tokens, longest_q, causal;
-    float scale2;  // scale log2(e)
+    int sequences, q_heads, group, dim, q_tokens, k_tokens, longest_q, causal, negate;
+    float scale2;  // |scale| log2(e); negate: scale is negative
 };
 
 // Rows [first, first + count) of a sequence, cut to the tensor.
@@ -51,7 +53,7 @@ __global__ __launch_bounds__(64) void prompt_any_kernel(PromptArgs a)
     if (i < 0 || i >= sq.count || i >= a.longest_q) return;
     const int seen = a.causal ? min(sk.count, max(0, sk.count - sq.count + i + 1)) : sk.count;
     const std::uint16_t* q = a.q + token * a.q_stride + static_cast<std::int64_t>(head) * a.dim;
-    for (int d = lane; d < a.dim; d += 64) qs[d] = h2f(q[d]) * a.scale2;
+    for (int d = lane; d < a.dim; d += 64) qs[d] = h2f(q[d]) * (a.negate ? -a.scale2 : a.scale2);
     __syncthreads();
     const std::int64_t column = static_cast<std::int64_t>(head / a.group) * a.dim;
     constexpr int kColumns = kMaxHeadDim / 64;
@@ -88,6 +90,309 @@ __global__ __launch_bounds__(64) void prompt_any_kernel(PromptArgs a)
         if (c * 64 + lane < a.dim) out[c * 64 + lane] = f2h(opaque(acc[c] * r));
 }
 
+// ------------------------------------------------------------ matrix cores
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kRawBufferFlags = 0x00020000;
+constexpr int kKeys = 64;          // keys of a tile
+constexpr float kSlack = 8.0f;     // how far, in powers of two, a score may pass the running maximum before it moves
+
+// Maximum (sum) of a lane's value and that of the lane 32 away, in both.
+__device__ __forceinline__ float both_max(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_sum(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Heads of D values, rows on 16 bytes. A workgroup of WAVES waves takes
+// WAVES * QT * 32 queries of a head; a wave holds QT * 32 of them as columns
+// of S^T = K Q^T (32x32x16 products, keys as rows), so that
+//   * a lane's scores all belong to one query: the softmax needs one exchange,
+//     between the two lanes of a column;
+//   * the accumulator registers of S^T, rounded to FP16, are the B operand of
+//     O^T += V^T P^T as they stand (the 16 keys of a step are taken in the order
+//     the registers hold them), so weights never leave the lane.
+// Tiles of 64 keys are staged by LDS DMA, double-buffered, 16-byte pieces of a
+// row permuted (piece ^ f(row)) so that both reads are free of bank conflicts:
+// K rows by 16 bytes, V by the transposing read. Rows past a sequence's end are
+// out of the buffer's range and read as zeros.
+//
+// The running maximum moves only when a score passes it by 2^8 (weights up to
+// 2^8 lose nothing in FP16 or in the FP32 sums), so the accumulators are seldom
+// rescaled. Weights are rounded to FP16, the type the matrix cores take beside
+// V: one rounding of 2^-11 each, no more than the output's own.
+template <int D_, int WAVES_, int QT_>
+struct PromptCfg {
+    static constexpr int D = D_, WAVES = WAVES_, QT = QT_;
+    static constexpr int ROWS = WAVES * QT * 32;     // queries of a workgroup
+    static constexpr int PIECES = D / 8;             // 16-byte pieces of a row
+    static constexpr int DMA_ROWS = 64 / PIECES;     // rows of a DMA instruction
+    static constexpr int DMA = kKeys / DMA_ROWS;     // instructions of a tile
+    static constexpr int TILE = kKeys * D;           // halves
+    static constexpr size_t LDS = 4 * TILE * 2;      // K and V, two buffers
+};
+
+template <class C>
+__global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, int tiles)
+{
+    constexpr int D = C::D, QT = C::QT, KS = D / 16, DT = D / 32;
+    extern __shared__ __attribute__((aligned(16))) std::uint16_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int column = lane & 31, hi = lane >> 5;
+
+    // Workgroup i runs on XCD i % 8: with a multiple of 8 heads an XCD keeps the
+    // same heads, of all sequences, so their keys stay in its L2. The last
+    // tiles of the queries, which see most keys, go first.
+    int head, n, tile;
+    if (a.q_heads % kXcds == 0) {
+        const int per = a.q_heads / kXcds, i = blockIdx.x / kXcds, j = i / per;
+        head = blockIdx.x % kXcds * per + i % per;
+        n = j % a.sequences;
+        tile = tiles - 1 - j / a.sequences;
+    } else {
+        const int j = blockIdx.x / a.q_heads;
+        head = blockIdx.x % a.q_heads;
+        n = j % a.sequences;
+        tile = tiles - 1 - j / a.sequences;
+    }
+    const Span sq = span(a.q_starts, n, a.q_tokens), sk = span(a.k_starts, n, a.k_tokens);
+    const int q0 = tile * C::ROWS, nq = min(sq.count, a.longest_q);
+    if (q0 >= nq) return;
+    const int behind = sk.count - sq.count;  // keys before the first query
+    const int last = min(q0 + C::ROWS, nq) - 1;
+    const int keys = a.causal ? max(0, min(sk.count, behind + last + 1)) : sk.count;  // seen by any query here
+    const int steps = (keys + kKeys - 1) / kKeys;
+
+    // This wave's queries, as B fragments.
+    const int w0 = q0 + wave * QT * 32;
+    half8 q[QT][KS];
+    int seen[QT];  // keys this lane's query sees
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int i = w0 + qt * 32 + column, at = min(i, nq - 1);
+        const std::uint16_t* row = a.q + (sq.first + at) * a.q_stride + static_cast<std::int64_t>(head) * D + hi * 8;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            u32x4 v = *reinterpret_cast<const u32x4*>(row + ks * 16);
+            if (a.negate)
+                for (int e = 0; e < 4; ++e) v[e] ^= 0x80008000u;
+            q[qt][ks] = __builtin_bit_cast(half8, v);
+        }
+        seen[qt] = a.causal ? max(0, min(sk.count, behind + at + 1)) : sk.count;
+    }
+    // Keys that every query of this wave sees, and that any of them sees.
+    const int all = w0 >= nq ? 0 : a.causal ? max(0, min(sk.count, behind + w0 + 1)) : sk.count;
+    const int any = w0 >= nq ? 0 : a.causal ? max(0, min(sk.count, behind + min(w0 + QT * 32, nq))) : sk.count;
+
+    const std::int64_t kv = static_cast<std::int64_t>(head / a.group) * D;
+    const std::uint16_t* const k0 = a.k + sk.first * a.k_stride + kv;
+    const std::uint16_t* const v0 = a.v + sk.first * a.v_stride + kv;
+    // Piece p of row t is kept at place p ^ f(t), f(t) = 2 (t & 3) + (t >> 2 & 1).
+    const int drow = lane / C::PIECES, first_row = wave * C::DMA_ROWS + drow;
+    const int piece = (lane % C::PIECES) ^ (2 * (first_row & 3) + (first_row >> 2 & 1));
+    static_assert(C::DMA_ROWS * C::WAVES % 8 == 0 && C::DMA % C::WAVES == 0);
+    auto stage = [&](const std::uint16_t* x, std::int64_t stride, int step, std::uint16_t* to) {
+        const std::uint32_t stride2 = static_cast<std::uint32_t>(stride) * 2u;
+        const std::uint64_t p = reinterpret_cast<std::uint64_t>(x + static_cast<std::int64_t>(step) * kKeys * stride);
+        const int rows = min(kKeys, sk.count - step * kKeys);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+            reinterpret_cast<void*>(p), 0, static_cast<int>((rows - 1) * stride2 + 2u * D), kRawBufferFlags);
+        const std::uint32_t at = first_row * stride2 + piece * 16u;
+#pragma unroll
+        for (int i = 0; i < C::DMA / C::WAVES; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                r, (__attribute__((address_space(3))) void*)(to + (wave + i * C::WAVES) * 512), 16,
+                static_cast<int>(at + i * C::WAVES * C::DMA_ROWS * stride2), 0, 0, 0);
+    };
+    // Places of this lane's pieces: K row lane & 31, pieces 2 ks + hi; V rows 4 hi + (lane & 15) / 4 ..., the
+    // transposing read of 16 lanes gives each lane the four rows of one column.
+    const int fk = 2 * (column & 3) + (column >> 2 & 1);
+    int kat[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) kat[b] = column * D + ((2 * b + hi) ^ fk) * 8;
+    const int vrow = (lane & 15) >> 2, fv = 2 * vrow + hi;
+    int vat[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+        vat[b] = (4 * hi + vrow) * D + ((4 * b + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ fv) * 8 + (lane & 1) * 4;
+    auto value_fragment = [&](const std::uint16_t* tile_v, int step, int dt) {
+        u32x2 v[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            v[e] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                 (__attribute__((address_space(3))) s16x4*)(
+                                                     tile_v + vat[dt & 1] + (dt >> 1) * 64 + (step * 16 + e * 8) * D)));
+        return u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
+    };
+
+    floatx16 acc[QT][DT];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        m[qt] = -INFINITY, l[qt] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[qt][dt][r] = 0.0f;
+    }
+
+    auto compute = [&](int step, const std::uint16_t* tile_k, const std::uint16_t* tile_v, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const int j0 = step * kKeys;
+        floatx16 s[QT][2] = {};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            half8 kf[2];
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+                kf[tt] = *reinterpret_cast<const half8*>(tile_k + kat[ks & 3] + (ks >> 2) * 64 + tt * 32 * D);
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+                    s[qt][tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[tt], q[qt][ks], s[qt][tt], 0, 0, 0);
+        }
+        half8 p[QT][4];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (j0 + tt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen[qt]) s[qt][tt][r] = -INFINITY;
+            }
+            float top = fmaxf(s[qt][0][0], s[qt][1][0]);
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, fmaxf(s[qt][0][r], s[qt][1][r]));
+            top = both_max(top) * a.scale2;
+            if (__any(top > m[qt] + kSlack)) {
+                const float now = fmaxf(m[qt], top), keep = __builtin_amdgcn_exp2f(m[qt] - (now == -INFINITY ? 0.0f : now));
+                m[qt] = now;
+                l[qt] *= keep;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[qt][dt][r] *= keep;
+            }
+            const float base = m[qt] == -INFINITY ? 0.0f : m[qt];
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[qt][tt][r], a.scale2, -base)),
+                                y = __builtin_amdgcn_exp2f(fmaf(s[qt][tt][r + 1], a.scale2, -base));
+                    sum[0] += x;
+                    sum[1] += y;
+                    p[qt][tt * 2 + (r >> 3)][r & 7] = static_cast<_Float16>(x);
+                    p[qt][tt * 2 + (r >> 3)][(r & 7) + 1] = static_cast<_Float16>(y);
+                }
+            l[qt] += sum[0] + sum[1];
+        }
+        std::uint32_t odd = 0;
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                u32x4 vf = value_fragment(tile_v, st, dt);
+                if constexpr (MASKED) {
+                    // Values whose weight may be zero must be finite: 0 * inf is NaN.
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const std::uint32_t lo = (vf[e] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u,
+                                            up = (vf[e] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
+                        odd |= lo | up;
+                        vf[e] &= ~(lo | up);
+                    }
+                }
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+                    acc[qt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, vf), p[qt][st], acc[qt][dt], 0, 0, 0);
+            }
+        if constexpr (MASKED) {
+            // What was left out above: a query that sees an infinity or NaN gets
+            // it. Counted by products of 0 / 1 matrices, once for +inf and NaN,
+            // once for -inf and NaN.
+            if (__any(odd != 0)) {
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+                        for (int sign = 0; sign < 2; ++sign) {
+                            floatx16 count = {};
+                            for (int st = 0; st < 4; ++st) {
+                                const u32x4 vf = value_fragment(tile_v, st, dt);
+                                half8 is, sees;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const std::uint32_t v = vf[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+                                    const bool bad = (v & 0x7fffu) > 0x7c00u || v == (sign ? 0xfc00u : 0x7c00u);
+                                    is[e] = static_cast<_Float16>(bad ? 1.0f : 0.0f);
+                                    const int j = j0 + st * 16 + 8 * (e >> 2) + 4 * hi + (e & 3);
+                                    sees[e] = static_cast<_Float16>(j < seen[qt] ? 1.0f : 0.0f);
+                                }
+                                count = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, count, 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                if (count[r] > 0.0f) acc[qt][dt][r] += sign ? -INFINITY : INFINITY;
+                        }
+            }
+        }
+    };
+
+    std::uint16_t* const tile_k = lds;
+    std::uint16_t* const tile_v = lds + 2 * C::TILE;
+    if (steps > 0) {
+        stage(k0, a.k_stride, 0, tile_k);
+        stage(v0, a.v_stride, 0, tile_v);
+    }
+    for (int step = 0; step < steps; ++step) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's DMA of the tile
+        __syncthreads();
+        const int now = step & 1, next = now ^ 1;
+        if (step + 1 < steps) {
+            stage(k0, a.k_stride, step + 1, tile_k + next * C::TILE);
+            stage(v0, a.v_stride, step + 1, tile_v + next * C::TILE);
+        }
+        const int j1 = step * kKeys + kKeys;
+        if (j1 <= all) compute(step, tile_k + now * C::TILE, tile_v + now * C::TILE, std::false_type{});
+        else if (j1 - kKeys < any) compute(step, tile_k + now * C::TILE, tile_v + now * C::TILE, std::true_type{});
+    }
+
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int i = w0 + qt * 32 + column;
+        const float sum = both_sum(l[qt]), r = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (i >= nq) continue;
+        std::uint16_t* out = a.out + (sq.first + i) * a.out_stride + static_cast<std::int64_t>(head) * D + 4 * hi;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<uint2*>(out + dt * 32 + 8 * g) =
+                    make_uint2(pack_rounded(acc[qt][dt][4 * g] * r, acc[qt][dt][4 * g + 1] * r),
+                               pack_rounded(acc[qt][dt][4 * g + 2] * r, acc[qt][dt][4 * g + 3] * r));
+    }
+}
+
+template <class C>
+void launch_prompt(const PromptArgs& a, hipStream_t s)
+{
+    const int tiles = (a.longest_q + C::ROWS - 1) / C::ROWS;
+    const std::int64_t grid = static_cast<std::int64_t>(tiles) * a.q_heads * a.sequences;
+    require(grid <= INT_MAX, "attention_prompt", "too many sequences, heads and queries in one call");
+    prompt_kernel<C><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles);
+}
+
 void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
 {
     const char* op = "attention_prompt";
@@ -115,8 +420,16 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
     a.q_starts = d->q_starts, a.k_starts = d->k_starts;
     a.sequences = d->sequences, a.q_heads = d->q_heads, a.group = d->q_heads / d->kv_heads, a.dim = d->head_dim;
     a.q_tokens = d->q_tokens, a.k_tokens = d->k_tokens, a.longest_q = d->longest_q, a.causal = d->causal != 0;
-    a.scale2 = d->scale * 1.4426950408889634f;
-    prompt_any_kernel<<<dim3(static_cast<unsigned>(d->q_tokens), static_cast<unsigned>(d->q_heads)), 64, 0, s>>>(a);
+    a.scale2 = std::fabs(d->scale) * 1.4426950408889634f, a.negate = d->scale < 0.0f;
+    // The matrix-core kernel addresses a tile's rows by 32-bit byte offsets,
+    // and scales masked scores (-inf) by the factor, which must not be 0.
+    constexpr std::int64_t kFarthest = std::int64_t{1} << 23;
+    const bool rows = vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride) && vector_rows(d->k, d->k_stride) &&
+                      vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f;
+    if (rows && d->head_dim == 128) launch_prompt<PromptCfg<128, 4, 1>>(a, s);
+    else if (rows && d->head_dim == 64) launch_prompt<PromptCfg<64, 4, 1>>(a, s);
+    else
+        prompt_any_kernel<<<dim3(static_cast<unsigned>(d->q_tokens), static_cast<unsigned>(d->q_heads)), 64, 0, s>>>(a);
     check(hipGetLastError(), "attention_prompt launch");
 }
 
