@@ -99,6 +99,22 @@ constexpr int kRawBufferFlags = 0x00020000;
 constexpr int kKeys = 64;          // keys of a tile
 constexpr float kSlack = 8.0f;     // how far, in powers of two, a score may pass the running maximum before it moves
 
+__device__ __forceinline__ std::uint32_t uniform(std::uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// 16 bytes a lane from `at` bytes into a raw buffer to LDS, lane after lane;
+// out of the buffer's range, zeros. In assembly because the compiler lets every
+// LDS read that follows the builtin wait for it: here the tile that is read and
+// the one being filled are never the same, and the caller waits (vmcnt) and
+// synchronises before it turns to the next.
+__device__ __forceinline__ void lds_dma16(u32x4 buffer, std::uint32_t to, std::uint32_t at)
+{
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(buffer) : "memory", "m0");
+}
+__device__ __forceinline__ std::uint32_t lds_address(const void* p)
+{
+    return static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) const void*)p));
+}
+
 // Maximum (sum) of a lane's value and that of the lane 32 away, in both.
 __device__ __forceinline__ float both_max(float x)
 {
@@ -187,8 +203,8 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
         }
         seen[qt] = a.causal ? max(0, min(sk.count, behind + at + 1)) : sk.count;
     }
-    // Keys that every query of this wave sees, and that any of them sees.
-    const int all = w0 >= nq ? 0 : a.causal ? max(0, min(sk.count, behind + w0 + 1)) : sk.count;
+    // Tiles that every query of the workgroup sees whole, and keys that any of this wave's sees.
+    const int clear = (a.causal ? max(0, min(sk.count, behind + q0 + 1)) : sk.count) / kKeys;
     const int any = w0 >= nq ? 0 : a.causal ? max(0, min(sk.count, behind + min(w0 + QT * 32, nq))) : sk.count;
 
     const std::int64_t kv = static_cast<std::int64_t>(head / a.group) * D;
@@ -198,18 +214,16 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
     const int drow = lane / C::PIECES, first_row = wave * C::DMA_ROWS + drow;
     const int piece = (lane % C::PIECES) ^ (2 * (first_row & 3) + (first_row >> 2 & 1));
     static_assert(C::DMA_ROWS * C::WAVES % 8 == 0 && C::DMA % C::WAVES == 0);
-    auto stage = [&](const std::uint16_t* x, std::int64_t stride, int step, std::uint16_t* to) {
+    auto stage = [&](const std::uint16_t* x, std::int64_t stride, int step, std::uint32_t to) {
         const std::uint32_t stride2 = static_cast<std::uint32_t>(stride) * 2u;
         const std::uint64_t p = reinterpret_cast<std::uint64_t>(x + static_cast<std::int64_t>(step) * kKeys * stride);
         const int rows = min(kKeys, sk.count - step * kKeys);
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-            reinterpret_cast<void*>(p), 0, static_cast<int>((rows - 1) * stride2 + 2u * D), kRawBufferFlags);
+        const u32x4 r = {uniform(static_cast<std::uint32_t>(p)), uniform(static_cast<std::uint32_t>(p >> 32)) & 0xffffu,
+                         uniform((rows - 1) * stride2 + 2u * D), kRawBufferFlags};
         const std::uint32_t at = first_row * stride2 + piece * 16u;
 #pragma unroll
         for (int i = 0; i < C::DMA / C::WAVES; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                r, (__attribute__((address_space(3))) void*)(to + (wave + i * C::WAVES) * 512), 16,
-                static_cast<int>(at + i * C::WAVES * C::DMA_ROWS * stride2), 0, 0, 0);
+            lds_dma16(r, to + (wave + i * C::WAVES) * 1024, at + i * C::WAVES * C::DMA_ROWS * stride2);
     };
     // Places of this lane's pieces: K row lane & 31, pieces 2 ks + hi; V rows 4 hi + (lane & 15) / 4 ..., the
     // transposing read of 16 lanes gives each lane the four rows of one column.
@@ -246,7 +260,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
     auto compute = [&](int step, const std::uint16_t* tile_k, const std::uint16_t* tile_v, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         const int j0 = step * kKeys;
-        floatx16 s[QT][2] = {};
+        floatx16 s[QT][2];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             half8 kf[2];
@@ -257,7 +271,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
             for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt)
-                    s[qt][tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[tt], q[qt][ks], s[qt][tt], 0, 0, 0);
+                    s[qt][tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[tt], q[qt][ks], ks ? s[qt][tt] : floatx16{}, 0, 0, 0);
         }
         half8 p[QT][4];
 #pragma unroll
@@ -269,9 +283,12 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
                     for (int r = 0; r < 16; ++r)
                         if (j0 + tt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen[qt]) s[qt][tt][r] = -INFINITY;
             }
-            float top = fmaxf(s[qt][0][0], s[qt][1][0]);
+            // The NaN-propagating maximum of three is one instruction; a score that
+            // is NaN leaves the maximum where it was, and its query becomes NaN.
+            float top = __builtin_elementwise_maximum(s[qt][0][0], s[qt][1][0]);
 #pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, fmaxf(s[qt][0][r], s[qt][1][r]));
+            for (int r = 1; r < 16; ++r)
+                top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[qt][0][r]), s[qt][1][r]);
             top = both_max(top) * a.scale2;
             if (__any(top > m[qt] + kSlack)) {
                 const float now = fmaxf(m[qt], top), keep = __builtin_amdgcn_exp2f(m[qt] - (now == -INFINITY ? 0.0f : now));
@@ -283,6 +300,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
                     for (int r = 0; r < 16; ++r) acc[qt][dt][r] *= keep;
             }
             const float base = m[qt] == -INFINITY ? 0.0f : m[qt];
+            const half2_t ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
@@ -290,10 +308,10 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
                 for (int r = 0; r < 16; r += 2) {
                     const float x = __builtin_amdgcn_exp2f(fmaf(s[qt][tt][r], a.scale2, -base)),
                                 y = __builtin_amdgcn_exp2f(fmaf(s[qt][tt][r + 1], a.scale2, -base));
-                    sum[0] += x;
-                    sum[1] += y;
-                    p[qt][tt * 2 + (r >> 3)][r & 7] = static_cast<_Float16>(x);
-                    p[qt][tt * 2 + (r >> 3)][(r & 7) + 1] = static_cast<_Float16>(y);
+                    const half2_t w = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
+                    sum[tt] = __builtin_amdgcn_fdot2(w, ones, sum[tt], false);
+                    p[qt][tt * 2 + (r >> 3)][r & 7] = w[0];
+                    p[qt][tt * 2 + (r >> 3)][(r & 7) + 1] = w[1];
                 }
             l[qt] += sum[0] + sum[1];
         }
@@ -351,22 +369,24 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
 
     std::uint16_t* const tile_k = lds;
     std::uint16_t* const tile_v = lds + 2 * C::TILE;
+    const std::uint32_t to_k = uniform(lds_address(tile_k)), to_v = uniform(lds_address(tile_v));
     if (steps > 0) {
-        stage(k0, a.k_stride, 0, tile_k);
-        stage(v0, a.v_stride, 0, tile_v);
+        stage(k0, a.k_stride, 0, to_k);
+        stage(v0, a.v_stride, 0, to_v);
     }
-    for (int step = 0; step < steps; ++step) {
+    auto turn = [&](int step, auto masked) {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's DMA of the tile
         __syncthreads();
         const int now = step & 1, next = now ^ 1;
         if (step + 1 < steps) {
-            stage(k0, a.k_stride, step + 1, tile_k + next * C::TILE);
-            stage(v0, a.v_stride, step + 1, tile_v + next * C::TILE);
+            stage(k0, a.k_stride, step + 1, to_k + next * C::TILE * 2);
+            stage(v0, a.v_stride, step + 1, to_v + next * C::TILE * 2);
         }
-        const int j1 = step * kKeys + kKeys;
-        if (j1 <= all) compute(step, tile_k + now * C::TILE, tile_v + now * C::TILE, std::false_type{});
-        else if (j1 - kKeys < any) compute(step, tile_k + now * C::TILE, tile_v + now * C::TILE, std::true_type{});
-    }
+        if (!masked || step * kKeys < any) compute(step, tile_k + now * C::TILE, tile_v + now * C::TILE, masked);
+    };
+    int step = 0;
+    for (; step < clear; ++step) turn(step, std::false_type{});
+    for (; step < steps; ++step) turn(step, std::true_type{});
 
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
