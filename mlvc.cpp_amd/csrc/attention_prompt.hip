@@ -97,6 +97,7 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kRawBufferFlags = 0x00020000;
 constexpr int kKeys = 64;          // keys of a tile
+constexpr int kProducts = 0x8, kReads = 0x100;  // instruction groups of sched_group_barrier: MFMA, LDS reads
 constexpr float kSlack = 8.0f;     // how far, in powers of two, a score may pass the running maximum before it moves
 
 __device__ __forceinline__ std::uint32_t uniform(std::uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -153,6 +154,12 @@ struct PromptCfg {
     static constexpr int DMA = kKeys / DMA_ROWS;     // instructions of a tile
     static constexpr int TILE = kKeys * D;           // halves
     static constexpr size_t LDS = 4 * TILE * 2;      // K and V, two buffers
+    // Piece p of row t is kept at place p ^ swizzle(t): 16 rows of one piece
+    // (a K read) fall on all 64 banks, and so do 4 rows of 4 pieces (a V read).
+    __host__ __device__ static constexpr int swizzle(int t)
+    {
+        return D == 128 ? 4 * (t & 3) + (t >> 2 & 3) : 4 * (t >> 1 & 1) + (t >> 2 & 3);
+    }
 };
 
 template <class C>
@@ -210,10 +217,9 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
     const std::int64_t kv = static_cast<std::int64_t>(head / a.group) * D;
     const std::uint16_t* const k0 = a.k + sk.first * a.k_stride + kv;
     const std::uint16_t* const v0 = a.v + sk.first * a.v_stride + kv;
-    // Piece p of row t is kept at place p ^ f(t), f(t) = 2 (t & 3) + (t >> 2 & 1).
     const int drow = lane / C::PIECES, first_row = wave * C::DMA_ROWS + drow;
-    const int piece = (lane % C::PIECES) ^ (2 * (first_row & 3) + (first_row >> 2 & 1));
-    static_assert(C::DMA_ROWS * C::WAVES % 8 == 0 && C::DMA % C::WAVES == 0);
+    const int piece = (lane % C::PIECES) ^ C::swizzle(first_row);  // the same for all of this lane's rows
+    static_assert(C::DMA_ROWS * C::WAVES % 16 == 0 && C::DMA % C::WAVES == 0);
     auto stage = [&](const std::uint16_t* x, std::int64_t stride, int step, std::uint32_t to) {
         const std::uint32_t stride2 = static_cast<std::uint32_t>(stride) * 2u;
         const std::uint64_t p = reinterpret_cast<std::uint64_t>(x + static_cast<std::int64_t>(step) * kKeys * stride);
@@ -225,24 +231,25 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
         for (int i = 0; i < C::DMA / C::WAVES; ++i)
             lds_dma16(r, to + (wave + i * C::WAVES) * 1024, at + i * C::WAVES * C::DMA_ROWS * stride2);
     };
-    // Places of this lane's pieces: K row lane & 31, pieces 2 ks + hi; V rows 4 hi + (lane & 15) / 4 ..., the
-    // transposing read of 16 lanes gives each lane the four rows of one column.
-    const int fk = 2 * (column & 3) + (column >> 2 & 1);
-    int kat[4];
+    // Places of this lane's pieces: of K, pieces 2 ks + hi of row lane & 31; of
+    // V, the transposing read of 16 lanes takes 4 halves of each of 4 rows
+    // (4 hi + 8 e + 0..3 of a 16-row step) a lane and returns one column's four.
+    int kat[KS], vat[DT][2];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) kat[b] = column * D + ((2 * b + hi) ^ fk) * 8;
-    const int vrow = (lane & 15) >> 2, fv = 2 * vrow + hi;
-    int vat[2];
+    for (int ks = 0; ks < KS; ++ks) kat[ks] = column * D + ((2 * ks + hi) ^ C::swizzle(column)) * 8;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-        vat[b] = (4 * hi + vrow) * D + ((4 * b + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ fv) * 8 + (lane & 1) * 4;
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int row = 8 * e + 4 * hi + ((lane & 15) >> 2);
+            vat[dt][e] = row * D + ((4 * dt + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ C::swizzle(row)) * 8 + (lane & 1) * 4;
+        }
     auto value_fragment = [&](const std::uint16_t* tile_v, int step, int dt) {
         u32x2 v[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
             v[e] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                 (__attribute__((address_space(3))) s16x4*)(
-                                                     tile_v + vat[dt & 1] + (dt >> 1) * 64 + (step * 16 + e * 8) * D)));
+                                                 (__attribute__((address_space(3))) s16x4*)(tile_v + vat[dt][e] + step * 16 * D)));
         return u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
     };
 
@@ -260,19 +267,30 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
     auto compute = [&](int step, const std::uint16_t* tile_k, const std::uint16_t* tile_v, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         const int j0 = step * kKeys;
+        // Eight K fragments are read ahead of the products, then one for each
+        // fragment used: an LDS read takes as long as four products.
         floatx16 s[QT][2];
+        half8 kf[2 * KS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            half8 kf[2];
+        for (int i = 0; i < 2 * KS; ++i) kf[i] = *reinterpret_cast<const half8*>(tile_k + kat[i >> 1] + (i & 1) * 32 * D);
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-                kf[tt] = *reinterpret_cast<const half8*>(tile_k + kat[ks & 3] + (ks >> 2) * 64 + tt * 32 * D);
+        for (int i = 0; i < 2 * KS; ++i)
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt)
+                s[qt][i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], q[qt][i >> 1], i > 1 ? s[qt][i & 1] : floatx16{}, 0, 0, 0);
+        __builtin_amdgcn_sched_group_barrier(kReads, 8, 0);
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-                    s[qt][tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[tt], q[qt][ks], ks ? s[qt][tt] : floatx16{}, 0, 0, 0);
+        for (int i = 0; i < 2 * KS - 8; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kProducts, QT, 0);
+            __builtin_amdgcn_sched_group_barrier(kReads, 1, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(kProducts, 8 * QT, 0);
+        // The first step's V fragments come in under the softmax.
+        u32x4 vf[2][DT];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) vf[0][dt] = value_fragment(tile_v, 0, dt);
+        __builtin_amdgcn_sched_barrier(0);
         half8 p[QT][4];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
@@ -320,20 +338,22 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
         for (int st = 0; st < 4; ++st)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                u32x4 vf = value_fragment(tile_v, st, dt);
+                u32x4 v = vf[st & 1][dt];
+                if (st < 3) vf[st & 1 ^ 1][dt] = value_fragment(tile_v, st + 1, dt);
                 if constexpr (MASKED) {
                     // Values whose weight may be zero must be finite: 0 * inf is NaN.
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const std::uint32_t lo = (vf[e] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u,
-                                            up = (vf[e] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
+                        const std::uint32_t lo = (v[e] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u,
+                                            up = (v[e] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
                         odd |= lo | up;
-                        vf[e] &= ~(lo | up);
+                        v[e] &= ~(lo | up);
                     }
                 }
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt)
-                    acc[qt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, vf), p[qt][st], acc[qt][dt], 0, 0, 0);
+                    acc[qt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, v), p[qt][st], acc[qt][dt], 0, 0, 0);
+                if constexpr (!MASKED) __builtin_amdgcn_sched_barrier(0);
             }
         if constexpr (MASKED) {
             // What was left out above: a query that sees an infinity or NaN gets
@@ -446,8 +466,15 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
     constexpr std::int64_t kFarthest = std::int64_t{1} << 23;
     const bool rows = vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride) && vector_rows(d->k, d->k_stride) &&
                       vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f;
-    if (rows && d->head_dim == 128) launch_prompt<PromptCfg<128, 4, 1>>(a, s);
-    else if (rows && d->head_dim == 64) launch_prompt<PromptCfg<64, 4, 1>>(a, s);
+    // 256 queries a workgroup read the keys half as often as 128, and one
+    // such workgroup a CU is as many waves; 8160 tokens, 16 heads of 128: 283
+    // against 301 us. They need work for every CU twice over, and sequences of
+    // like length (packed 1..2040: 68 against 67 us).
+    const std::int64_t large = static_cast<std::int64_t>(d->q_tokens) / 256 * d->q_heads;
+    const bool even = static_cast<std::int64_t>(d->longest_q) * d->sequences <= 2 * static_cast<std::int64_t>(d->q_tokens);
+    const bool eight = even && large >= 2 * conv::cu_count() - d->q_heads;
+    if (rows && d->head_dim == 128) eight ? launch_prompt<PromptCfg<128, 8, 1>>(a, s) : launch_prompt<PromptCfg<128, 4, 1>>(a, s);
+    else if (rows && d->head_dim == 64) eight ? launch_prompt<PromptCfg<64, 8, 1>>(a, s) : launch_prompt<PromptCfg<64, 4, 1>>(a, s);
     else
         prompt_any_kernel<<<dim3(static_cast<unsigned>(d->q_tokens), static_cast<unsigned>(d->q_heads)), 64, 0, s>>>(a);
     check(hipGetLastError(), "attention_prompt launch");
