@@ -9,6 +9,7 @@
 
 #include "attention.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace mlvc_hip {
@@ -128,32 +129,36 @@ __device__ __forceinline__ float both_sum(float x)
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Heads of D values, rows on 16 bytes. A workgroup of WAVES waves takes
-// WAVES * QT * 32 queries of a head; a wave holds QT * 32 of them as columns
-// of S^T = K Q^T (32x32x16 products, keys as rows), so that
+// Heads of D values, rows on 16 bytes. A workgroup of RG x KG waves takes
+// RG * 32 queries of a head. A wave holds 32 of them as columns of S^T = K Q^T
+// (32x32x16 products, keys as rows), so that
 //   * a lane's scores all belong to one query: the softmax needs one exchange,
 //     between the two lanes of a column;
 //   * the accumulator registers of S^T, rounded to FP16, are the B operand of
 //     O^T += V^T P^T as they stand (the 16 keys of a step are taken in the order
 //     the registers hold them), so weights never leave the lane.
-// Tiles of 64 keys are staged by LDS DMA, double-buffered, 16-byte pieces of a
-// row permuted (piece ^ f(row)) so that both reads are free of bank conflicts:
-// K rows by 16 bytes, V by the transposing read. Rows past a sequence's end are
+// The KG groups of waves take every KG-th tile of 64 keys and are put together
+// in LDS at the end: more waves where there are too few queries to fill the GPU.
+//
+// Tiles are staged by LDS DMA into NBUF buffers, 16-byte pieces of a row
+// permuted (piece ^ f(row)) so that both reads are free of bank conflicts: K
+// rows by 16 bytes, V by the transposing read. Rows past a sequence's end are
 // out of the buffer's range and read as zeros.
 //
 // The running maximum moves only when a score passes it by 2^8 (weights up to
 // 2^8 lose nothing in FP16 or in the FP32 sums), so the accumulators are seldom
 // rescaled. Weights are rounded to FP16, the type the matrix cores take beside
 // V: one rounding of 2^-11 each, no more than the output's own.
-template <int D_, int WAVES_, int QT_>
+template <int D_, int RG_, int KG_, int NBUF_, int OCC_>
 struct PromptCfg {
-    static constexpr int D = D_, WAVES = WAVES_, QT = QT_;
-    static constexpr int ROWS = WAVES * QT * 32;     // queries of a workgroup
+    static constexpr int D = D_, RG = RG_, KG = KG_, NBUF = NBUF_, OCC = OCC_;
+    static constexpr int WAVES = RG * KG;
+    static constexpr int ROWS = RG * 32;             // queries of a workgroup
     static constexpr int PIECES = D / 8;             // 16-byte pieces of a row
     static constexpr int DMA_ROWS = 64 / PIECES;     // rows of a DMA instruction
     static constexpr int DMA = kKeys / DMA_ROWS;     // instructions of a tile
     static constexpr int TILE = kKeys * D;           // halves
-    static constexpr size_t LDS = 4 * TILE * 2;      // K and V, two buffers
+    static constexpr size_t LDS = static_cast<size_t>(KG) * NBUF * 2 * TILE * 2;  // K and V
     // Piece p of row t is kept at place p ^ swizzle(t): 16 rows of one piece
     // (a K read) fall on all 64 banks, and so do 4 rows of 4 pieces (a V read).
     __host__ __device__ static constexpr int swizzle(int t)
@@ -163,12 +168,12 @@ struct PromptCfg {
 };
 
 template <class C>
-__global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, int tiles)
+__global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArgs a, int tiles)
 {
-    constexpr int D = C::D, QT = C::QT, KS = D / 16, DT = D / 32;
+    constexpr int D = C::D, KS = D / 16, DT = D / 32;
     extern __shared__ __attribute__((aligned(16))) std::uint16_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int column = lane & 31, hi = lane >> 5;
+    const int row_group = wave % C::RG, key_group = wave / C::RG, column = lane & 31, hi = lane >> 5;
 
     // Workgroup i runs on XCD i % 8: with a multiple of 8 heads an XCD keeps the
     // same heads, of all sequences, so their keys stay in its L2. The last
@@ -194,42 +199,40 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
     const int steps = (keys + kKeys - 1) / kKeys;
 
     // This wave's queries, as B fragments.
-    const int w0 = q0 + wave * QT * 32;
-    half8 q[QT][KS];
-    int seen[QT];  // keys this lane's query sees
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        const int i = w0 + qt * 32 + column, at = min(i, nq - 1);
-        const std::uint16_t* row = a.q + (sq.first + at) * a.q_stride + static_cast<std::int64_t>(head) * D + hi * 8;
+    const int w0 = q0 + row_group * 32, i_query = w0 + column, at_query = min(i_query, nq - 1);
+    half8 q[KS];
+    {
+        const std::uint16_t* row = a.q + (sq.first + at_query) * a.q_stride + static_cast<std::int64_t>(head) * D + hi * 8;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             u32x4 v = *reinterpret_cast<const u32x4*>(row + ks * 16);
             if (a.negate)
                 for (int e = 0; e < 4; ++e) v[e] ^= 0x80008000u;
-            q[qt][ks] = __builtin_bit_cast(half8, v);
+            q[ks] = __builtin_bit_cast(half8, v);
         }
-        seen[qt] = a.causal ? max(0, min(sk.count, behind + at + 1)) : sk.count;
     }
+    const int seen = a.causal ? max(0, min(sk.count, behind + at_query + 1)) : sk.count;  // keys this lane's query sees
     // Tiles that every query of the workgroup sees whole, and keys that any of this wave's sees.
     const int clear = (a.causal ? max(0, min(sk.count, behind + q0 + 1)) : sk.count) / kKeys;
-    const int any = w0 >= nq ? 0 : a.causal ? max(0, min(sk.count, behind + min(w0 + QT * 32, nq))) : sk.count;
+    const int any = w0 >= nq ? 0 : a.causal ? max(0, min(sk.count, behind + min(w0 + 32, nq))) : sk.count;
 
     const std::int64_t kv = static_cast<std::int64_t>(head / a.group) * D;
     const std::uint16_t* const k0 = a.k + sk.first * a.k_stride + kv;
     const std::uint16_t* const v0 = a.v + sk.first * a.v_stride + kv;
-    const int drow = lane / C::PIECES, first_row = wave * C::DMA_ROWS + drow;
-    const int piece = (lane % C::PIECES) ^ C::swizzle(first_row);  // the same for all of this lane's rows
-    static_assert(C::DMA_ROWS * C::WAVES % 16 == 0 && C::DMA % C::WAVES == 0);
+    // A tile's DMA instructions are dealt to the waves of its group.
+    const int first_row = row_group * C::DMA_ROWS + lane / C::PIECES;
     auto stage = [&](const std::uint16_t* x, std::int64_t stride, int step, std::uint32_t to) {
         const std::uint32_t stride2 = static_cast<std::uint32_t>(stride) * 2u;
         const std::uint64_t p = reinterpret_cast<std::uint64_t>(x + static_cast<std::int64_t>(step) * kKeys * stride);
         const int rows = min(kKeys, sk.count - step * kKeys);
         const u32x4 r = {uniform(static_cast<std::uint32_t>(p)), uniform(static_cast<std::uint32_t>(p >> 32)) & 0xffffu,
                          uniform((rows - 1) * stride2 + 2u * D), kRawBufferFlags};
-        const std::uint32_t at = first_row * stride2 + piece * 16u;
 #pragma unroll
-        for (int i = 0; i < C::DMA / C::WAVES; ++i)
-            lds_dma16(r, to + (wave + i * C::WAVES) * 1024, at + i * C::WAVES * C::DMA_ROWS * stride2);
+        for (int i = 0; i < (C::DMA + C::RG - 1) / C::RG; ++i) {
+            if (C::DMA % C::RG != 0 && row_group + i * C::RG >= C::DMA) continue;
+            const int t = first_row + i * C::RG * C::DMA_ROWS;
+            lds_dma16(r, to + (row_group + i * C::RG) * 1024, t * stride2 + ((lane % C::PIECES) ^ C::swizzle(t)) * 16u);
+        }
     };
     // Places of this lane's pieces: of K, pieces 2 ks + hi of row lane & 31; of
     // V, the transposing read of 16 lanes takes 4 halves of each of 4 rows
@@ -253,85 +256,86 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
         return u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
     };
 
-    floatx16 acc[QT][DT];
-    float m[QT], l[QT];
+    floatx16 acc[DT];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        m[qt] = -INFINITY, l[qt] = 0.0f;
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[qt][dt][r] = 0.0f;
-    }
+        for (int r = 0; r < 16; ++r) acc[dt][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
 
     auto compute = [&](int step, const std::uint16_t* tile_k, const std::uint16_t* tile_v, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         const int j0 = step * kKeys;
         // Eight K fragments are read ahead of the products, then one for each
         // fragment used: an LDS read takes as long as four products.
-        floatx16 s[QT][2];
+        floatx16 s[2];
         half8 kf[2 * KS];
 #pragma unroll
         for (int i = 0; i < 2 * KS; ++i) kf[i] = *reinterpret_cast<const half8*>(tile_k + kat[i >> 1] + (i & 1) * 32 * D);
 #pragma unroll
         for (int i = 0; i < 2 * KS; ++i)
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-                s[qt][i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], q[qt][i >> 1], i > 1 ? s[qt][i & 1] : floatx16{}, 0, 0, 0);
+            s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], q[i >> 1], i > 1 ? s[i & 1] : floatx16{}, 0, 0, 0);
         __builtin_amdgcn_sched_group_barrier(kReads, 8, 0);
 #pragma unroll
         for (int i = 0; i < 2 * KS - 8; ++i) {
-            __builtin_amdgcn_sched_group_barrier(kProducts, QT, 0);
+            __builtin_amdgcn_sched_group_barrier(kProducts, 1, 0);
             __builtin_amdgcn_sched_group_barrier(kReads, 1, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(kProducts, 8 * QT, 0);
+        __builtin_amdgcn_sched_group_barrier(kProducts, 8, 0);
         // The first step's V fragments come in under the softmax.
         u32x4 vf[2][DT];
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) vf[0][dt] = value_fragment(tile_v, 0, dt);
         __builtin_amdgcn_sched_barrier(0);
-        half8 p[QT][4];
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
+        half8 p[4];
+        {
             if constexpr (MASKED) {
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (j0 + tt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen[qt]) s[qt][tt][r] = -INFINITY;
+                        if (j0 + tt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen) s[tt][r] = -INFINITY;
             }
             // The NaN-propagating maximum of three is one instruction; a score that
             // is NaN leaves the maximum where it was, and its query becomes NaN.
-            float top = __builtin_elementwise_maximum(s[qt][0][0], s[qt][1][0]);
+            float tops[2];
 #pragma unroll
-            for (int r = 1; r < 16; ++r)
-                top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[qt][0][r]), s[qt][1][r]);
+            for (int tt = 0; tt < 2; ++tt) {
+                tops[tt] = s[tt][0];
+#pragma unroll
+                for (int r = 1; r < 15; r += 2)
+                    tops[tt] = __builtin_elementwise_maximum(__builtin_elementwise_maximum(tops[tt], s[tt][r]), s[tt][r + 1]);
+            }
+            float top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(tops[0], s[0][15]),
+                                                      __builtin_elementwise_maximum(tops[1], s[1][15]));
             top = both_max(top) * a.scale2;
-            if (__any(top > m[qt] + kSlack)) {
-                const float now = fmaxf(m[qt], top), keep = __builtin_amdgcn_exp2f(m[qt] - (now == -INFINITY ? 0.0f : now));
-                m[qt] = now;
-                l[qt] *= keep;
+            if (__any(top > m + kSlack)) {
+                const float now = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
+                m = now;
+                l *= keep;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[qt][dt][r] *= keep;
+                    for (int r = 0; r < 16; ++r) acc[dt][r] *= keep;
             }
-            const float base = m[qt] == -INFINITY ? 0.0f : m[qt];
-            const half2_t ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-            float sum[2] = {0.0f, 0.0f};
+            const float base = m == -INFINITY ? 0.0f : m;
+            // Plain additions: the dot-product instructions share the matrix cores'
+            // pipe, and take 26 cycles instead of 5 beside another wave's products.
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[qt][tt][r], a.scale2, -base)),
-                                y = __builtin_amdgcn_exp2f(fmaf(s[qt][tt][r + 1], a.scale2, -base));
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[tt][r], a.scale2, -base)),
+                                y = __builtin_amdgcn_exp2f(fmaf(s[tt][r + 1], a.scale2, -base));
                     const half2_t w = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
-                    sum[tt] = __builtin_amdgcn_fdot2(w, ones, sum[tt], false);
-                    p[qt][tt * 2 + (r >> 3)][r & 7] = w[0];
-                    p[qt][tt * 2 + (r >> 3)][(r & 7) + 1] = w[1];
+                    sum[2 * tt] += x;
+                    sum[2 * tt + 1] += y;
+                    p[tt * 2 + (r >> 3)][r & 7] = w[0];
+                    p[tt * 2 + (r >> 3)][(r & 7) + 1] = w[1];
                 }
-            l[qt] += sum[0] + sum[1];
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         std::uint32_t odd = 0;
 #pragma unroll
@@ -350,9 +354,7 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
                         v[e] &= ~(lo | up);
                     }
                 }
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-                    acc[qt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, v), p[qt][st], acc[qt][dt], 0, 0, 0);
+                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, v), p[st], acc[dt], 0, 0, 0);
                 if constexpr (!MASKED) __builtin_amdgcn_sched_barrier(0);
             }
         if constexpr (MASKED) {
@@ -360,8 +362,6 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
             // it. Counted by products of 0 / 1 matrices, once for +inf and NaN,
             // once for -inf and NaN.
             if (__any(odd != 0)) {
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt)
                         for (int sign = 0; sign < 2; ++sign) {
@@ -375,53 +375,88 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void prompt_kernel(PromptArgs a, 
                                     const bool bad = (v & 0x7fffu) > 0x7c00u || v == (sign ? 0xfc00u : 0x7c00u);
                                     is[e] = static_cast<_Float16>(bad ? 1.0f : 0.0f);
                                     const int j = j0 + st * 16 + 8 * (e >> 2) + 4 * hi + (e & 3);
-                                    sees[e] = static_cast<_Float16>(j < seen[qt] ? 1.0f : 0.0f);
+                                    sees[e] = static_cast<_Float16>(j < seen ? 1.0f : 0.0f);
                                 }
                                 count = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, count, 0, 0, 0);
                             }
 #pragma unroll
                             for (int r = 0; r < 16; ++r)
-                                if (count[r] > 0.0f) acc[qt][dt][r] += sign ? -INFINITY : INFINITY;
+                                if (count[r] > 0.0f) acc[dt][r] += sign ? -INFINITY : INFINITY;
                         }
             }
         }
     };
 
-    std::uint16_t* const tile_k = lds;
-    std::uint16_t* const tile_v = lds + 2 * C::TILE;
-    const std::uint32_t to_k = uniform(lds_address(tile_k)), to_v = uniform(lds_address(tile_v));
-    if (steps > 0) {
-        stage(k0, a.k_stride, 0, to_k);
-        stage(v0, a.v_stride, 0, to_v);
-    }
-    auto turn = [&](int step, auto masked) {
+    // This group's buffers: K and V of one tile, then of the next.
+    std::uint16_t* const tiles_of_group = lds + key_group * C::NBUF * 2 * C::TILE;
+    const std::uint32_t to = uniform(lds_address(tiles_of_group));
+    auto stage_both = [&](int step, int buffer) {
+        stage(k0, a.k_stride, step, to + buffer * C::TILE * 4);
+        stage(v0, a.v_stride, step, to + buffer * C::TILE * 4 + C::TILE * 2);
+    };
+    if (key_group < steps) stage_both(key_group, 0);
+    auto turn = [&](int step, int buffer, auto masked) {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's DMA of the tile
         __syncthreads();
-        const int now = step & 1, next = now ^ 1;
-        if (step + 1 < steps) {
-            stage(k0, a.k_stride, step + 1, to_k + next * C::TILE * 2);
-            stage(v0, a.v_stride, step + 1, to_v + next * C::TILE * 2);
+        if (C::NBUF == 2 && step + C::KG < steps) stage_both(step + C::KG, buffer ^ 1);
+        const std::uint16_t* const tile = tiles_of_group + buffer * 2 * C::TILE;
+        if (!masked || step * kKeys < any) compute(step, tile, tile + C::TILE, masked);
+        if (C::NBUF == 1) {
+            __syncthreads();
+            if (step + C::KG < steps) stage_both(step + C::KG, 0);
         }
-        if (!masked || step * kKeys < any) compute(step, tile_k + now * C::TILE, tile_v + now * C::TILE, masked);
     };
-    int step = 0;
-    for (; step < clear; ++step) turn(step, std::false_type{});
-    for (; step < steps; ++step) turn(step, std::true_type{});
+    // All groups take as many turns; `any` is at most `steps` tiles.
+    int round = 0, buffer = 0;
+    for (; (round + 1) * C::KG <= clear; ++round, buffer ^= C::NBUF - 1) turn(round * C::KG + key_group, buffer, std::false_type{});
+    for (; round * C::KG < steps; ++round, buffer ^= C::NBUF - 1) turn(round * C::KG + key_group, buffer, std::true_type{});
 
+    if constexpr (C::KG > 1) {
+        // The other groups hand their states to the first, lane by lane.
+        constexpr int kWords = DT * 4 + 1, kLanes = C::RG * 64;
+        static_assert(sizeof(floatx4) * kWords * kLanes * (C::KG - 1) <= C::LDS);
+        floatx4* const states = reinterpret_cast<floatx4*>(lds) + row_group * 64 + lane;
+        __syncthreads();
+        if (key_group > 0) {
+            floatx4* const to_state = states + (key_group - 1) * kWords * kLanes;
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        const int i = w0 + qt * 32 + column;
-        const float sum = both_sum(l[qt]), r = sum == 0.0f ? 0.0f : 1.0f / sum;
-        if (i >= nq) continue;
-        std::uint16_t* out = a.out + (sq.first + i) * a.out_stride + static_cast<std::int64_t>(head) * D + 4 * hi;
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+                for (int g = 0; g < 4; ++g)
+                    to_state[(dt * 4 + g) * kLanes] = floatx4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+            to_state[DT * 4 * kLanes] = floatx4{m, l, 0.0f, 0.0f};
+        }
+        __syncthreads();
+        if (key_group > 0) return;
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<uint2*>(out + dt * 32 + 8 * g) =
-                    make_uint2(pack_rounded(acc[qt][dt][4 * g] * r, acc[qt][dt][4 * g + 1] * r),
-                               pack_rounded(acc[qt][dt][4 * g + 2] * r, acc[qt][dt][4 * g + 3] * r));
+        for (int k = 0; k < C::KG - 1; ++k) {
+            const floatx4* const from = states + k * kWords * kLanes;
+            const floatx4 st = from[DT * 4 * kLanes];
+            const float now = fmaxf(m, st[0]), base = now == -INFINITY ? 0.0f : now;
+            const float mine = __builtin_amdgcn_exp2f(m - base), other = __builtin_amdgcn_exp2f(st[0] - base);
+            m = now;
+            l = l * mine + st[1] * other;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const floatx4 v = from[(dt * 4 + g) * kLanes];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[dt][4 * g + e] = acc[dt][4 * g + e] * mine + v[e] * other;
+                }
+        }
     }
+
+    const float sum = both_sum(l), r = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (i_query >= nq) return;
+    std::uint16_t* out = a.out + (sq.first + i_query) * a.out_stride + static_cast<std::int64_t>(head) * D + 4 * hi;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2*>(out + dt * 32 + 8 * g) =
+                make_uint2(pack_rounded(acc[dt][4 * g] * r, acc[dt][4 * g + 1] * r),
+                           pack_rounded(acc[dt][4 * g + 2] * r, acc[dt][4 * g + 3] * r));
 }
 
 template <class C>
@@ -431,6 +466,42 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
     const std::int64_t grid = static_cast<std::int64_t>(tiles) * a.q_heads * a.sequences;
     require(grid <= INT_MAX, "attention_prompt", "too many sequences, heads and queries in one call");
     prompt_kernel<C><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles);
+}
+
+// Workgroups of 128 queries, two a CU, read each key tile once for 128 queries
+// and balance well; they need two of them for every CU. Fewer queries are
+// given more waves by key groups, at first beside as many queries, then fewer.
+// us, the same work by the alternatives (16 query heads, causal):
+//   heads of 128          (4,1)  (4,2)  (2,4)  (1,4)  (8,1)
+//     240                  11.8   13.0   11.8    9.6   18.3
+//     920                  23.0   21.2   17.9   23.4   30.8
+//     2040                 43.8   36.2   38.6   62.0   59.6
+//     4080                 95.2   87.4    116    184    113
+//     1..2040 packed       61.4   79.7    124    193   65.1
+//     4 x 2040             87.8    105    159    264   91.9
+//     8160                  302    296    399    661    281
+//   heads of 64           (4,1)  (4,2)  (4,3)  (2,4)  (1,4)
+//     240                   9.2    9.0   11.4    8.0    7.2
+//     920                  17.2   14.7   16.1   11.2   15.5
+//     920 on 4600, 460 on 3001  62.5  47.5  44.5  54.4  95.9
+//     8160                  176    184    188    218    372
+// 256 queries a workgroup halve the key traffic again, which pays where a
+// sequence is long enough for its last, partly seen tiles not to count.
+template <int D>
+void launch_prompt(const PromptArgs& a, hipStream_t s)
+{
+    const std::int64_t cus = conv::cu_count();
+    auto workgroups = [&](int queries) {  // at most, from what the host knows
+        const std::int64_t by_longest = static_cast<std::int64_t>((a.longest_q + queries - 1) / queries) * a.sequences;
+        return a.q_heads * std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / queries) + a.sequences);
+    };
+    if (workgroups(32) <= cus) launch_prompt<PromptCfg<D, 1, 4, D == 64 ? 2 : 1, 1>>(a, s);
+    else if (workgroups(64) <= cus) launch_prompt<PromptCfg<D, 2, 4, D == 64 ? 2 : 1, 2>>(a, s);
+    else if (D == 64 && workgroups(128) <= cus) launch_prompt<PromptCfg<64, 4, 3, 2, 3>>(a, s);
+    else if (workgroups(128) <= 2 * cus) launch_prompt<PromptCfg<D, 4, 2, 2, 2>>(a, s);
+    else if (D == 128 && a.longest_q >= 4096 && workgroups(128) >= 4 * cus && static_cast<std::int64_t>(a.longest_q) * a.sequences <= 2 * static_cast<std::int64_t>(a.q_tokens))
+        launch_prompt<PromptCfg<128, 8, 1, 2, 2>>(a, s);
+    else launch_prompt<PromptCfg<D, 4, 1, 2, D == 64 ? 3 : 2>>(a, s);
 }
 
 void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
@@ -466,15 +537,8 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
     constexpr std::int64_t kFarthest = std::int64_t{1} << 23;
     const bool rows = vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride) && vector_rows(d->k, d->k_stride) &&
                       vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f;
-    // 256 queries a workgroup read the keys half as often as 128, and one
-    // such workgroup a CU is as many waves; 8160 tokens, 16 heads of 128: 283
-    // against 301 us. They need work for every CU twice over, and sequences of
-    // like length (packed 1..2040: 68 against 67 us).
-    const std::int64_t large = static_cast<std::int64_t>(d->q_tokens) / 256 * d->q_heads;
-    const bool even = static_cast<std::int64_t>(d->longest_q) * d->sequences <= 2 * static_cast<std::int64_t>(d->q_tokens);
-    const bool eight = even && large >= 2 * conv::cu_count() - d->q_heads;
-    if (rows && d->head_dim == 128) eight ? launch_prompt<PromptCfg<128, 8, 1>>(a, s) : launch_prompt<PromptCfg<128, 4, 1>>(a, s);
-    else if (rows && d->head_dim == 64) eight ? launch_prompt<PromptCfg<64, 8, 1>>(a, s) : launch_prompt<PromptCfg<64, 4, 1>>(a, s);
+    if (rows && d->head_dim == 128) launch_prompt<128>(a, s);
+    else if (rows && d->head_dim == 64) launch_prompt<64>(a, s);
     else
         prompt_any_kernel<<<dim3(static_cast<unsigned>(d->q_tokens), static_cast<unsigned>(d->q_heads)), 64, 0, s>>>(a);
     check(hipGetLastError(), "attention_prompt launch");

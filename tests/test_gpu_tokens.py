@@ -401,3 +401,59 @@ def test_token_step_captured(dev, rng):
     finally:
         dev.check(lib.mlvc_hip_graph_destroy(graph))
         dev.check(lib.mlvc_hip_stream_destroy(stream))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("queries,keys,q_heads", [
+    ([130], [130], 64), ([97, 1, 64], [210, 7, 64], 64),       # a few queries a workgroup, keys in four groups
+    ([261], [261], 64), ([200, 77], [333, 50], 64),            # 128 queries, keys in groups
+    ([530], [700], 64), ([1100, 3], [1100, 65], 64),           # 128 queries, one group and several
+    ([4100], [4100], 32), ([4100], [4300], 32),                # 256 queries
+])
+def test_prompt_tiles(dev, rng, queries, keys, q_heads, dim, causal):
+    """Sizes for every tile shape: a sample of the queries, with the first and last of each sequence."""
+    q = normal(rng, sum(queries), q_heads, dim)
+    k, v = (normal(rng, sum(keys), 2, dim) for _ in range(2))
+    got = Prompt(dev, q, k, v, queries, keys, causal, dim ** -0.5).run()
+    assert np.isfinite(got).all()
+    i = j = 0
+    for nq, nk in zip(queries, keys):
+        rows = np.unique(np.r_[0, nq - 1, rng.integers(0, nq, 8)])
+        heads = rng.permutation(q_heads)[:4]
+        for r in rows:
+            n = min(nk, max(0, nk - nq + r + 1)) if causal else nk
+            for h in heads:
+                g = h // (q_heads // 2)
+                want, tol = attend64(f64(q[i + r:i + r + 1, h:h + 1]), f64(k[j:j + n, g:g + 1]), f64(v[j:j + n, g:g + 1]),
+                                     dim ** -0.5, False)
+                within(got[i + r:i + r + 1, h:h + 1], want, tol, f"query {r} of {nq} on {nk}, head {h}")
+        i, j = i + nq, j + nk
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n,q_heads", [(130, 64), (261, 64), (530, 64), (1100, 64)])
+def test_prompt_tiles_unseen_rows(dev, rng, n, q_heads, dim):
+    """A value that is not finite reaches the queries from its place on, in every tile shape."""
+    q, k, v = normal(rng, n, q_heads, dim), normal(rng, n, 1, dim), normal(rng, n, 1, dim)
+    bad = {n - 2: np.nan, n // 2: np.inf, n // 2 + 1: -np.inf}
+    for at, x in bad.items():
+        v[at, 0, at % dim] = x
+    got = Prompt(dev, q, k, v, [n], [n], True, dim ** -0.5).run()
+    for column in {at % dim for at in bad}:
+        at = min(a for a in bad if a % dim == column)  # two of them may share a column
+        assert np.isfinite(got[:at, :, column]).all() and not np.isfinite(got[at:, :, column]).any()
+    columns = np.setdiff1d(np.arange(dim), [at % dim for at in bad])
+    assert np.isfinite(got[:, :, columns]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,dim,lengths", [
+    (2, 64, [0, 30000, 1, 700]),          # one stream in many shares, others inside one
+    (1, 128, [40] * 100 + [2000]),        # more streams than a wave has lanes, many in a share
+    (4, 64, [2048, 4096, 8192, 0, 5]),    # shares that end where streams do
+])
+def test_tokens_shares(dev, rng, kind, heads, dim, lengths):
+    cache, table, ks, vs = _streams(dev, rng, kind, lengths, heads, dim, 64)
+    q = normal(rng, len(lengths), 2 * heads, dim)
+    _check_tokens(Token(cache, q, table, lengths, dim ** -0.5).run(), q, ks, vs, lengths, dim ** -0.5)
