@@ -45,16 +45,16 @@ struct RowsArgs {
     std::uint16_t* x[2];
     std::int64_t stride[2];
     const std::int32_t* slots;
-    std::int64_t rows;       // tokens * heads
+    unsigned rows;           // tokens * heads
     int heads, dim, page, slot_count;
 };
 
 // Row of the cache (of all its heads' rows) that a token's head goes to, or -1.
-__device__ __forceinline__ std::int64_t cache_row(const RowsArgs& a, std::int64_t token, int head)
+__device__ __forceinline__ std::int64_t cache_row(const RowsArgs& a, unsigned token, int head)
 {
     const std::int32_t slot = a.slots[token];
     if (slot < 0 || slot >= a.slot_count) return -1;
-    const int page = slot / a.page;
+    const int page = static_cast<int>(static_cast<unsigned>(slot) / static_cast<unsigned>(a.page));
     return (static_cast<std::int64_t>(page) * a.heads + head) * a.page + (slot - page * a.page);
 }
 
@@ -116,9 +116,9 @@ template <int KIND, int LANES>
 __global__ __launch_bounds__(kBlock) void kv_write_kernel(RowsArgs a)
 {
     const int of = blockIdx.y, lane = threadIdx.x % LANES, d0 = lane * 8;
-    const std::int64_t row = blockIdx.x * static_cast<std::int64_t>(kBlock / LANES) + threadIdx.x / LANES;
+    const unsigned row = blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
     if (row >= a.rows) return;
-    const std::int64_t token = row / a.heads;
+    const unsigned token = row / static_cast<unsigned>(a.heads);
     const int head = static_cast<int>(row - token * a.heads);
     const bool mine = d0 < a.dim;
     u32x4 v = {0, 0, 0, 0};
@@ -147,9 +147,9 @@ template <int KIND, int LANES>
 __global__ __launch_bounds__(kBlock) void kv_read_kernel(RowsArgs a)
 {
     const int of = blockIdx.y, lane = threadIdx.x % LANES, d0 = lane * 8;
-    const std::int64_t row = blockIdx.x * static_cast<std::int64_t>(kBlock / LANES) + threadIdx.x / LANES;
+    const unsigned row = blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
     if (row >= a.rows || d0 >= a.dim) return;
-    const std::int64_t token = row / a.heads;
+    const unsigned token = row / static_cast<unsigned>(a.heads);
     const int head = static_cast<int>(row - token * a.heads);
     const std::int64_t from = cache_row(a, token, head);
     u32x4 v = {0, 0, 0, 0};
@@ -174,9 +174,9 @@ template <int KIND, bool WRITE>
 __global__ __launch_bounds__(kBlock) void kv_any_kernel(RowsArgs a)
 {
     const int of = blockIdx.y, lane = threadIdx.x & 63;
-    const std::int64_t row = blockIdx.x * static_cast<std::int64_t>(kBlock / 64) + (threadIdx.x >> 6);
+    const unsigned row = blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
     if (row >= a.rows) return;
-    const std::int64_t token = row / a.heads;
+    const unsigned token = row / static_cast<unsigned>(a.heads);
     const int head = static_cast<int>(row - token * a.heads);
     std::uint16_t* x = a.x[of] + token * a.stride[of] + static_cast<std::int64_t>(head) * a.dim;
     const std::int64_t at = cache_row(a, token, head);
@@ -237,9 +237,10 @@ void run(const mlvc_hip_kv_cache* c, const mlvc_hip_kv_rows* r, hipStream_t s)
     a.x[0] = static_cast<std::uint16_t*>(r->k), a.x[1] = static_cast<std::uint16_t*>(r->v);
     a.stride[0] = r->k_stride, a.stride[1] = r->v_stride;
     a.slots = r->slots;
-    a.rows = static_cast<std::int64_t>(r->tokens) * c->heads;
+    const std::int64_t rows = static_cast<std::int64_t>(r->tokens) * c->heads;
+    require(rows <= INT_MAX, op, "too many rows in one call");
+    a.rows = static_cast<unsigned>(rows);
     a.heads = c->heads, a.dim = c->head_dim, a.page = c->page_size, a.slot_count = c->pages * c->page_size;
-    require((a.rows + 3) / 4 <= INT_MAX, op, "too many rows in one call");
     const bool vectors = c->head_dim > 32 && c->head_dim <= 256 && vector_rows(r->k, r->k_stride) && vector_rows(r->v, r->v_stride);
     if (c->kind == MLVC_KV_F16) launch<MLVC_KV_F16, WRITE>(a, vectors, s);
     else if (c->kind == MLVC_KV_E4M3) launch<MLVC_KV_E4M3, WRITE>(a, vectors, s);
