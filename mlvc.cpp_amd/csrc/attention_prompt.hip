@@ -97,7 +97,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kRawBufferFlags = 0x00020000;
-constexpr int kKeys = 64;          // keys of a tile
 constexpr int kProducts = 0x8, kReads = 0x100;  // instruction groups of sched_group_barrier: MFMA, LDS reads
 constexpr float kSlack = 8.0f;     // how far, in powers of two, a score may pass the running maximum before it moves
 
@@ -137,10 +136,10 @@ __device__ __forceinline__ float both_sum(float x)
 //   * the accumulator registers of S^T, rounded to FP16, are the B operand of
 //     O^T += V^T P^T as they stand (the 16 keys of a step are taken in the order
 //     the registers hold them), so weights never leave the lane.
-// The KG groups of waves take every KG-th tile of 64 keys and are put together
+// The KG groups of waves take every KG-th tile of KEYS keys and are put together
 // in LDS at the end: more waves where there are too few queries to fill the GPU.
 //
-// Tiles are staged by LDS DMA into NBUF buffers, 16-byte pieces of a row
+// Tiles are staged by LDS DMA, double-buffered, 16-byte pieces of a row
 // permuted (piece ^ f(row)) so that both reads are free of bank conflicts: K
 // rows by 16 bytes, V by the transposing read. Rows past a sequence's end are
 // out of the buffer's range and read as zeros.
@@ -149,16 +148,16 @@ __device__ __forceinline__ float both_sum(float x)
 // 2^8 lose nothing in FP16 or in the FP32 sums), so the accumulators are seldom
 // rescaled. Weights are rounded to FP16, the type the matrix cores take beside
 // V: one rounding of 2^-11 each, no more than the output's own.
-template <int D_, int RG_, int KG_, int NBUF_, int OCC_>
+template <int D_, int RG_, int KG_, int KEYS_, int OCC_>
 struct PromptCfg {
-    static constexpr int D = D_, RG = RG_, KG = KG_, NBUF = NBUF_, OCC = OCC_;
+    static constexpr int D = D_, RG = RG_, KG = KG_, KEYS = KEYS_, OCC = OCC_;
     static constexpr int WAVES = RG * KG;
     static constexpr int ROWS = RG * 32;             // queries of a workgroup
     static constexpr int PIECES = D / 8;             // 16-byte pieces of a row
     static constexpr int DMA_ROWS = 64 / PIECES;     // rows of a DMA instruction
-    static constexpr int DMA = kKeys / DMA_ROWS;     // instructions of a tile
-    static constexpr int TILE = kKeys * D;           // halves
-    static constexpr size_t LDS = static_cast<size_t>(KG) * NBUF * 2 * TILE * 2;  // K and V
+    static constexpr int DMA = KEYS / DMA_ROWS;      // instructions of a tile
+    static constexpr int TILE = KEYS * D;            // halves
+    static constexpr size_t LDS = static_cast<size_t>(KG) * 2 * 2 * TILE * 2;  // two buffers of K and V
     // Piece p of row t is kept at place p ^ swizzle(t): 16 rows of one piece
     // (a K read) fall on all 64 banks, and so do 4 rows of 4 pieces (a V read).
     __host__ __device__ static constexpr int swizzle(int t)
@@ -170,7 +169,7 @@ struct PromptCfg {
 template <class C>
 __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArgs a, int tiles)
 {
-    constexpr int D = C::D, KS = D / 16, DT = D / 32;
+    constexpr int D = C::D, KS = D / 16, DT = D / 32, kKeys = C::KEYS, TT = kKeys / 32;
     extern __shared__ __attribute__((aligned(16))) std::uint16_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row_group = wave % C::RG, key_group = wave / C::RG, column = lane & 31, hi = lane >> 5;
@@ -268,47 +267,48 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
         const int j0 = step * kKeys;
         // Eight K fragments are read ahead of the products, then one for each
         // fragment used: an LDS read takes as long as four products.
-        floatx16 s[2];
-        half8 kf[2 * KS];
+        floatx16 s[TT];
+        half8 kf[TT * KS];
 #pragma unroll
-        for (int i = 0; i < 2 * KS; ++i) kf[i] = *reinterpret_cast<const half8*>(tile_k + kat[i >> 1] + (i & 1) * 32 * D);
+        for (int i = 0; i < TT * KS; ++i) kf[i] = *reinterpret_cast<const half8*>(tile_k + kat[i / TT] + i % TT * 32 * D);
 #pragma unroll
-        for (int i = 0; i < 2 * KS; ++i)
-            s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], q[i >> 1], i > 1 ? s[i & 1] : floatx16{}, 0, 0, 0);
-        __builtin_amdgcn_sched_group_barrier(kReads, 8, 0);
+        for (int i = 0; i < TT * KS; ++i)
+            s[i % TT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], q[i / TT], i >= TT ? s[i % TT] : floatx16{}, 0, 0, 0);
+        constexpr int kAhead = TT * KS < 8 ? TT * KS : 8;
+        __builtin_amdgcn_sched_group_barrier(kReads, kAhead, 0);
 #pragma unroll
-        for (int i = 0; i < 2 * KS - 8; ++i) {
+        for (int i = 0; i < TT * KS - kAhead; ++i) {
             __builtin_amdgcn_sched_group_barrier(kProducts, 1, 0);
             __builtin_amdgcn_sched_group_barrier(kReads, 1, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(kProducts, 8, 0);
+        __builtin_amdgcn_sched_group_barrier(kProducts, kAhead, 0);
         // The first step's V fragments come in under the softmax.
         u32x4 vf[2][DT];
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) vf[0][dt] = value_fragment(tile_v, 0, dt);
         __builtin_amdgcn_sched_barrier(0);
-        half8 p[4];
+        half8 p[2 * TT];
         {
             if constexpr (MASKED) {
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
+                for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         if (j0 + tt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen) s[tt][r] = -INFINITY;
             }
             // The NaN-propagating maximum of three is one instruction; a score that
             // is NaN leaves the maximum where it was, and its query becomes NaN.
-            float tops[2];
+            float tops[TT];
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt) {
+            for (int tt = 0; tt < TT; ++tt) {
                 tops[tt] = s[tt][0];
 #pragma unroll
                 for (int r = 1; r < 15; r += 2)
                     tops[tt] = __builtin_elementwise_maximum(__builtin_elementwise_maximum(tops[tt], s[tt][r]), s[tt][r + 1]);
             }
             float top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(tops[0], s[0][15]),
-                                                      __builtin_elementwise_maximum(tops[1], s[1][15]));
+                                                      __builtin_elementwise_maximum(tops[TT - 1], s[TT - 1][15]));
             top = both_max(top) * a.scale2;
             if (__any(top > m + kSlack)) {
                 const float now = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
@@ -322,9 +322,9 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
             const float base = m == -INFINITY ? 0.0f : m;
             // Plain additions: the dot-product instructions share the matrix cores'
             // pipe, and take 26 cycles instead of 5 beside another wave's products.
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float sum[2 * TT] = {};
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
+            for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) {
                     const float x = __builtin_amdgcn_exp2f(fmaf(s[tt][r], a.scale2, -base)),
@@ -335,15 +335,16 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
                     p[tt * 2 + (r >> 3)][r & 7] = w[0];
                     p[tt * 2 + (r >> 3)][(r & 7) + 1] = w[1];
                 }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l += sum[0] + sum[1];
+            if constexpr (TT == 2) l += sum[2] + sum[3];
         }
         std::uint32_t odd = 0;
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
+        for (int st = 0; st < 2 * TT; ++st)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 u32x4 v = vf[st & 1][dt];
-                if (st < 3) vf[st & 1 ^ 1][dt] = value_fragment(tile_v, st + 1, dt);
+                if (st < 2 * TT - 1) vf[st & 1 ^ 1][dt] = value_fragment(tile_v, st + 1, dt);
                 if constexpr (MASKED) {
                     // Values whose weight may be zero must be finite: 0 * inf is NaN.
 #pragma unroll
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
                     for (int dt = 0; dt < DT; ++dt)
                         for (int sign = 0; sign < 2; ++sign) {
                             floatx16 count = {};
-                            for (int st = 0; st < 4; ++st) {
+                            for (int st = 0; st < 2 * TT; ++st) {
                                 const u32x4 vf = value_fragment(tile_v, st, dt);
                                 half8 is, sees;
 #pragma unroll
@@ -388,7 +389,7 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     };
 
     // This group's buffers: K and V of one tile, then of the next.
-    std::uint16_t* const tiles_of_group = lds + key_group * C::NBUF * 2 * C::TILE;
+    std::uint16_t* const tiles_of_group = lds + key_group * 4 * C::TILE;
     const std::uint32_t to = uniform(lds_address(tiles_of_group));
     auto stage_both = [&](int step, int buffer) {
         stage(k0, a.k_stride, step, to + buffer * C::TILE * 4);
@@ -398,18 +399,14 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     auto turn = [&](int step, int buffer, auto masked) {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's DMA of the tile
         __syncthreads();
-        if (C::NBUF == 2 && step + C::KG < steps) stage_both(step + C::KG, buffer ^ 1);
+        if (step + C::KG < steps) stage_both(step + C::KG, buffer ^ 1);
         const std::uint16_t* const tile = tiles_of_group + buffer * 2 * C::TILE;
         if (!masked || step * kKeys < any) compute(step, tile, tile + C::TILE, masked);
-        if (C::NBUF == 1) {
-            __syncthreads();
-            if (step + C::KG < steps) stage_both(step + C::KG, 0);
-        }
     };
     // All groups take as many turns; `any` is at most `steps` tiles.
     int round = 0, buffer = 0;
-    for (; (round + 1) * C::KG <= clear; ++round, buffer ^= C::NBUF - 1) turn(round * C::KG + key_group, buffer, std::false_type{});
-    for (; round * C::KG < steps; ++round, buffer ^= C::NBUF - 1) turn(round * C::KG + key_group, buffer, std::true_type{});
+    for (; (round + 1) * C::KG <= clear; ++round, buffer ^= 1) turn(round * C::KG + key_group, buffer, std::false_type{});
+    for (; round * C::KG < steps; ++round, buffer ^= 1) turn(round * C::KG + key_group, buffer, std::true_type{});
 
     if constexpr (C::KG > 1) {
         // The other groups hand their states to the first, lane by lane.
@@ -471,20 +468,24 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 // Workgroups of 128 queries, two a CU, read each key tile once for 128 queries
 // and balance well; they need two of them for every CU. Fewer queries are
 // given more waves by key groups, at first beside as many queries, then fewer.
+// Tiles of 32 keys leave LDS for two buffers of four or eight groups; eight
+// groups take longer to start than they save on up to 512 keys.
 // us, the same work by the alternatives (16 query heads, causal):
-//   heads of 128          (4,1)  (4,2)  (2,4)  (1,4)  (8,1)
-//     240                  11.8   13.0   11.8    9.6   18.3
-//     920                  23.0   21.2   17.9   23.4   30.8
-//     2040                 43.8   36.2   38.6   62.0   59.6
-//     4080                 95.2   87.4    116    184    113
-//     1..2040 packed       61.4   79.7    124    193   65.1
-//     4 x 2040             87.8    105    159    264   91.9
-//     8160                  302    296    399    661    281
-//   heads of 64           (4,1)  (4,2)  (4,3)  (2,4)  (1,4)
-//     240                   9.2    9.0   11.4    8.0    7.2
-//     920                  17.2   14.7   16.1   11.2   15.5
-//     920 on 4600, 460 on 3001  62.5  47.5  44.5  54.4  95.9
-//     8160                  176    184    188    218    372
+//   heads of 128               (4,1)  (4,2)  (2,4)  (1,4)  (8,1)
+//     10 on 1500                             20.6   17.4
+//     240                       11.8   13.0  11.1    8.9   18.3
+//     920                       23.0   21.2  17.9   19.8   30.8
+//     2040                      43.8   36.2  38.6   62.0   59.6
+//     4080                      95.2   87.4   116    184    113
+//     1..2040 packed            61.4   79.7   124    193   65.1
+//     4 x 2040                  87.8    105   159    264   91.9
+//     8160                       302    296   399    661    281
+//   heads of 64                (4,1)  (4,2)  (4,3)  (2,4)  (1,8)
+//     10 on 1500                                    13.2   11.7
+//     240                        9.2    9.0  11.4    8.0    7.6
+//     920                       17.2   14.7  16.1   11.2   15.9
+//     920 on 4600, 460 on 3001  62.5   47.5  44.5   54.4
+//     8160                       176    184   188    218
 // 256 queries a workgroup halve the key traffic again, which pays where a
 // sequence is long enough for its last, partly seen tiles not to count.
 template <int D>
@@ -495,13 +496,17 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
         const std::int64_t by_longest = static_cast<std::int64_t>((a.longest_q + queries - 1) / queries) * a.sequences;
         return a.q_heads * std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / queries) + a.sequences);
     };
-    if (workgroups(32) <= cus) launch_prompt<PromptCfg<D, 1, 4, D == 64 ? 2 : 1, 1>>(a, s);
-    else if (workgroups(64) <= cus) launch_prompt<PromptCfg<D, 2, 4, D == 64 ? 2 : 1, 2>>(a, s);
-    else if (D == 64 && workgroups(128) <= cus) launch_prompt<PromptCfg<64, 4, 3, 2, 3>>(a, s);
-    else if (workgroups(128) <= 2 * cus) launch_prompt<PromptCfg<D, 4, 2, 2, 2>>(a, s);
+    if (workgroups(32) <= cus) {
+        if (D == 128) launch_prompt<PromptCfg<D, 1, 4, 32, 2>>(a, s);
+        else if (a.k_tokens > 512LL * a.sequences) launch_prompt<PromptCfg<64, 1, 8, 32, 2>>(a, s);
+        else launch_prompt<PromptCfg<64, 1, 4, 64, 2>>(a, s);
+    }
+    else if (workgroups(64) <= cus) launch_prompt<PromptCfg<D, 2, 4, D == 64 ? 64 : 32, 2>>(a, s);
+    else if (D == 64 && workgroups(128) <= cus) launch_prompt<PromptCfg<64, 4, 3, 64, 3>>(a, s);
+    else if (workgroups(128) <= 2 * cus) launch_prompt<PromptCfg<D, 4, 2, 64, 2>>(a, s);
     else if (D == 128 && a.longest_q >= 4096 && workgroups(128) >= 4 * cus && static_cast<std::int64_t>(a.longest_q) * a.sequences <= 2 * static_cast<std::int64_t>(a.q_tokens))
-        launch_prompt<PromptCfg<128, 8, 1, 2, 2>>(a, s);
-    else launch_prompt<PromptCfg<D, 4, 1, 2, D == 64 ? 3 : 2>>(a, s);
+        launch_prompt<PromptCfg<128, 8, 1, 64, 2>>(a, s);
+    else launch_prompt<PromptCfg<D, 4, 1, 64, D == 64 ? 3 : 2>>(a, s);
 }
 
 void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
