@@ -26,7 +26,8 @@ struct RopeArgs {
     const double* freqs;
     int tokens, dim, rot;
     float eps, inv_dim, rot_scale;
-    int per;                      // tokens of a workgroup
+    int per;                      // tokens of a workgroup (rope_rows_kernel)
+    int pairs;                    // adjacent pairs (rope_any_kernel)
 };
 
 // (m cos, m sin) of position p at frequency f.
@@ -44,7 +45,11 @@ __device__ __forceinline__ float2 turn(std::int32_t p, double f, float m)
 // pairs: 8 adjacent values where pairs are adjacent, else 4 of the first half
 // of the rotated part and their 4 partners (8 adjacent ones past that part).
 // Two rows a lane are on their way while one is worked on. At 8160 tokens of
-// 32 + 8 heads of 128, 64 values of each rotated: 34.5 us, 4.8 TB/s.
+// 32 + 8 heads of 128, 64 values of each rotated, 167 MB in and out: 45 us,
+// 3.7 TB/s; 4080 tokens 28 us. Stores past the caches take 31 and 21 us, but
+// the attention that reads the result next then takes longer by more than
+// that (4 sequences of 1020 tokens, both kernels: 86.4 us, 83.7 with plain
+// stores), so the result stays in the caches.
 template <int LANES, bool PAIRS>
 __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
 {
@@ -173,9 +178,9 @@ __global__ __launch_bounds__(kBlock) void rope_any_kernel(RopeArgs a)
             for (int d = lane; d < a.dim; d += 64) {
                 float y = x[d];
                 if (d < a.rot) {
-                    const bool second = a.per ? (d & 1) : d >= half;  // per: adjacent pairs here
-                    const int i = a.per ? d >> 1 : (second ? d - half : d);
-                    const int mate = a.per ? d ^ 1 : (second ? d - half : d + half);
+                    const bool second = a.pairs ? (d & 1) : d >= half;
+                    const int i = a.pairs ? d >> 1 : (second ? d - half : d);
+                    const int mate = a.pairs ? d ^ 1 : (second ? d - half : d + half);
                     const float2 c = turn(p, a.freqs[i], a.rot_scale);
                     y = second ? y * c.x + x[mate] * c.y : y * c.x - x[mate] * c.y;
                 }
@@ -242,7 +247,7 @@ void qk_norm_rope(const mlvc_hip_qk_norm_rope_desc* d, hipStream_t s)
         else if (d->head_dim <= 128) launch_rows<16>(a, d->interleaved != 0, grid, s);
         else launch_rows<32>(a, d->interleaved != 0, grid, s);
     } else {
-        a.per = d->interleaved != 0;
+        a.pairs = d->interleaved != 0;
         const std::int64_t blocks = (static_cast<std::int64_t>(d->tokens) * (d->q_heads + d->k_heads) + 3) / 4;
         rope_any_kernel<<<static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20)), kBlock, 0, s>>>(a);
     }
