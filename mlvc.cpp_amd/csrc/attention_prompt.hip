@@ -23,7 +23,7 @@ struct PromptArgs {
     std::int64_t q_stride, k_stride, v_stride, out_stride;
     const std::int32_t* q_starts;
     const std::int32_t* k_starts;
-    int sequences, q_heads, group, dim, q_tokens, k_tokens, longest_q, causal, negate;
+    int sequences, q_heads, group, dim, q_tokens, k_tokens, longest_q, causal, negate, cus;
     float scale2;  // |scale| log2(e); negate: scale is negative
 };
 
@@ -152,12 +152,15 @@ template <int D_, int RG_, int KG_, int KEYS_, int OCC_>
 struct PromptCfg {
     static constexpr int D = D_, RG = RG_, KG = KG_, KEYS = KEYS_, OCC = OCC_;
     static constexpr int WAVES = RG * KG;
+    // Several workgroups on a CU: long ones are put beside short ones.
+    static constexpr bool PAIRED = KG == 1 && OCC * 4 / WAVES > 1;
     static constexpr int ROWS = RG * 32;             // queries of a workgroup
     static constexpr int PIECES = D / 8;             // 16-byte pieces of a row
     static constexpr int DMA_ROWS = 64 / PIECES;     // rows of a DMA instruction
     static constexpr int DMA = KEYS / DMA_ROWS;      // instructions of a tile
     static constexpr int TILE = KEYS * D;            // halves
-    static constexpr size_t LDS = static_cast<size_t>(KG) * 2 * 2 * TILE * 2;  // two buffers of K and V
+    static constexpr int TILES = KG * 2 * 2 * TILE;  // two buffers of K and V
+    static constexpr size_t LDS = TILES * 2 + 2 * WAVES * sizeof(int);
     // Piece p of row t is kept at place p ^ swizzle(t): 16 rows of one piece
     // (a K read) fall on all 64 banks, and so do 4 rows of 4 pieces (a V read).
     __host__ __device__ static constexpr int swizzle(int t)
@@ -165,6 +168,53 @@ struct PromptCfg {
         return D == 128 ? 4 * (t & 3) + (t >> 2 & 3) : 4 * (t >> 1 & 1) + (t >> 2 & 3);
     }
 };
+
+// The rank-th tile of queries; false past the last, and for one that is not
+// there. Where workgroups share a CU, by the number of keys a tile may see,
+// most first: tile t of sequence n has level base_n + t, in ROWS keys, and the
+// tiles above a level are counted for 64 levels at a time, one a lane (up to
+// 64 sequences, one a lane too). That takes half a microsecond, and takes 8
+// ragged sequences (1 to 2040 tokens, 16 heads of 128) from 64.5 to 57 us.
+// Else by turns, sequence after sequence within a tile number.
+template <class C>
+__device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles, int& n, int& tile, Span& sq, Span& sk)
+{
+    constexpr int ROWS = C::ROWS;
+    if (!C::PAIRED || a.sequences > 64 || a.sequences == 1) {
+        n = rank % a.sequences;
+        tile = tiles - 1 - rank / a.sequences;
+        sq = span(a.q_starts, n, a.q_tokens), sk = span(a.k_starts, n, a.k_tokens);
+        return tile >= 0 && tile * ROWS < min(sq.count, a.longest_q);
+    }
+    const int lane = threadIdx.x & 63;
+    Span q = {0, 0}, k = {0, 0};
+    if (lane < a.sequences) q = span(a.q_starts, lane, a.q_tokens), k = span(a.k_starts, lane, a.k_tokens);
+    const int count = (min(q.count, a.longest_q) + ROWS - 1) / ROWS;
+    const int base = (a.causal ? max(k.count - q.count, 0) : k.count) / ROWS;
+    int level = 0, above = 0;
+    for (int width = (a.k_tokens / ROWS + tiles + 64) / 64;; width = (width + 63) / 64) {
+        const int top = level + (lane + 1) * width - 1;
+        above = 0;
+        for (int s = 0; s < a.sequences; ++s) {
+            const int c = __builtin_amdgcn_readlane(count, s), b = __builtin_amdgcn_readlane(base, s);
+            above += min(max(b + c - 1 - top, 0), c);
+        }
+        const int at = __builtin_ctzll(__ballot(above <= rank) | 1ull << 63);
+        level += at * width;
+        above = __builtin_amdgcn_readlane(above, at);
+        if (width == 1) break;
+    }
+    const bool has = static_cast<unsigned>(level - base) < static_cast<unsigned>(count);
+    const unsigned long long all = __ballot(has);
+    const int before = __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(all >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(all), 0));
+    const unsigned long long mine = __ballot(has && above + before == rank);
+    if (!mine) return false;
+    n = __builtin_ctzll(mine);
+    tile = level - __builtin_amdgcn_readlane(base, n);
+    sq = {__builtin_amdgcn_readlane(q.first, n), __builtin_amdgcn_readlane(q.count, n)};
+    sk = {__builtin_amdgcn_readlane(k.first, n), __builtin_amdgcn_readlane(k.count, n)};
+    return true;
+}
 
 template <class C>
 __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArgs a, int tiles)
@@ -174,24 +224,33 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row_group = wave % C::RG, key_group = wave / C::RG, column = lane & 31, hi = lane >> 5;
 
-    // Workgroup i runs on XCD i % 8: with a multiple of 8 heads an XCD keeps the
-    // same heads, of all sequences, so their keys stay in its L2. The last
-    // tiles of the queries, which see most keys, go first.
+    // Workgroup i runs on XCD i % 8, its (i / 8)-th there: with a multiple of 8
+    // heads an XCD keeps the same heads, of all sequences, so their keys stay
+    // in its L2. Tiles of queries go in the order of their keys, most first. An
+    // XCD's first workgroups take a CU each and the next ones join them in the
+    // same order, so those come in the opposite one: the longest beside the
+    // shortest.
     int head, n, tile;
-    if (a.q_heads % kXcds == 0) {
-        const int per = a.q_heads / kXcds, i = blockIdx.x / kXcds, j = i / per;
-        head = blockIdx.x % kXcds * per + i % per;
-        n = j % a.sequences;
-        tile = tiles - 1 - j / a.sequences;
-    } else {
-        const int j = blockIdx.x / a.q_heads;
-        head = blockIdx.x % a.q_heads;
-        n = j % a.sequences;
-        tile = tiles - 1 - j / a.sequences;
+    Span sq, sk;
+    {
+        unsigned i = blockIdx.x / kXcds;
+        if constexpr (C::PAIRED) {
+            const unsigned cus = a.cus / kXcds, joined = min(2 * cus, gridDim.x / kXcds);
+            if (i >= cus && i < joined) i = cus + joined - 1 - i;
+        }
+        int rank;
+        if (a.q_heads % kXcds == 0) {
+            const int per = a.q_heads / kXcds;
+            head = blockIdx.x % kXcds * per + i % per;
+            rank = i / per;
+        } else {
+            i = i * kXcds + blockIdx.x % kXcds;
+            head = i % a.q_heads;
+            rank = i / a.q_heads;
+        }
+        if (!choose<C>(a, rank, tiles, n, tile, sq, sk)) return;
     }
-    const Span sq = span(a.q_starts, n, a.q_tokens), sk = span(a.k_starts, n, a.k_tokens);
     const int q0 = tile * C::ROWS, nq = min(sq.count, a.longest_q);
-    if (q0 >= nq) return;
     const int behind = sk.count - sq.count;  // keys before the first query
     const int last = min(q0 + C::ROWS, nq) - 1;
     const int keys = a.causal ? max(0, min(sk.count, behind + last + 1)) : sk.count;  // seen by any query here
@@ -262,8 +321,8 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
         for (int r = 0; r < 16; ++r) acc[dt][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    auto compute = [&](int step, const std::uint16_t* tile_k, const std::uint16_t* tile_v, auto masked) {
-        constexpr bool MASKED = decltype(masked)::value;
+    auto compute = [&](int step, const std::uint16_t* tile_k, const std::uint16_t* tile_v, auto masked, auto cleaned) {
+        constexpr bool MASKED = decltype(masked)::value, CLEANED = decltype(cleaned)::value;
         const int j0 = step * kKeys;
         // Eight K fragments are read ahead of the products, then one for each
         // fragment used: an LDS read takes as long as four products.
@@ -338,53 +397,45 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
             l += sum[0] + sum[1];
             if constexpr (TT == 2) l += sum[2] + sum[3];
         }
-        std::uint32_t odd = 0;
 #pragma unroll
         for (int st = 0; st < 2 * TT; ++st)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 u32x4 v = vf[st & 1][dt];
                 if (st < 2 * TT - 1) vf[st & 1 ^ 1][dt] = value_fragment(tile_v, st + 1, dt);
-                if constexpr (MASKED) {
-                    // Values whose weight may be zero must be finite: 0 * inf is NaN.
+                if constexpr (CLEANED) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const std::uint32_t lo = (v[e] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u,
-                                            up = (v[e] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
-                        odd |= lo | up;
-                        v[e] &= ~(lo | up);
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        v[e] &= ~(((v[e] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((v[e] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u));
                 }
                 acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, v), p[st], acc[dt], 0, 0, 0);
-                if constexpr (!MASKED) __builtin_amdgcn_sched_barrier(0);
+                if constexpr (!CLEANED) __builtin_amdgcn_sched_barrier(0);
             }
-        if constexpr (MASKED) {
+        if constexpr (CLEANED) {
             // What was left out above: a query that sees an infinity or NaN gets
             // it. Counted by products of 0 / 1 matrices, once for +inf and NaN,
             // once for -inf and NaN.
-            if (__any(odd != 0)) {
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-                        for (int sign = 0; sign < 2; ++sign) {
-                            floatx16 count = {};
-                            for (int st = 0; st < 2 * TT; ++st) {
-                                const u32x4 vf = value_fragment(tile_v, st, dt);
-                                half8 is, sees;
+            for (int dt = 0; dt < DT; ++dt)
+                for (int sign = 0; sign < 2; ++sign) {
+                    floatx16 count = {};
+                    for (int st = 0; st < 2 * TT; ++st) {
+                        const u32x4 vf = value_fragment(tile_v, st, dt);
+                        half8 is, sees;
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const std::uint32_t v = vf[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-                                    const bool bad = (v & 0x7fffu) > 0x7c00u || v == (sign ? 0xfc00u : 0x7c00u);
-                                    is[e] = static_cast<_Float16>(bad ? 1.0f : 0.0f);
-                                    const int j = j0 + st * 16 + 8 * (e >> 2) + 4 * hi + (e & 3);
-                                    sees[e] = static_cast<_Float16>(j < seen ? 1.0f : 0.0f);
-                                }
-                                count = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, count, 0, 0, 0);
-                            }
-#pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                if (count[r] > 0.0f) acc[dt][r] += sign ? -INFINITY : INFINITY;
+                        for (int e = 0; e < 8; ++e) {
+                            const std::uint32_t v = vf[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+                            const bool bad = (v & 0x7fffu) > 0x7c00u || v == (sign ? 0xfc00u : 0x7c00u);
+                            is[e] = static_cast<_Float16>(bad ? 1.0f : 0.0f);
+                            const int j = j0 + st * 16 + 8 * (e >> 2) + 4 * hi + (e & 3);
+                            sees[e] = static_cast<_Float16>(j < seen ? 1.0f : 0.0f);
                         }
-            }
+                        count = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, count, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (count[r] > 0.0f) acc[dt][r] += sign ? -INFINITY : INFINITY;
+                }
         }
     };
 
@@ -396,17 +447,48 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
         stage(v0, a.v_stride, step, to + buffer * C::TILE * 4 + C::TILE * 2);
     };
     if (key_group < steps) stage_both(key_group, 0);
-    auto turn = [&](int step, int buffer, auto masked) {
+    // Whether the pieces of V that this wave staged hold an infinity or NaN.
+    auto any_odd = [&](const std::uint16_t* tile_v) {
+        typedef std::uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 top = {0, 0};
+#pragma unroll
+        for (int i = 0; i < (C::DMA + C::RG - 1) / C::RG; ++i) {
+            if (C::DMA % C::RG != 0 && row_group + i * C::RG >= C::DMA) continue;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(tile_v + (row_group + i * C::RG) * 512 + lane * 8);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[e] & 0x7fff7fffu));
+        }
+        return __any(max(top[0], top[1]) >= 0x7c00u) != 0;
+    };
+    int* const flags = reinterpret_cast<int*>(lds + C::TILES);  // [2][WAVES]
+    auto arrived = [&](auto&& after) {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's DMA of the tile
+        after();
         __syncthreads();
+    };
+    auto turn = [&](int step, int buffer, auto masked, auto cleaned) {
         if (step + C::KG < steps) stage_both(step + C::KG, buffer ^ 1);
         const std::uint16_t* const tile = tiles_of_group + buffer * 2 * C::TILE;
-        if (!masked || step * kKeys < any) compute(step, tile, tile + C::TILE, masked);
+        if (!masked || step * kKeys < any) compute(step, tile, tile + C::TILE, masked, cleaned);
     };
-    // All groups take as many turns; `any` is at most `steps` tiles.
+    // All groups take as many turns; `any` is at most `steps` tiles. First the
+    // tiles that are seen whole; then those with masked keys, whose values get
+    // the weight 0, while all of them are finite; then, cleaned, the rest.
     int round = 0, buffer = 0;
-    for (; (round + 1) * C::KG <= clear; ++round, buffer ^= 1) turn(round * C::KG + key_group, buffer, std::false_type{});
-    for (; round * C::KG < steps; ++round, buffer ^= 1) turn(round * C::KG + key_group, buffer, std::true_type{});
+    for (; (round + 1) * C::KG <= clear; ++round, buffer ^= 1) {
+        arrived([] {});
+        turn(round * C::KG + key_group, buffer, std::false_type{}, std::false_type{});
+    }
+    for (; round * C::KG < steps; ++round, buffer ^= 1) {
+        const int step = round * C::KG + key_group;
+        arrived([&] { flags[buffer * C::WAVES + wave] = step < steps && any_odd(tiles_of_group + (2 * buffer + 1) * C::TILE); });
+        if (__any(flags[buffer * C::WAVES + lane % C::WAVES])) break;
+        turn(step, buffer, std::true_type{}, std::false_type{});
+    }
+    for (; round * C::KG < steps; ++round, buffer ^= 1) {
+        arrived([] {});
+        turn(round * C::KG + key_group, buffer, std::true_type{}, std::true_type{});
+    }
 
     if constexpr (C::KG > 1) {
         // The other groups hand their states to the first, lane by lane.
@@ -460,7 +542,10 @@ template <class C>
 void launch_prompt(const PromptArgs& a, hipStream_t s)
 {
     const int tiles = (a.longest_q + C::ROWS - 1) / C::ROWS;
-    const std::int64_t grid = static_cast<std::int64_t>(tiles) * a.q_heads * a.sequences;
+    // Tiles, at most, from what the host knows; a multiple of the XCDs' number.
+    const std::int64_t by_longest = static_cast<std::int64_t>(tiles) * a.sequences;
+    const std::int64_t most = !C::PAIRED || a.sequences > 64 ? by_longest : std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / C::ROWS) + a.sequences);
+    const std::int64_t grid = (most * a.q_heads + kXcds - 1) / kXcds * kXcds;
     require(grid <= INT_MAX, "attention_prompt", "too many sequences, heads and queries in one call");
     prompt_kernel<C><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles);
 }
@@ -477,9 +562,9 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 //     920                       23.0   21.2  17.9   19.8   30.8
 //     2040                      43.8   36.2  38.6   62.0   59.6
 //     4080                      95.2   87.4   116    184    113
-//     1..2040 packed            61.4   79.7   124    193   65.1
-//     4 x 2040                  87.8    105   159    264   91.9
-//     8160                       302    296   399    661    281
+//     1..2040 packed            56.1   79.7   124    193   65.1
+//     4 x 2040                  85.8    105   159    264   91.9
+//     8160                       302    296   399    661    268
 //   heads of 64                (4,1)  (4,2)  (4,3)  (2,4)  (1,8)
 //     10 on 1500                                    13.2   11.7
 //     240                        9.2    9.0  11.4    8.0    7.6
@@ -535,7 +620,8 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
     a.q_stride = d->q_stride, a.k_stride = d->k_stride, a.v_stride = d->v_stride, a.out_stride = d->out_stride;
     a.q_starts = d->q_starts, a.k_starts = d->k_starts;
     a.sequences = d->sequences, a.q_heads = d->q_heads, a.group = d->q_heads / d->kv_heads, a.dim = d->head_dim;
-    a.q_tokens = d->q_tokens, a.k_tokens = d->k_tokens, a.longest_q = d->longest_q, a.causal = d->causal != 0;
+    a.q_tokens = d->q_tokens, a.k_tokens = d->k_tokens, a.longest_q = std::min(d->longest_q, d->q_tokens), a.causal = d->causal != 0;
+    a.cus = conv::cu_count();
     a.scale2 = std::fabs(d->scale) * 1.4426950408889634f, a.negate = d->scale < 0.0f;
     // The matrix-core kernel addresses a tile's rows by 32-bit byte offsets,
     // and scales masked scores (-inf) by the factor, which must not be 0.

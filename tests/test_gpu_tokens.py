@@ -447,6 +447,31 @@ def test_prompt_tiles_unseen_rows(dev, rng, n, q_heads, dim):
     assert np.isfinite(got[:, :, columns]).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("sequences,q_heads,kv_heads,longest", [
+    (23, 32, 4, None),     # a CU holds several workgroups, an XCD whole heads
+    (55, 10, 5, None),     # heads that the XCDs do not divide
+    (64, 16, 16, 5000),    # a bound on the queries far above them
+    (90, 8, 2, None),      # more sequences than a wave has lanes
+])
+def test_prompt_many_ragged_sequences(dev, rng, dim, causal, sequences, q_heads, kv_heads, longest):
+    """Sequences of 0 to 300 queries on fewer or more keys: every query is answered once, by its own keys."""
+    queries = [int(n) for n in rng.choice([0, 1, 5, 31, 128, 129, 300], sequences)]
+    keys = [max(0, n + int(more)) for n, more in zip(queries, rng.choice([0, 0, -40, 3, 64, 500], sequences))]
+    q = normal(rng, sum(queries), q_heads, dim)
+    k, v = normal(rng, sum(keys), kv_heads, dim), normal(rng, sum(keys), kv_heads, dim)
+    got = Prompt(dev, q, k, v, queries, keys, causal, dim ** -0.5, longest=longest).run()
+    assert np.isfinite(got).all()
+    sq, sk = np.cumsum([0] + queries), np.cumsum([0] + keys)
+    for head in {0, q_heads // 2 + 1}:
+        kv = head // (q_heads // kv_heads)
+        for n in range(sequences):
+            a, b = slice(sq[n], sq[n + 1]), slice(sk[n], sk[n + 1])
+            want, tol = attend64(f64(q[a, head:head + 1]), f64(k[b, kv:kv + 1]), f64(v[b, kv:kv + 1]), dim ** -0.5, causal)
+            within(got[a, head:head + 1], want, tol)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("heads,dim,lengths", [
     (2, 64, [0, 30000, 1, 700]),          # one stream in many shares, others inside one
