@@ -25,6 +25,9 @@ inline bool vector_rows(const void* p, std::int64_t stride) { return aligned16(p
 
 constexpr int kMaxHeadDim = 512;
 
+// A launch counts its threads in 32 bits along an axis.
+inline bool launchable(std::int64_t workgroups, int threads) { return workgroups <= UINT_MAX / threads; }
+
 // Checks a cache descriptor; `op` names the caller in the message.
 void check_cache(const mlvc_hip_kv_cache* cache, const char* op);
 

@@ -546,7 +546,7 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
     const std::int64_t by_longest = static_cast<std::int64_t>(tiles) * a.sequences;
     const std::int64_t most = !C::PAIRED || a.sequences > 64 ? by_longest : std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / C::ROWS) + a.sequences);
     const std::int64_t grid = (most * a.q_heads + kXcds - 1) / kXcds * kXcds;
-    require(grid <= INT_MAX, "attention_prompt", "too many sequences, heads and queries in one call");
+    require(launchable(grid, C::WAVES * 64), "attention_prompt", "too many sequences, heads and queries in one call");
     prompt_kernel<C><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles);
 }
 
@@ -630,8 +630,10 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
                       vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f;
     if (rows && d->head_dim == 128) launch_prompt<128>(a, s);
     else if (rows && d->head_dim == 64) launch_prompt<64>(a, s);
-    else
+    else {
+        require(launchable(d->q_tokens, 64), op, "too many sequences, heads and queries in one call");
         prompt_any_kernel<<<dim3(static_cast<unsigned>(d->q_tokens), static_cast<unsigned>(d->q_heads)), 64, 0, s>>>(a);
+    }
     check(hipGetLastError(), "attention_prompt launch");
 }
 

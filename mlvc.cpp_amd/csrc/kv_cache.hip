@@ -238,7 +238,7 @@ void run(const mlvc_hip_kv_cache* c, const mlvc_hip_kv_rows* r, hipStream_t s)
     a.stride[0] = r->k_stride, a.stride[1] = r->v_stride;
     a.slots = r->slots;
     const std::int64_t rows = static_cast<std::int64_t>(r->tokens) * c->heads;
-    require(rows <= INT_MAX, op, "too many rows in one call");
+    require(launchable(rows / 4 + 1, kBlock), op, "too many rows in one call");
     a.rows = static_cast<unsigned>(rows);
     a.heads = c->heads, a.dim = c->head_dim, a.page = c->page_size, a.slot_count = c->pages * c->page_size;
     const bool vectors = c->head_dim > 32 && c->head_dim <= 256 && vector_rows(r->k, r->k_stride) && vector_rows(r->v, r->v_stride);

@@ -11,6 +11,8 @@
 
 #include "attention.hpp"
 
+#include <algorithm>
+
 namespace mlvc_hip {
 namespace {
 
@@ -26,8 +28,7 @@ struct RopeArgs {
     const double* freqs;
     int tokens, dim, rot;
     float eps, inv_dim, rot_scale;
-    int per;                      // tokens of a workgroup (rope_rows_kernel)
-    int pairs;                    // adjacent pairs (rope_any_kernel)
+    int pairs;  // adjacent pairs (rope_any_kernel)
 };
 
 // (m cos, m sin) of position p at frequency f.
@@ -44,17 +45,20 @@ __device__ __forceinline__ float2 turn(std::int32_t p, double f, float m)
 // values each, and a wave holds 64 / LANES rows. A lane has both values of its
 // pairs: 8 adjacent values where pairs are adjacent, else 4 of the first half
 // of the rotated part and their 4 partners (8 adjacent ones past that part).
-// Two rows a lane are on their way while one is worked on. At 8160 tokens of
-// 32 + 8 heads of 128, 64 values of each rotated, 167 MB in and out: 45 us,
-// 3.7 TB/s; 4080 tokens 28 us. Stores past the caches take 31 and 21 us, but
-// the attention that reads the result next then takes longer by more than
-// that (4 sequences of 1020 tokens, both kernels: 86.4 us, 83.7 with plain
-// stores), so the result stays in the caches.
+// Two rows a lane are on their way while one is worked on, and a workgroup
+// takes every gridDim.x-th token, so that the GPU reads and writes one narrow
+// stretch at a time. At 8160 tokens of 32 + 8 heads of 128, 64 values of each
+// rotated, 167 MB in and out: 44 us, 3.8 TB/s; 4080 tokens 18.4 us, 4.5 TB/s
+// (neighbouring tokens to a workgroup: 45 and 22). Neither the turns nor the
+// sums bound it (1 us each). Stores past the caches take 31 us alone, but the
+// attention that reads the result next then takes longer by more than that (4
+// sequences of 1020 tokens, both kernels: 86.4 us, 83.7 with plain stores), so
+// the result stays in the caches.
 template <int LANES, bool PAIRS>
 __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
 {
     extern __shared__ float2 table[];  // [per][rot / 2]
-    const int t0 = blockIdx.x * a.per, nt = min(a.per, a.tokens - t0), half = a.rot >> 1;
+    const int t0 = blockIdx.x, every = gridDim.x, nt = (a.tokens - t0 + every - 1) / every, half = a.rot >> 1;
     const int lane = threadIdx.x % LANES, heads = a.heads[0] + a.heads[1];
     const bool mine = lane * 8 < a.dim, turned = lane * 8 < a.rot;
     // First values of the lane's two runs of 4.
@@ -67,6 +71,7 @@ __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
     struct Eight {
         uint2 lo, hi;
     };
+    auto token = [&](int t) { return t0 + static_cast<std::int64_t>(t) * every; };
     auto further = [&](Row r) {
         r.h += kStep;
         while (r.h >= heads) r.h -= heads, ++r.t;
@@ -84,7 +89,7 @@ __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
     auto fetch = [&](Row r) {
         const int of = r.h >= a.heads[0];
         if (r.t >= nt || !mine) return Eight{};
-        return load(a.in[of] + (t0 + r.t) * a.in_stride[of] + column(r, of));
+        return load(a.in[of] + token(r.t) * a.in_stride[of] + column(r, of));
     };
     const int group = threadIdx.x / LANES;
     Row now{group / heads, group % heads}, next = further(now);
@@ -92,7 +97,7 @@ __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
 
     for (int i = threadIdx.x; i < nt * half; i += kBlock) {
         const int t = i / half;
-        table[i] = turn(a.positions[t0 + t], a.freqs[i - t * half], a.rot_scale);
+        table[i] = turn(a.positions[token(t)], a.freqs[i - t * half], a.rot_scale);
     }
     Eight w[2];
 #pragma unroll
@@ -134,7 +139,7 @@ __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
         if (!mine) continue;
         const uint2 lo = make_uint2(pack_rounded(x[0], x[1]), pack_rounded(x[2], x[3])),
                     hi = make_uint2(pack_rounded(x[4], x[5]), pack_rounded(x[6], x[7]));
-        std::uint16_t* out = a.out[of] + (t0 + now.t) * a.out_stride[of] + column(now, of);
+        std::uint16_t* out = a.out[of] + token(now.t) * a.out_stride[of] + column(now, of);
         if constexpr (PAIRS) {
             *reinterpret_cast<u32x4*>(out + d0) = u32x4{lo.x, lo.y, hi.x, hi.y};
         } else {
@@ -192,9 +197,13 @@ __global__ __launch_bounds__(kBlock) void rope_any_kernel(RopeArgs a)
 }
 
 template <int LANES>
-void launch_rows(const RopeArgs& a, bool pairs, unsigned grid, hipStream_t s)
+void launch_rows(const RopeArgs& a, bool pairs, hipStream_t s)
 {
-    const size_t lds = static_cast<size_t>(a.per) * (a.rot / 2) * sizeof(float2);
+    // As many workgroups as the GPU holds at once, so that one's launch and
+    // first loads are paid once; up to kMost tokens each, and their tables.
+    constexpr int kMost = 4;
+    const int held = 8 * conv::cu_count(), grid = std::max(std::min(a.tokens, held), (a.tokens - 1) / kMost + 1);
+    const size_t lds = static_cast<size_t>((a.tokens - 1) / grid + 1) * (a.rot / 2) * sizeof(float2);
     if (pairs) rope_rows_kernel<LANES, true><<<grid, kBlock, lds, s>>>(a);
     else rope_rows_kernel<LANES, false><<<grid, kBlock, lds, s>>>(a);
 }
@@ -204,6 +213,7 @@ void qk_norm_rope(const mlvc_hip_qk_norm_rope_desc* d, hipStream_t s)
     const char* op = "qk_norm_rope";
     require(d != nullptr, op, "no descriptor");
     require(d->tokens >= 0, op, "negative token count");
+    require(launchable(d->tokens / 4 + 1, kBlock), op, "too many tokens in one call");
     require(d->head_dim >= 1 && d->head_dim <= kMaxHeadDim, op, "head_dim must be 1..512");
     require(d->q_heads >= 0 && d->k_heads >= 0 && d->q_heads <= 65536 && d->k_heads <= 65536 && d->q_heads + d->k_heads > 0,
             op, "head counts must be 0..65536 and not both 0");
@@ -239,13 +249,9 @@ void qk_norm_rope(const mlvc_hip_qk_norm_rope_desc* d, hipStream_t s)
     if (d->q_heads) rows = rows && vector_rows(d->q, d->q_stride) && vector_rows(d->q_out, d->q_out_stride);
     if (d->k_heads) rows = rows && vector_rows(d->k, d->k_stride) && vector_rows(d->k_out, d->k_out_stride);
     if (rows) {
-        // Four tokens a workgroup share the launch and give every thread a
-        // frequency; few tokens go one to a workgroup, over more CUs.
-        a.per = d->tokens >= 8 * conv::cu_count() ? 4 : 1;
-        const unsigned grid = static_cast<unsigned>((static_cast<std::int64_t>(d->tokens) + a.per - 1) / a.per);
-        if (d->head_dim <= 64) launch_rows<8>(a, d->interleaved != 0, grid, s);
-        else if (d->head_dim <= 128) launch_rows<16>(a, d->interleaved != 0, grid, s);
-        else launch_rows<32>(a, d->interleaved != 0, grid, s);
+        if (d->head_dim <= 64) launch_rows<8>(a, d->interleaved != 0, s);
+        else if (d->head_dim <= 128) launch_rows<16>(a, d->interleaved != 0, s);
+        else launch_rows<32>(a, d->interleaved != 0, s);
     } else {
         a.pairs = d->interleaved != 0;
         const std::int64_t blocks = (static_cast<std::int64_t>(d->tokens) * (d->q_heads + d->k_heads) + 3) / 4;

@@ -79,6 +79,19 @@ def test_rotation_in_place_scaled_and_far(dev, rng, dim, shift, interleaved):
         within(g, want, tol)
 
 
+@pytest.mark.parametrize("tokens", [2050, 4111, 8191, 8193, 10007])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_norm_and_rotation_of_many_tokens(dev, rng, tokens, in_place):
+    """More tokens than the GPU holds workgroups: one to several of them each, some with one less."""
+    q, k, w = normal(rng, tokens, 2, 64), normal(rng, tokens, 1, 64), normal(rng, 64)
+    positions = rng.integers(0, 70000, tokens)
+    freqs, _ = mlvc_hip.rope_frequencies(32)
+    got = _rope(dev, q, k, w, w, positions, freqs, False, in_place=in_place)
+    for g, x in zip(got, (q, k)):
+        want, tol = rope64(x, w, 1e-6, positions, freqs, False, 1.0)
+        within(g, want, tol)
+
+
 def test_norm_of_zero_and_large_rows(dev):
     q = np.zeros((3, 2, 64), np.float16)
     q[1] = 60000.0
