@@ -45,15 +45,15 @@ __device__ __forceinline__ float2 turn(std::int32_t p, double f, float m)
 // values each, and a wave holds 64 / LANES rows. A lane has both values of its
 // pairs: 8 adjacent values where pairs are adjacent, else 4 of the first half
 // of the rotated part and their 4 partners (8 adjacent ones past that part).
-// Two rows a lane are on their way while one is worked on, and a workgroup
-// takes every gridDim.x-th token, so that the GPU reads and writes one narrow
-// stretch at a time. At 8160 tokens of 32 + 8 heads of 128, 64 values of each
-// rotated, 167 MB in and out: 44 us, 3.8 TB/s; 4080 tokens 18.4 us, 4.5 TB/s
-// (neighbouring tokens to a workgroup: 45 and 22). Neither the turns nor the
-// sums bound it (1 us each). Stores past the caches take 31 us alone, but the
-// attention that reads the result next then takes longer by more than that (4
-// sequences of 1020 tokens, both kernels: 86.4 us, 83.7 with plain stores), so
-// the result stays in the caches.
+// A row is worked on while the next one is on its way, and a workgroup takes
+// every gridDim.x-th token, so that the GPU reads and writes one narrow stretch
+// at a time. At 8160 tokens of 32 + 8 heads of 128, 64 values of each rotated,
+// 167 MB in and out: 33.6 us, 5.0 TB/s, a copy's rate (neighbouring tokens to a
+// workgroup 34.7; two rows on their way 34.5, three 35.6); 4080 tokens 14.8 us.
+// Stores past the caches take 27.3 us alone, but the attention that reads the
+// result next then takes longer by as much or more (4 sequences of 1020 tokens,
+// both kernels: 74.8 us, 71.5 with plain stores), so the result stays in the
+// caches.
 template <int LANES, bool PAIRS>
 __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
 {
@@ -61,23 +61,28 @@ __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
     const int t0 = blockIdx.x, every = gridDim.x, nt = (a.tokens - t0 + every - 1) / every, half = a.rot >> 1;
     const int lane = threadIdx.x % LANES, heads = a.heads[0] + a.heads[1];
     const bool mine = lane * 8 < a.dim, turned = lane * 8 < a.rot;
-    // First values of the lane's two runs of 4.
-    const int d0 = PAIRS || !turned ? lane * 8 : lane * 4, d1 = PAIRS || !turned ? d0 + 4 : half + d0;
+    // First values of the lane's two runs of 4; those of lane 0 past the row.
+    const int d0 = !mine ? 0 : PAIRS || !turned ? lane * 8 : lane * 4, d1 = !mine || PAIRS || !turned ? d0 + 4 : half + d0;
 
     constexpr int kStep = kBlock / LANES;
+    const int step_t = kStep / heads, step_h = kStep % heads;
     struct Row {
         int t, h;
     };
     struct Eight {
         uint2 lo, hi;
     };
-    auto token = [&](int t) { return t0 + static_cast<std::int64_t>(t) * every; };
     auto further = [&](Row r) {
-        r.h += kStep;
-        while (r.h >= heads) r.h -= heads, ++r.t;
+        r.h += step_h, r.t += step_t;
+        if (r.h >= heads) r.h -= heads, ++r.t;
         return r;
     };
-    auto column = [&](Row r, int of) { return static_cast<std::int64_t>(r.h - (of ? a.heads[0] : 0)) * a.dim; };
+    // Queries or keys, lane by lane: a choice of two values, where an index
+    // into the arguments would be a load from memory.
+    auto of = [&](Row r, auto q, auto k) { return r.h >= a.heads[0] ? k : q; };
+    auto place = [&](int t, Row r, auto q, auto k, std::int64_t q_stride, std::int64_t k_stride) {
+        return of(r, q, k) + (t0 + static_cast<std::int64_t>(t) * every) * of(r, q_stride, k_stride) + (r.h - of(r, 0, a.heads[0])) * a.dim;
+    };
     auto load = [&](const std::uint16_t* p) {
         if constexpr (PAIRS) {
             const u32x4 v = *reinterpret_cast<const u32x4*>(p + d0);
@@ -86,42 +91,43 @@ __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
             return Eight{*reinterpret_cast<const uint2*>(p + d0), *reinterpret_cast<const uint2*>(p + d1)};
         }
     };
-    auto fetch = [&](Row r) {
-        const int of = r.h >= a.heads[0];
-        if (r.t >= nt || !mine) return Eight{};
-        return load(a.in[of] + token(r.t) * a.in_stride[of] + column(r, of));
-    };
+    // Past the last token, that one again: without a branch the loads stay in flight.
+    auto fetch = [&](Row r) { return load(place(min(r.t, nt - 1), r, a.in[0], a.in[1], a.in_stride[0], a.in_stride[1])); };
     const int group = threadIdx.x / LANES;
-    Row now{group / heads, group % heads}, next = further(now);
-    Eight raw = fetch(now), raw_next = fetch(next);
+    Row now{group / heads, group % heads};
+    Eight raw = fetch(now);
 
     for (int i = threadIdx.x; i < nt * half; i += kBlock) {
         const int t = i / half;
-        table[i] = turn(a.positions[token(t)], a.freqs[i - t * half], a.rot_scale);
+        table[i] = turn(a.positions[t0 + static_cast<std::int64_t>(t) * every], a.freqs[i - t * half], a.rot_scale);
     }
-    Eight w[2];
-#pragma unroll
-    for (int of = 0; of < 2; ++of) w[of] = a.weight[of] && mine ? load(a.weight[of]) : Eight{};
+    const bool normed[2] = {a.weight[0] != nullptr, a.weight[1] != nullptr};
+    const Eight w[2] = {normed[0] ? load(a.weight[0]) : Eight{}, normed[1] ? load(a.weight[1]) : Eight{}};
     __syncthreads();
 
     auto widen = [](const Eight& v, float* x) {
         x[0] = lo_f16(v.lo.x), x[1] = hi_f16(v.lo.x), x[2] = lo_f16(v.lo.y), x[3] = hi_f16(v.lo.y);
         x[4] = lo_f16(v.hi.x), x[5] = hi_f16(v.hi.x), x[6] = lo_f16(v.hi.y), x[7] = hi_f16(v.hi.y);
     };
-    for (; now.t < nt; now = next, next = further(next)) {
-        const int of = now.h >= a.heads[0];
+    for (Row next; now.t < nt; now = next) {
         float x[8];
         widen(raw, x);
-        raw = raw_next;
-        raw_next = fetch(further(next));
-        if (a.weight[of]) {
+        next = further(now);
+        raw = fetch(next);
+        if (normed[0] || normed[1]) {
             float sum = 0.0f, f[8];
+            if (!mine)
+                for (int i = 0; i < 8; ++i) x[i] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
             const float r = rsqrtf(fmaf(group_sum<LANES>(sum), a.inv_dim, a.eps));
-            widen(of ? w[1] : w[0], f);
+            const Eight wide = {make_uint2(of(now, w[0].lo.x, w[1].lo.x), of(now, w[0].lo.y, w[1].lo.y)),
+                                make_uint2(of(now, w[0].hi.x, w[1].hi.x), of(now, w[0].hi.y, w[1].hi.y))};
+            widen(wide, f);
+            if (of(now, normed[0], normed[1])) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * r * f[i];
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * f[i];
+            }
         }
         if (turned) {
             const float2* cs = table + now.t * half + lane * 4;
@@ -139,7 +145,7 @@ __global__ __launch_bounds__(kBlock) void rope_rows_kernel(RopeArgs a)
         if (!mine) continue;
         const uint2 lo = make_uint2(pack_rounded(x[0], x[1]), pack_rounded(x[2], x[3])),
                     hi = make_uint2(pack_rounded(x[4], x[5]), pack_rounded(x[6], x[7]));
-        std::uint16_t* out = a.out[of] + token(now.t) * a.out_stride[of] + column(now, of);
+        std::uint16_t* out = place(now.t, now, a.out[0], a.out[1], a.out_stride[0], a.out_stride[1]);
         if constexpr (PAIRS) {
             *reinterpret_cast<u32x4*>(out + d0) = u32x4{lo.x, lo.y, hi.x, hi.y};
         } else {
