@@ -44,13 +44,13 @@ __device__ __forceinline__ std::uint32_t pack_rounded(float a, float b) { return
 // Value of the lane O away, where the values already agree between lanes 2 O
 // away (or O is half the group). Within 16 lanes by the adders' own lane
 // exchange, without a trip through LDS.
-template <int O, int LANES>
-__device__ __forceinline__ float across(float x)
+template <int O, int LANES, typename T>
+__device__ __forceinline__ T across(T x)
 {
     constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kRotate = 0x120, kMirror8 = 0x141;
     constexpr int kHow = O == 1 ? kSwap1 : O == 2 ? kSwap2 : LANES == 8 ? kMirror8 : kRotate + O;
     if constexpr (O >= 16) return __shfl_xor(x, O);
-    else return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), kHow, 0xf, 0xf, true));
+    else return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), kHow, 0xf, 0xf, true));
 }
 
 // Reductions over groups of LANES adjacent lanes; every lane gets the result.
@@ -66,6 +66,14 @@ template <int LANES, int O = LANES / 2>
 __device__ __forceinline__ float group_max(float x)
 {
     x = fmaxf(x, across<O, LANES>(x));
+    if constexpr (O > 1) return group_max<LANES, O / 2>(x);
+    else return x;
+}
+
+template <int LANES, int O = LANES / 2>
+__device__ __forceinline__ std::uint32_t group_max(std::uint32_t x)
+{
+    x = max(x, across<O, LANES>(x));
     if constexpr (O > 1) return group_max<LANES, O / 2>(x);
     else return x;
 }
