@@ -490,7 +490,10 @@ int mlvc_hip_attention_prompt(const mlvc_hip_attention_prompt_desc* desc, mlvc_h
  * sees lengths[n] tokens, token j in page table[n][j / page_size]. A length of
  * zero gives zeros; tokens of pages outside the cache are not seen. Long
  * contexts are split over workgroups, which leave FP32 partials in the
- * workspace that a second kernel joins in a fixed order. */
+ * workspace that a second kernel joins in a fixed order. Where a context is cut
+ * follows from all lengths of the call: a stream's result may differ in its
+ * last bits from the one it has in another batch, and is the same every time in
+ * the same one. */
 typedef struct mlvc_hip_attention_token_desc {
     const mlvc_hip_kv_cache* cache;
     int streams, q_heads;          /* q_heads a multiple of the cache's heads */
@@ -505,7 +508,8 @@ typedef struct mlvc_hip_attention_token_desc {
     void* workspace;               /* 16-byte aligned; mlvc_hip_attention_token_workspace_bytes */
     size_t workspace_bytes;
 } mlvc_hip_attention_token_desc;
-/* Depends on streams, q_heads, longest and the cache's layout only (0: none needed). */
+/* Depends on streams, q_heads, longest and the cache's layout only (0: none
+ * needed), and grows with streams and longest. */
 size_t mlvc_hip_attention_token_workspace_bytes(const mlvc_hip_attention_token_desc* desc);
 int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip_stream s);
 

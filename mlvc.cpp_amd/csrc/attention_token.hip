@@ -1,7 +1,7 @@
 // Attention of one query per stream on its paged, quantised context.
 //
-// Contexts up to kDirect tokens go to one workgroup a stream and key head,
-// which writes the output itself. Longer ones are dealt evenly: the contexts
+// Short contexts, and longer ones of large batches, go to one workgroup a stream
+// and key head, which writes the output itself. The others are dealt evenly: the contexts
 // of all streams, in steps of 32 tokens, are laid end to end and cut into one
 // share for each workgroup the GPU holds at once, so ragged batches leave no CU
 // idle and a single long stream fills them all. A workgroup finds its share from
@@ -35,7 +35,7 @@ struct TokenArgs {
     float* part;    // [q_heads][2 shares + streams][dim]
     float2* state;  // [q_heads][2 shares + streams]: m, l
     int table_stride, pages, page, heads, q_heads, group, dim, longest, streams;
-    int shares;     // workgroups of a key head that the GPU holds at once; 0: one workgroup a stream
+    int shares;     // workgroups of a key head that the GPU holds at once; 0: a context goes to one workgroup
     unsigned long long tiles;  // 2^32 / (page / 16), rounded up: a tile's page by a product, for tiles below 2^32 / (page / 16)
     float scale2;
 };
@@ -51,24 +51,21 @@ __device__ __forceinline__ int steps_of(const TokenArgs& a, int stream)
     return stream < a.streams ? (context(a, stream) + kStep - 1) / kStep : 0;
 }
 
-__device__ __forceinline__ int wave_sum(int x)
+// Sum over this lane and those before it: rows of 16 lanes by shifts, then
+// each row's total to the rows after it.
+__device__ __forceinline__ int wave_scan(int x)
 {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+    constexpr int kShift = 0x110, kLast15 = 0x142, kLast31 = 0x143;
+    x += __builtin_amdgcn_update_dpp(0, x, kShift + 1, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, kShift + 2, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, kShift + 4, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, kShift + 8, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, kLast15, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, kLast31, 0xc, 0xf, false);
     return x;
 }
 
-// Sum over this lane and those before it.
-__device__ __forceinline__ int wave_scan(int x)
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    return x;
-}
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
 // The shares of a key head's steps: `shares` large ones, all on the GPU at
 // once, cover five sixths of them, and as many small ones cover the rest,
@@ -83,16 +80,29 @@ struct Shares {
         count = few ? max(1, min(a.shares, total / kLeast)) : a.shares;
         large = few ? total : total - total / 6;
     }
+    // First step of share i of n that cut `steps` evenly: i * steps / n without
+    // a 64-bit product (n is a few workgroups a CU).
+    __device__ static int cut(int i, int n, int steps)
+    {
+        const unsigned whole = static_cast<unsigned>(steps) / static_cast<unsigned>(n), rest = static_cast<unsigned>(steps) - whole * n;
+        return static_cast<int>(i * whole + i * rest / static_cast<unsigned>(n));
+    }
+    // The share that holds a step: an estimate that is off by at most one.
+    __device__ static int holds(int step, int n, int steps)
+    {
+        int i = min(static_cast<int>(static_cast<float>(step) * static_cast<float>(n) / static_cast<float>(steps)), n - 1);
+        if (cut(i, n, steps) > step) --i;
+        else if (cut(i + 1, n, steps) <= step) ++i;
+        return i;
+    }
     // First step of a share, and the share that holds a step.
     __device__ int first(int share) const
     {
-        if (share <= count) return static_cast<int>(static_cast<long long>(share) * large / count);
-        return large + static_cast<int>(static_cast<long long>(min(share - count, count)) * (total - large) / count);
+        return share <= count ? cut(share, count, large) : large + cut(min(share - count, count), count, total - large);
     }
     __device__ int holder(int step) const
     {
-        if (step < large) return static_cast<int>((static_cast<long long>(step + 1) * count - 1) / large);
-        return count + static_cast<int>((static_cast<long long>(step - large + 1) * count - 1) / (total - large));
+        return step < large ? holds(step, count, large) : count + holds(step - large, count, total - large);
     }
 };
 
@@ -107,7 +117,7 @@ __device__ __forceinline__ void each_piece(const TokenArgs& a, int share, F&& fn
     auto tokens = [&](int b) { return b + lane < a.streams ? context(a, b + lane) : 0; };
     auto steps = [](int n) { return (n + kStep - 1) / kStep; };
     int block = 0, n = tokens(0), upto = wave_scan(steps(n));
-    int total = __shfl(upto, 63);
+    int total = __builtin_amdgcn_readlane(upto, 63);
     for (int b = 64; b < a.streams; b += 64) total += wave_sum(steps(tokens(b)));
     total = __builtin_amdgcn_readfirstlane(total);
     const Shares shares(a, total);
@@ -116,7 +126,7 @@ __device__ __forceinline__ void each_piece(const TokenArgs& a, int share, F&& fn
     const int end = __builtin_amdgcn_readfirstlane(shares.first(share + 1));
     if (at >= end) return;
     auto next_block = [&] {
-        const int before = __shfl(upto, 63);
+        const int before = __builtin_amdgcn_readlane(upto, 63);
         block += 64;
         n = tokens(block);
         upto = before + wave_scan(steps(n));
@@ -621,21 +631,40 @@ struct Plan {
     size_t part_bytes, bytes;
 };
 
-// Contexts up to this many tokens are not split: a workgroup of eight waves is
-// done with them before a second kernel would start. One stream, 16 heads on 4
-// of 64, INT8: 920 tokens 8.2 us, cut and joined 11.4.
-constexpr int kDirect = 1024;
+// Whether a context goes to one workgroup of eight waves, without a cut. Up to
+// 1024 tokens it is done before a second kernel would start; longer ones are
+// not cut where enough workgroups keep the GPU busy through the longest: half
+// one a CU up to 2048 tokens, three a CU up to 4096. us, whole / cut:
+//   1 x 920, 4 heads of 64, INT8      8.2 / 11.4
+//   200 x 512..1024, 8 of 128, INT8    75 / 91      (1600 workgroups)
+//   16 x 1000..2000, 8 of 128, INT8  20.6 / 20.3    (128)
+//   64 x 1000..2000, 4 of 64, FP16   20.0 / 25.3    (256)
+//   64 x 1..2000, 8 of 128, INT8     41.4 / 39.4    (512)
+//   16 x 1000..2000, 4 of 64, FP16   14.4 / 13.2    (64)
+//   200 x 1..4080, 8 of 128, INT8     172 / 183     (1600)
+//   200 x 1..4080, 4 of 64, E4M3     56.2 / 65.1    (800)
+//   64 x 2040..4080, 4 of 64, FP16   42.4 / 45.6    (256)
+//   64 x 1..4080, 8 of 128, INT8     73.0 / 64.4    (512)
+//   200 x 4080..8160, 4 of 64, FP16   238 / 228     (800)
+bool whole(int longest, std::int64_t workgroups)
+{
+    const std::int64_t cus = conv::cu_count();
+    return longest <= 1024 || (longest <= 2048 && 2 * workgroups >= cus) || (longest <= 4096 && workgroups >= 3 * cus);
+}
 
 Plan plan(const mlvc_hip_attention_token_desc* d)
 {
     Plan p{};
-    if (d->longest <= kDirect) return p;
+    if (d->longest <= 1024) return p;
     // Three workgroups of four waves fit a CU (up to 168 registers).
-    const int group = d->q_heads / d->cache->heads;
-    p.shares = std::max(1, 3 * conv::cu_count() / (d->cache->heads * ((group + 15) / 16)));
-    const size_t slots = (2 * static_cast<size_t>(p.shares) + d->streams) * d->q_heads;
+    const int group = d->q_heads / d->cache->heads, of_stream = d->cache->heads * ((group + 15) / 16);
+    const int shares = std::max(1, 3 * conv::cu_count() / of_stream);
+    const size_t slots = (2 * static_cast<size_t>(shares) + d->streams) * d->q_heads;
     p.part_bytes = slots * d->cache->head_dim * sizeof(float);
+    // Asked for whether this call cuts or not, so that what is enough for a
+    // batch is enough for a smaller one.
     p.bytes = p.part_bytes + slots * sizeof(float2);
+    if (!whole(d->longest, static_cast<std::int64_t>(d->streams) * of_stream)) p.shares = shares;
     return p;
 }
 

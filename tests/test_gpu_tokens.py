@@ -495,3 +495,22 @@ def test_tokens_shares(dev, rng, kind, heads, dim, lengths):
     cache, table, ks, vs = _streams(dev, rng, kind, lengths, heads, dim, 64)
     q = normal(rng, len(lengths), 2 * heads, dim)
     _check_tokens(Token(cache, q, table, lengths, dim ** -0.5).run(), q, ks, vs, lengths, dim ** -0.5)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,dim,streams,longest", [
+    (4, 128, 48, 2048),     # half as many contexts as CUs and more
+    (8, 64, 100, 4096),     # three times as many
+    (3, 96, 70, 2047),      # heads without matrix cores
+])
+def test_tokens_whole_contexts_of_large_batches(dev, rng, kind, heads, dim, streams, longest):
+    """Contexts past 1024 tokens that are not cut, beside short and empty ones; a smaller batch fits the same workspace."""
+    lengths = [int(n) for n in rng.choice([0, 1, 33, 250], streams)]
+    lengths[3], lengths[streams - 1] = longest, longest - 40
+    cache, table, ks, vs = _streams(dev, rng, kind, lengths, heads, dim, 32)
+    q = normal(rng, streams, heads, dim)
+    call = Token(cache, q, table, lengths, dim ** -0.5)
+    _check_tokens(call.run(), q, ks, vs, lengths, dim ** -0.5)
+    call.desc.streams = 5
+    assert mlvc_hip.attention_token_workspace_bytes(call.desc) <= call.desc.workspace_bytes
+    _check_tokens(call.run()[:5], q[:5], ks[:5], vs[:5], lengths[:5], dim ** -0.5)
