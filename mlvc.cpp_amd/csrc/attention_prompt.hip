@@ -154,6 +154,9 @@ struct PromptCfg {
     static constexpr int WAVES = RG * KG;
     // Several workgroups on a CU: long ones are put beside short ones.
     static constexpr bool PAIRED = KG == 1 && OCC * 4 / WAVES > 1;
+    // Tiles in the order of their keys, none that is not there: also where they
+    // just fit the CUs, and an empty one would take a CU's turn.
+    static constexpr bool ORDERED = PAIRED || RG == 3;
     static constexpr int ROWS = RG * 32;             // queries of a workgroup
     static constexpr int PIECES = D / 8;             // 16-byte pieces of a row
     static constexpr int DMA_ROWS = 64 / PIECES;     // rows of a DMA instruction
@@ -170,17 +173,17 @@ struct PromptCfg {
 };
 
 // The rank-th tile of queries; false past the last, and for one that is not
-// there. Where workgroups share a CU, by the number of keys a tile may see,
-// most first: tile t of sequence n has level base_n + t, in ROWS keys, and the
-// tiles above a level are counted for 64 levels at a time, one a lane (up to
-// 64 sequences, one a lane too). That takes half a microsecond, and takes 8
-// ragged sequences (1 to 2040 tokens, 16 heads of 128) from 64.5 to 57 us.
-// Else by turns, sequence after sequence within a tile number.
+// there. ORDERED: by the number of keys a tile may see, most first. Tile t of
+// sequence n has level base_n + t, in ROWS keys, and the tiles above a level are
+// counted for 64 levels at a time, one a lane (up to 64 sequences, one a lane
+// too). That takes half a microsecond, and takes 8 ragged sequences (1 to 2040
+// tokens, 16 heads of 128) from 64.5 to 57 us. Else by turns, sequence after
+// sequence within a tile number.
 template <class C>
 __device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles, int& n, int& tile, Span& sq, Span& sk)
 {
     constexpr int ROWS = C::ROWS;
-    if (!C::PAIRED || a.sequences > 64 || a.sequences == 1) {
+    if (!C::ORDERED || a.sequences > 64 || a.sequences == 1) {
         n = rank % a.sequences;
         tile = tiles - 1 - rank / a.sequences;
         sq = span(a.q_starts, n, a.q_tokens), sk = span(a.k_starts, n, a.k_tokens);
@@ -544,7 +547,7 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
     const int tiles = (a.longest_q + C::ROWS - 1) / C::ROWS;
     // Tiles, at most, from what the host knows; a multiple of the XCDs' number.
     const std::int64_t by_longest = static_cast<std::int64_t>(tiles) * a.sequences;
-    const std::int64_t most = !C::PAIRED || a.sequences > 64 ? by_longest : std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / C::ROWS) + a.sequences);
+    const std::int64_t most = !C::ORDERED || a.sequences > 64 ? by_longest : std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / C::ROWS) + a.sequences);
     const std::int64_t grid = (most * a.q_heads + kXcds - 1) / kXcds * kXcds;
     require(launchable(grid, C::WAVES * 64), "attention_prompt", "too many sequences, heads and queries in one call");
     prompt_kernel<C><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles);
@@ -552,7 +555,8 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 
 // Workgroups of 128 queries, two a CU, read each key tile once for 128 queries
 // and balance well; they need two of them for every CU. Fewer queries are
-// given more waves by key groups, at first beside as many queries, then fewer.
+// given more waves by key groups, at first beside as many queries, then fewer:
+// 96 where those workgroups just fit the CUs, so that they all take part.
 // Tiles of 32 keys leave LDS for two buffers of four or eight groups; eight
 // groups take longer to start than they save on up to 512 keys.
 // us, the same work by the alternatives (16 query heads, causal):
@@ -565,12 +569,14 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 //     1..2040 packed            56.1   79.7   124    193   65.1
 //     4 x 2040                  85.8    105   159    264   91.9
 //     8160                       302    296   399    661    268
-//   heads of 64                (4,1)  (4,2)  (4,3)  (2,4)  (1,8)
-//     10 on 1500                                    13.2   11.7
-//     240                        9.2    9.0  11.4    8.0    7.6
-//     920                       17.2   14.7  16.1   11.2   15.9
-//     920 on 4600, 460 on 3001  62.5   47.5  44.5   54.4
-//     8160                       176    184   188    218
+//   heads of 64                (4,1)  (4,2)  (4,3)  (3,4)  (2,4)  (1,8)
+//     10 on 1500                                           13.2   11.7
+//     240                        9.2    9.0  11.4           8.0    7.6
+//     920                       17.2   14.7  16.1          11.2   15.9
+//     1400                                   20.2   17.9
+//     700 and 600, not causal                14.4   14.0
+//     920 on 4600, 460 on 3001  62.5   47.5  44.2   39.0   54.4
+//     8160                       176    184   188           218
 // 256 queries a workgroup halve the key traffic again, which pays where a
 // sequence is long enough for its last, partly seen tiles not to count.
 template <int D>
@@ -587,6 +593,7 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
         else launch_prompt<PromptCfg<64, 1, 4, 64, 2>>(a, s);
     }
     else if (workgroups(64) <= cus) launch_prompt<PromptCfg<D, 2, 4, D == 64 ? 64 : 32, 2>>(a, s);
+    else if (D == 64 && workgroups(96) <= cus) launch_prompt<PromptCfg<64, 3, 4, 64, 3>>(a, s);
     else if (D == 64 && workgroups(128) <= cus) launch_prompt<PromptCfg<64, 4, 3, 64, 3>>(a, s);
     else if (workgroups(128) <= 2 * cus) launch_prompt<PromptCfg<D, 4, 2, 64, 2>>(a, s);
     else if (D == 128 && a.longest_q >= 4096 && workgroups(128) >= 4 * cus && static_cast<std::int64_t>(a.longest_q) * a.sequences <= 2 * static_cast<std::int64_t>(a.q_tokens))

@@ -485,6 +485,30 @@ def test_prompt_many_ragged_sequences(dev, rng, dim, causal, sequences, q_heads,
             within(got[a, head:head + 1], want, tol)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("queries,keys,q_heads", [
+    ([700, 500], [1100, 500], 16),          # tiles that just fit the CUs
+    ([95, 0, 97, 960], [95, 300, 96, 960], 16),
+    ([450, 449, 1], [900, 3, 70], 24),
+])
+def test_prompt_tiles_that_fit_the_gpu(dev, rng, dim, causal, queries, keys, q_heads):
+    q = normal(rng, sum(queries), q_heads, dim)
+    k, v = normal(rng, sum(keys), 8, dim), normal(rng, sum(keys), 8, dim)
+    v[sum(keys) - 2, :, 5] = np.inf
+    got = Prompt(dev, q, k, v, queries, keys, causal, dim ** -0.5).run()
+    sq, sk = np.cumsum([0] + queries), np.cumsum([0] + keys)
+    columns = np.delete(np.arange(dim), 5)
+    assert np.isfinite(got[:, :, columns]).all()
+    for head in (0, q_heads - 1):
+        kv = head // (q_heads // 8)
+        for n in range(len(queries)):
+            a, b = slice(sq[n], sq[n + 1]), slice(sk[n], sk[n + 1])
+            want, tol = attend64(f64(q[a, head:head + 1]), f64(k[b, kv:kv + 1]), f64(v[b, kv:kv + 1]), dim ** -0.5, causal)
+            within(got[a, head:head + 1][:, :, columns], want[:, :, columns], tol[:, :, columns])
+            assert np.array_equal(np.isfinite(got[a, head, 5]), np.isfinite(want[:, 0, 5]))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("heads,dim,lengths", [
     (2, 64, [0, 30000, 1, 700]),          # one stream in many shares, others inside one
