@@ -561,12 +561,12 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void token_kernel(TokenArgs 
 }
 
 // One workgroup for a query head of a stream. LANES threads hold a part's row,
-// four values each, and the others take every (256 / LANES)-th part, each
+// four values each, and the others take every (THREADS / LANES)-th part, each
 // with a running maximum of its own; they are put together in LDS.
-template <int LANES>
-__global__ __launch_bounds__(256) void token_join_kernel(TokenArgs a)
+template <int LANES, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_join_kernel(TokenArgs a)
 {
-    constexpr int kGroups = 256 / LANES;
+    constexpr int kGroups = THREADS / LANES;
     __shared__ floatx4 sums[kGroups][LANES];
     __shared__ float2 states[kGroups];
     const int lane = threadIdx.x & 63, head = blockIdx.x % a.q_heads, stream = blockIdx.x / a.q_heads;
@@ -743,8 +743,15 @@ void attention_token(const mlvc_hip_attention_token_desc* d, hipStream_t s)
     else token_any_kernel<MLVC_KV_INT8><<<n, 64, 0, s>>>(a);
     check(hipGetLastError(), "attention_token launch");
     if (p.shares) {
-        if (a.dim <= 64) token_join_kernel<16><<<static_cast<unsigned>(heads), 256, 0, s>>>(a);
-        else token_join_kernel<32><<<static_cast<unsigned>(heads), 256, 0, s>>>(a);
+        const unsigned n = static_cast<unsigned>(heads);
+        // A stream of few parts is put together by one wave instead of four: 200
+        // streams of up to 8160 tokens 225.6 us instead of 230, 64 of up to 4080
+        // 62.1 instead of 64.0; 16 of up to 3001 the same.
+        const bool few = 2 * p.shares <= 8 * d->streams;
+        if (few && a.dim <= 64) token_join_kernel<16, 64><<<n, 64, 0, s>>>(a);
+        else if (few) token_join_kernel<32, 64><<<n, 64, 0, s>>>(a);
+        else if (a.dim <= 64) token_join_kernel<16, 256><<<n, 256, 0, s>>>(a);
+        else token_join_kernel<32, 256><<<n, 256, 0, s>>>(a);
         check(hipGetLastError(), "attention_token join launch");
     }
 }
