@@ -31,11 +31,12 @@ struct PromptArgs {
 struct Span {
     int first, count;
 };
-__device__ __forceinline__ Span span(const std::int32_t* starts, int n, int tokens)
+__device__ __forceinline__ Span span(int start, int end, int tokens)
 {
-    const int a = min(max(starts[n], 0), tokens), b = min(max(starts[n + 1], a), tokens);
+    const int a = min(max(start, 0), tokens), b = min(max(end, a), tokens);
     return {a, b - a};
 }
+__device__ __forceinline__ Span span(const std::int32_t* starts, int n, int tokens) { return span(starts[n], starts[n + 1], tokens); }
 
 // Any head size and alignment: one wave for a query of a head, 64 keys at a
 // time, one key a lane for the scores and one value column a lane for the sum.
@@ -186,7 +187,9 @@ __device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles,
     if (!C::ORDERED || a.sequences > 64 || a.sequences == 1) {
         n = rank % a.sequences;
         tile = tiles - 1 - rank / a.sequences;
-        sq = span(a.q_starts, n, a.q_tokens), sk = span(a.k_starts, n, a.k_tokens);
+        const int qa = a.q_starts[n], qb = a.q_starts[n + 1], ka = a.k_starts[n], kb = a.k_starts[n + 1];
+        asm volatile("" ::"s"(qa), "s"(qb), "s"(ka), "s"(kb));
+        sq = span(qa, qb, a.q_tokens), sk = span(ka, kb, a.k_tokens);
         return tile >= 0 && tile * ROWS < min(sq.count, a.longest_q);
     }
     const int lane = threadIdx.x & 63;
@@ -233,6 +236,10 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     // XCD's first workgroups take a CU each and the next ones join them in the
     // same order, so those come in the opposite one: the longest beside the
     // shortest.
+    // All arguments at once: each would be asked for where it is first used, one
+    // latency after another (0.2 to 0.7 us of a small call).
+    asm volatile("" ::"s"(a.q), "s"(a.k), "s"(a.v), "s"(a.out), "s"(a.q_stride), "s"(a.k_stride), "s"(a.v_stride), "s"(a.out_stride),
+                 "s"(a.q_starts), "s"(a.k_starts), "s"(a.sequences), "s"(a.q_heads), "s"(a.scale2), "s"(a.cus));
     int head, n, tile;
     Span sq, sk;
     {
