@@ -78,6 +78,20 @@ __device__ __forceinline__ std::uint32_t group_max(std::uint32_t x)
     else return x;
 }
 
+// Sum over this lane and those before it: rows of 16 lanes by shifts, then
+// each row's total to the rows after it.
+__device__ __forceinline__ int wave_scan(int x)
+{
+    constexpr int kShift = 0x110, kLast15 = 0x142, kLast31 = 0x143;
+    x += __builtin_amdgcn_update_dpp(0, x, kShift + 1, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, kShift + 2, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, kShift + 4, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, kShift + 8, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, kLast15, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, kLast31, 0xc, 0xf, false);
+    return x;
+}
+
 // 8-bit values of a cached row, widened. INT8 is two's complement.
 __device__ __forceinline__ float from_byte(int kind, std::uint8_t b)
 {

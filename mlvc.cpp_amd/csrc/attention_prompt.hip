@@ -178,13 +178,14 @@ struct PromptCfg {
 // sequence n has level base_n + t, in ROWS keys, and the tiles above a level are
 // counted for 64 levels at a time, one a lane (up to 64 sequences, one a lane
 // too). That takes half a microsecond, and takes 8 ragged sequences (1 to 2040
-// tokens, 16 heads of 128) from 64.5 to 57 us. Else by turns, sequence after
-// sequence within a tile number.
+// tokens, 16 heads of 128) from 64.5 to 57 us. More sequences follow one another,
+// each with its last tile first, 64 at a time. by_turns: sequence after sequence
+// within a tile number.
 template <class C>
-__device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles, int& n, int& tile, Span& sq, Span& sk)
+__device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles, bool by_turns, int& n, int& tile, Span& sq, Span& sk)
 {
     constexpr int ROWS = C::ROWS;
-    if (!C::ORDERED || a.sequences > 64 || a.sequences == 1) {
+    if (!C::ORDERED || by_turns) {
         n = rank % a.sequences;
         tile = tiles - 1 - rank / a.sequences;
         const int qa = a.q_starts[n], qb = a.q_starts[n + 1], ka = a.k_starts[n], kb = a.k_starts[n + 1];
@@ -193,6 +194,28 @@ __device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles,
         return tile >= 0 && tile * ROWS < min(sq.count, a.longest_q);
     }
     const int lane = threadIdx.x & 63;
+    if (C::PAIRED && a.sequences > 64) {
+        auto ends = [&](int i) {
+            return i < a.sequences ? make_int4(a.q_starts[i], a.q_starts[i + 1], a.k_starts[i], a.k_starts[i + 1]) : make_int4(0, 0, 0, 0);
+        };
+        int before = 0;
+        int4 next = ends(lane);
+        for (int b = 0; b < a.sequences; b += 64) {
+            const Span q = span(next.x, next.y, a.q_tokens), k = span(next.z, next.w, a.k_tokens);
+            next = ends(b + 64 + lane);
+            const int count = (min(q.count, a.longest_q) + ROWS - 1) / ROWS, upto = before + wave_scan(count);
+            const unsigned long long past = __ballot(upto > rank);
+            before = __builtin_amdgcn_readlane(upto, 63);
+            if (!past) continue;
+            const int i = __builtin_ctzll(past);
+            n = b + i;
+            tile = __builtin_amdgcn_readlane(upto, i) - 1 - rank;
+            sq = {__builtin_amdgcn_readlane(q.first, i), __builtin_amdgcn_readlane(q.count, i)};
+            sk = {__builtin_amdgcn_readlane(k.first, i), __builtin_amdgcn_readlane(k.count, i)};
+            return true;
+        }
+        return false;
+    }
     Span q = {0, 0}, k = {0, 0};
     if (lane < a.sequences) q = span(a.q_starts, lane, a.q_tokens), k = span(a.k_starts, lane, a.k_tokens);
     const int count = (min(q.count, a.longest_q) + ROWS - 1) / ROWS;
@@ -223,7 +246,7 @@ __device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles,
 }
 
 template <class C>
-__global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArgs a, int tiles)
+__global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArgs a, int tiles, bool by_turns)
 {
     constexpr int D = C::D, KS = D / 16, DT = D / 32, kKeys = C::KEYS, TT = kKeys / 32;
     extern __shared__ __attribute__((aligned(16))) std::uint16_t lds[];
@@ -258,7 +281,7 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
             head = i % a.q_heads;
             rank = i / a.q_heads;
         }
-        if (!choose<C>(a, rank, tiles, n, tile, sq, sk)) return;
+        if (!choose<C>(a, rank, tiles, by_turns, n, tile, sq, sk)) return;
     }
     const int q0 = tile * C::ROWS, nq = min(sq.count, a.longest_q);
     const int behind = sk.count - sq.count;  // keys before the first query
@@ -553,11 +576,16 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 {
     const int tiles = (a.longest_q + C::ROWS - 1) / C::ROWS;
     // Tiles, at most, from what the host knows; a multiple of the XCDs' number.
-    const std::int64_t by_longest = static_cast<std::int64_t>(tiles) * a.sequences;
-    const std::int64_t most = !C::ORDERED || a.sequences > 64 ? by_longest : std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / C::ROWS) + a.sequences);
+    // Many sequences go by turns where nearly all have as many tiles as the
+    // longest (70 of 200 tokens, 16 heads of 128: 59.7 us, one after the other
+    // 65), else one after the other (99 of 100 and one of 4080: 112 us, by
+    // turns 193; 200 of 30 to 240, heads of 64: 52 and 64).
+    const std::int64_t by_longest = static_cast<std::int64_t>(tiles) * a.sequences, full = a.q_tokens / C::ROWS;
+    const bool by_turns = !C::ORDERED || a.sequences == 1 || (a.sequences > 64 && (!C::PAIRED || by_longest <= full + a.sequences * 3LL / 4));
+    const std::int64_t most = by_turns ? by_longest : std::min(by_longest, full + a.sequences);
     const std::int64_t grid = (most * a.q_heads + kXcds - 1) / kXcds * kXcds;
     require(launchable(grid, C::WAVES * 64), "attention_prompt", "too many sequences, heads and queries in one call");
-    prompt_kernel<C><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles);
+    prompt_kernel<C><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles, by_turns);
 }
 
 // Workgroups of 128 queries, two a CU, read each key tile once for 128 queries

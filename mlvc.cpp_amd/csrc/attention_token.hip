@@ -51,20 +51,6 @@ __device__ __forceinline__ int steps_of(const TokenArgs& a, int stream)
     return stream < a.streams ? (context(a, stream) + kStep - 1) / kStep : 0;
 }
 
-// Sum over this lane and those before it: rows of 16 lanes by shifts, then
-// each row's total to the rows after it.
-__device__ __forceinline__ int wave_scan(int x)
-{
-    constexpr int kShift = 0x110, kLast15 = 0x142, kLast31 = 0x143;
-    x += __builtin_amdgcn_update_dpp(0, x, kShift + 1, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, kShift + 2, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, kShift + 4, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, kShift + 8, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, kLast15, 0xa, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, kLast31, 0xc, 0xf, false);
-    return x;
-}
-
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
 // The shares of a key head's steps: `shares` large ones, all on the GPU at

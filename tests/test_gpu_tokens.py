@@ -486,6 +486,20 @@ def test_prompt_many_ragged_sequences(dev, rng, dim, causal, sequences, q_heads,
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lengths", [[130] * 70, [5] * 129 + [700], [900] + [0, 1, 40] * 43])
+def test_prompt_more_sequences_than_lanes(dev, rng, dim, lengths):
+    """Alike ones, and a long one behind or before many short ones, over more than one and two waves' lanes."""
+    q, k, v = (normal(rng, sum(lengths), heads, dim) for heads in (10, 2, 2))
+    got = Prompt(dev, q, k, v, lengths, lengths, True, dim ** -0.5).run()
+    assert np.isfinite(got).all()
+    ends = np.cumsum([0] + lengths)
+    for n in range(len(lengths)):
+        at = slice(ends[n], ends[n + 1])
+        want, tol = attend64(f64(q[at, 7:8]), f64(k[at, 1:]), f64(v[at, 1:]), dim ** -0.5, True)
+        within(got[at, 7:8], want, tol)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("queries,keys,q_heads", [
     ([700, 500], [1100, 500], 16),          # tiles that just fit the CUs
