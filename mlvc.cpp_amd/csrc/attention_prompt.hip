@@ -155,9 +155,6 @@ struct PromptCfg {
     static constexpr int WAVES = RG * KG;
     // Several workgroups on a CU: long ones are put beside short ones.
     static constexpr bool PAIRED = KG == 1 && OCC * 4 / WAVES > 1;
-    // Tiles in the order of their keys, none that is not there: also where they
-    // just fit the CUs, and an empty one would take a CU's turn.
-    static constexpr bool ORDERED = PAIRED || RG == 3;
     static constexpr int ROWS = RG * 32;             // queries of a workgroup
     static constexpr int PIECES = D / 8;             // 16-byte pieces of a row
     static constexpr int DMA_ROWS = 64 / PIECES;     // rows of a DMA instruction
@@ -174,18 +171,20 @@ struct PromptCfg {
 };
 
 // The rank-th tile of queries; false past the last, and for one that is not
-// there. ORDERED: by the number of keys a tile may see, most first. Tile t of
-// sequence n has level base_n + t, in ROWS keys, and the tiles above a level are
-// counted for 64 levels at a time, one a lane (up to 64 sequences, one a lane
-// too). That takes half a microsecond, and takes 8 ragged sequences (1 to 2040
-// tokens, 16 heads of 128) from 64.5 to 57 us. More sequences follow one another,
-// each with its last tile first, 64 at a time. by_turns: sequence after sequence
-// within a tile number.
+// there. By the number of keys a tile may see, most first: tile t of sequence n
+// has level base_n + t, in ROWS keys, and the tiles above a level are counted
+// for 64 levels at a time, one a lane (up to 64 sequences, one a lane too).
+// That takes 0.3 us. 8 ragged sequences (1 to 2040 tokens, 16 heads of 128) take
+// 57 us instead of 64.5, and where tiles just fit the CUs, ones that are not
+// there take no CU's turn: one sequence of 2000 and three of 100 tokens 37.7
+// instead of 52, of 300 and 20 tokens 9.4 instead of 13.5. More sequences follow
+// one another, each with its last tile first, 64 at a time. by_turns: sequence
+// after sequence within a tile number.
 template <class C>
 __device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles, bool by_turns, int& n, int& tile, Span& sq, Span& sk)
 {
     constexpr int ROWS = C::ROWS;
-    if (!C::ORDERED || by_turns) {
+    if (by_turns) {
         n = rank % a.sequences;
         tile = tiles - 1 - rank / a.sequences;
         const int qa = a.q_starts[n], qb = a.q_starts[n + 1], ka = a.k_starts[n], kb = a.k_starts[n + 1];
@@ -194,7 +193,7 @@ __device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles,
         return tile >= 0 && tile * ROWS < min(sq.count, a.longest_q);
     }
     const int lane = threadIdx.x & 63;
-    if (C::PAIRED && a.sequences > 64) {
+    if (a.sequences > 64) {
         auto ends = [&](int i) {
             return i < a.sequences ? make_int4(a.q_starts[i], a.q_starts[i + 1], a.k_starts[i], a.k_starts[i + 1]) : make_int4(0, 0, 0, 0);
         };
@@ -581,7 +580,7 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
     // 65), else one after the other (99 of 100 and one of 4080: 112 us, by
     // turns 193; 200 of 30 to 240, heads of 64: 52 and 64).
     const std::int64_t by_longest = static_cast<std::int64_t>(tiles) * a.sequences, full = a.q_tokens / C::ROWS;
-    const bool by_turns = !C::ORDERED || a.sequences == 1 || (a.sequences > 64 && (!C::PAIRED || by_longest <= full + a.sequences * 3LL / 4));
+    const bool by_turns = a.sequences == 1 || (a.sequences > 64 && by_longest <= full + a.sequences * 3LL / 4);
     const std::int64_t most = by_turns ? by_longest : std::min(by_longest, full + a.sequences);
     const std::int64_t grid = (most * a.q_heads + kXcds - 1) / kXcds * kXcds;
     require(launchable(grid, C::WAVES * 64), "attention_prompt", "too many sequences, heads and queries in one call");
