@@ -622,7 +622,7 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
         return a.q_heads * std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / queries) + a.sequences);
     };
     if (workgroups(32) <= cus) {
-        if (D == 128) launch_prompt<PromptCfg<D, 1, 4, 32, 2>>(a, s);
+        if constexpr (D == 128) launch_prompt<PromptCfg<D, 1, 4, 32, 2>>(a, s);
         else if (a.k_tokens > 512LL * a.sequences) launch_prompt<PromptCfg<64, 1, 8, 32, 2>>(a, s);
         else launch_prompt<PromptCfg<64, 1, 4, 64, 2>>(a, s);
     }
