@@ -65,3 +65,59 @@ def test_no_single_rounding_mix_or_packed_fp32(disassembly):
             if m:
                 bad.add((kernel, m.group(1)))
     assert not bad, sorted(bad)[:20]
+
+
+# Wait states the hardware asks for before a buffer load and does not insert itself; the compiler inserts
+# them for its own instructions and cannot see into assembly. Scalar write of m0 before a load to LDS: 1;
+# vector write of a scalar register (a lane's value made uniform) before a load that reads it: 5.
+BUFFER_LOAD = re.compile(r"^buffer_load_\S+ (.*)$")
+SCALARS = re.compile(r"\bs(?:(\d+)\b|\[(\d+):(\d+)\])")
+
+
+def _scalars(text):
+    """Numbers of the scalar registers that a piece of assembly names."""
+    found = set()
+    for one, first, last in SCALARS.findall(text):
+        found.update(range(int(first or one), int(last or one) + 1))
+    return found
+
+
+def _missing_waits(text):
+    """(kernel, load, write before it) of every load that comes too soon after a write of what it reads."""
+    bad, kernel, before = [], None, []  # before: (instruction, wait states it stands for), latest last
+    for line in text.splitlines():
+        if line.endswith(">:"):
+            kernel, before = line.split("<", 1)[-1][:-2], []
+            continue
+        code = line.split("//")[0].strip()
+        if not line.startswith("\t") or not code:
+            continue
+        load = BUFFER_LOAD.match(code)
+        if load:
+            to_lds, reads, waited = code.endswith(" lds"), _scalars(load[1]), 0
+            for instruction, states in reversed(before):
+                name, _, operands = instruction.partition(" ")
+                target = operands.split(",")[0].strip()
+                if waited < 1 and to_lds and name.startswith("s_") and target == "m0":
+                    bad.append((kernel, code, instruction))
+                if waited < 5 and name.startswith("v_") and reads & _scalars(target):
+                    bad.append((kernel, code, instruction))
+                waited += states
+                if waited >= 5:
+                    break
+        nop = re.match(r"s_nop (\d+)$", code)
+        before = before[-5:] + [(code, int(nop[1]) + 1 if nop else 1)]
+    return bad
+
+
+def test_wait_states_are_counted():
+    code = "0 <k>:\n\ts_mov_b32 m0, s1 // 0\n\t%sbuffer_load_dwordx4 v1, s[4:7], 0 offen lds // 1\n"
+    assert _missing_waits(code % "") and not _missing_waits(code % "s_nop 0\n\t")
+    code = "0 <k>:\n\tv_readfirstlane_b32 s6, v2\n\ts_nop %d\n\tbuffer_load_dwordx4 v1, v2, s[4:7], 0 offen\n"
+    assert _missing_waits(code % 3) and not _missing_waits(code % 4)
+
+
+def test_loads_wait_for_their_scalar_operands(disassembly):
+    assert any(" lds\n" in t or " lds " in t for t in disassembly)
+    bad = [b for text in disassembly for b in _missing_waits(text)]
+    assert not bad, (len(bad), bad[:5])
