@@ -515,7 +515,9 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = fmaf(v[r], f, o[r]);
         }
-        const float back = KIND == MLVC_KV_F16 ? 1.0f : __builtin_amdgcn_exp2f(basew - base);
+        // From weights in powers above topw to powers above top. Where every value
+        // seen is zero (scale 0) there is no topw, and the sums are zero.
+        const float back = KIND == MLVC_KV_F16 ? 1.0f : topw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(basew - base);
         if (whole) {
             const float f = total == 0.0f ? 0.0f : back / total;
             *reinterpret_cast<uint2*>(a.out + stream * a.out_stride + static_cast<std::int64_t>(q_head + h) * D + d) =
