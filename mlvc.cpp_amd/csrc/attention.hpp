@@ -78,6 +78,17 @@ __device__ __forceinline__ std::uint32_t group_max(std::uint32_t x)
     else return x;
 }
 
+// Weights go to the matrix cores in FP16, as 2^(score - m) with a base m of the
+// running softmax that lies kLift powers of two below a score: FP16's numbers
+// end at 2^-24, so with the largest weight at 2^12 or more one of 2^-26 of it
+// keeps all its bits, and what is lost below is 2^-37 of it. The base follows
+// once a score is kMost above it; FP16 ends at 2^16.
+constexpr float kLift = 12.0f, kMost = 15.0f;
+
+// The base for a largest score. From 2^22 on scores are too coarse to lie 12
+// below one another, and the score itself is the base.
+__device__ __forceinline__ float lifted(float top) { return fabsf(top) < 0x1p22f ? top - kLift : top; }
+
 // Sum over this lane and those before it: rows of 16 lanes by shifts, then
 // each row's total to the rows after it.
 __device__ __forceinline__ int wave_scan(int x)

@@ -205,8 +205,6 @@ __global__ __launch_bounds__(64) void token_any_kernel(TokenArgs a)
 
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr float kSlack = 8.0f;  // powers of two a score may pass the running maximum before it moves
-
 // Largest of a value over the four lanes of a column (16 apart).
 __device__ __forceinline__ float column_max(float x) { return fmaxf(fmaxf(x, __shfl_xor(x, 16)), fmaxf(__shfl_xor(x, 32), __shfl_xor(x, 48))); }
 __device__ __forceinline__ float column_sum(float x)
@@ -277,10 +275,11 @@ __device__ __forceinline__ void columns(std::uint32_t a, std::uint32_t b, std::u
 //
 // Scales are applied to scores and weights, not to values: s = (q . k) scale_k,
 // and the weight of a row of V is 2^(s + log2(scale_v) - mw) with a running
-// maximum mw of its own, so weights keep FP16's precision whatever the
-// scales. They go in as two halves, w and the rounding's remainder: the
-// products are few next to the bytes, and the result is as exact as the plain
-// FP32 form.
+// base mw of its own, so weights keep FP16's precision whatever the scales.
+// They go in as two halves, w and the rounding's remainder: the products are
+// few next to the bytes. A weight is off by 2^-22 of itself or, as both halves
+// end at 2^-24 and the largest weight is given as 2^12 at least (kLift), by
+// 2^-37 of the largest: 2^-21 of the values in a context of 65536.
 //
 // Bound by the bytes of the cache: 64 streams of 1 to 8160 tokens, 32 query
 // heads on 8 of 128, INT8, 0.55 GB in 112 us or 4.9 TB/s; one stream of 65280
@@ -448,11 +447,11 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
 #pragma unroll
             for (int e = 1; e < 8; ++e) topw = __builtin_elementwise_maximum(topw, y[e]);
         }
-        if (__any(top > m + kSlack || topw > mw + kSlack)) {
-            const float now = fmaxf(m, column_max(top));
+        if (__any(top - m > kMost || topw - mw > kMost)) {
+            const float now = fmaxf(m, lifted(column_max(top)));
             l *= __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
             m = now;
-            const float noww = KIND == MLVC_KV_F16 ? now : fmaxf(mw, column_max(topw));
+            const float noww = KIND == MLVC_KV_F16 ? now : fmaxf(mw, lifted(column_max(topw)));
             const float keep = __builtin_amdgcn_exp2f(mw - (noww == -INFINITY ? 0.0f : noww));
             mw = noww;
 #pragma unroll

@@ -61,3 +61,52 @@ def test_tokens_beside_a_stretch_of_zero_values(dev, rng, kind, dim):
     cache, table = _context(dev, rng, kind, k, v)
     want, tol = attend64(f64(q), stored64(k, kind), stored64(v, kind), dim ** -0.5, False)
     within(Token(cache, q, table, [n], dim ** -0.5).run(), want, tol)
+
+
+# ------------------------------------------------------------ small weights
+
+# The matrix kernels give weights to the matrix cores in FP16, the largest as at
+# least 2^12: below 2^-14, a quantum of 2^-24. So a weight is off by half of
+# that, 2^-37 of the largest, beside its rounding of 2^-11 (2^-22 with a
+# remainder).
+LEAST = 2.0 ** -37
+
+
+def _beside_a_sink(n, heads, dim):
+    """Query, keys and values: key 0 has the score 0 and a value in column 0 only, all others a score 17.7
+    lower (2^-25.5 of its weight) and values from 0.5 to 1.5."""
+    q = np.ones((1, 1, dim), np.float16)
+    k = np.full((n, heads, dim), -17.7 / 8 / dim ** 0.5, np.float16)
+    v = np.random.default_rng(9).uniform(0.5, 1.5, (n, heads, dim)).astype(np.float16)
+    k[0], v[0], v[0, :, 0] = 0, 0, 1
+    return q, k, v
+
+
+def _weighed(k, q, v, scale, rounding, least):
+    """(result, tolerance) of one query [dim] on keys and values [n, dim] for weights off by `rounding` of
+    themselves and by least[j] of the largest weight."""
+    s = k @ q * scale
+    p = np.exp(s - s.max())
+    w, out = p / p.sum(), p @ v / p.sum()
+    # Scores: FP32 products and sums of dim terms, the exponent's rounding; FP32 sums of n terms.
+    ds = (np.abs(k) @ np.abs(q)) * abs(scale) * (len(q) + 4) * 2.0 ** -24 + np.abs(s) * 2.0 ** -22 + 2.0 ** -21
+    off = w * (rounding + 2 * ds) + least / p.sum()
+    tol = np.abs(out) * 2.0 ** -11 + 2.0 ** -25 + off @ (np.abs(v) + np.abs(out)) + (len(p) + 8) * 2.0 ** -24 * (w @ np.abs(v))
+    return out, tol
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [900, 8160, 65280])
+def test_tokens_of_small_weights(dev, rng, kind, dim, n):
+    """Thousands of tokens that matter together and not each, beside one that dominates the sum of weights."""
+    q, k, v = _beside_a_sink(n, 1, dim)
+    cache, table = _context(dev, rng, kind, k, v)
+    k, v = stored64(k, kind)[:, 0], stored64(v, kind)[:, 0]
+    scale = dim ** -0.5 * 8
+    # With a quantised cache a weight is scaled by its value's scale, and the largest of those counts.
+    units = np.ones(n) if kind == KV_F16 else np.abs(v).max(-1) / (448 if kind == KV_E4M3 else 127)
+    p = np.exp(k @ f64(q[0, 0]) * scale)
+    # Exponents, with the scale's logarithm, are up to 2^6 in FP32: two roundings of 2^-19, times ln 2.
+    want, tol = _weighed(k, f64(q[0, 0]), v, scale, 2.0 ** -22 + 2.0 ** -18, LEAST * (p * units).max() / units / p.max())
+    within(Token(cache, q, table, [n], scale).run()[0, 0], want, tol)
