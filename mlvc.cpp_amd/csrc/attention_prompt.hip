@@ -99,7 +99,6 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kRawBufferFlags = 0x00020000;
 constexpr int kProducts = 0x8, kReads = 0x100;  // instruction groups of sched_group_barrier: MFMA, LDS reads
-constexpr float kSlack = 8.0f;     // how far, in powers of two, a score may pass the running maximum before it moves
 
 __device__ __forceinline__ std::uint32_t uniform(std::uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 
@@ -149,10 +148,11 @@ __device__ __forceinline__ float both_sum(float x)
 // rows by 16 bytes, V by the transposing read. Rows past a sequence's end are
 // out of the buffer's range and read as zeros.
 //
-// The running maximum moves only when a score passes it by 2^8 (weights up to
-// 2^8 lose nothing in FP16 or in the FP32 sums), so the accumulators are seldom
-// rescaled. Weights are rounded to FP16, the type the matrix cores take beside
-// V: one rounding of 2^-11 each, no more than the output's own.
+// The base of the weights lies 12 powers of two below a score and moves only
+// when one passes it by 15 (FP16 and the FP32 sums hold weights up to 2^15), so
+// the accumulators are seldom rescaled. Weights are rounded to FP16, the type
+// the matrix cores take beside V: by 2^-11 of themselves, as the output is, or
+// by 2^-37 of the largest where they are subnormal. Their sum is of FP32 values.
 template <int D_, int RG_, int KG_, int KEYS_, int OCC_>
 struct PromptCfg {
     static constexpr int D = D_, RG = RG_, KG = KG_, KEYS = KEYS_, OCC = OCC_;
@@ -405,8 +405,8 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
             float top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(tops[0], s[0][15]),
                                                       __builtin_elementwise_maximum(tops[TT - 1], s[TT - 1][15]));
             top = both_max(top) * a.scale2;
-            if (__any(top > m + kSlack)) {
-                const float now = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
+            if (__any(top - m > kMost)) {
+                const float now = fmaxf(m, lifted(top)), keep = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
                 m = now;
                 l *= keep;
 #pragma unroll

@@ -110,3 +110,27 @@ def test_tokens_of_small_weights(dev, rng, kind, dim, n):
     # Exponents, with the scale's logarithm, are up to 2^6 in FP32: two roundings of 2^-19, times ln 2.
     want, tol = _weighed(k, f64(q[0, 0]), v, scale, 2.0 ** -22 + 2.0 ** -18, LEAST * (p * units).max() / units / p.max())
     within(Token(cache, q, table, [n], scale).run()[0, 0], want, tol)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("queries,keys,q_heads", [
+    ([4], [3001], 4), ([4], [400], 4), ([130], [1300], 64), ([261], [1261], 64), ([200, 77], [933, 1050], 64),
+    ([530], [1700], 64), ([1100, 3], [1100, 2065], 64), ([4100], [4100], 32),
+])
+def test_prompt_of_small_weights(dev, rng, queries, keys, q_heads, dim, causal):
+    """The same in every tile shape, the dominating key first in each sequence."""
+    parts = [_beside_a_sink(n, 2, dim) for n in keys]
+    k, v = (np.concatenate([p[i] for p in parts]) for i in (1, 2))
+    q = np.ones((sum(queries), q_heads, dim), np.float16)
+    scale = dim ** -0.5 * 8
+    got = Prompt(dev, q, k, v, queries, keys, causal, scale).run()
+    i = j = 0
+    for nq, nk in zip(queries, keys):
+        for r in np.unique(np.r_[0, nq // 2, nq - 1]):
+            n = nk - nq + r + 1 if causal else nk
+            for head in (0, q_heads - 1):
+                at = slice(j, j + n), head // (q_heads // 2)
+                want, tol = _weighed(f64(k[at]), f64(q[0, 0]), f64(v[at]), scale, 2.0 ** -11, LEAST)
+                within(got[i + r, head], want, tol, f"query {r} of {nq} on {nk}, head {head}")
+        i, j = i + nq, j + nk
