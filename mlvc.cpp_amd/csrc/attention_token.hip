@@ -274,8 +274,10 @@ __device__ __forceinline__ void columns(std::uint32_t a, std::uint32_t b, std::u
 // conversion to halves, which takes one column of two rows at a time.
 //
 // Scales are applied to scores and weights, not to values: s = (q . k) scale_k,
-// and the weight of a row of V is 2^(s + log2(scale_v) - mw) with a running
-// base mw of its own, so weights keep FP16's precision whatever the scales.
+// and the weight of a row of V is 2^(s - m + log2(scale_v) - mw) with a running
+// base mw of its own on top of m, so weights keep FP16's precision whatever the
+// scales, and the logarithm its bits whatever the scores. It is -inf while all
+// values seen are zero (scale 0).
 // They go in as two halves, w and the rounding's remainder: the products are
 // few next to the bytes. A weight is off by 2^-22 of itself or, as both halves
 // end at 2^-24 and the largest weight is given as 2^12 at least (kLift), by
@@ -404,6 +406,7 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
     // K of the next step is asked for as soon as this step's has been used, V
     // likewise, so a wave always has about a step of the cache in flight.
     for (int j = from; j < to; j += kStride) {
+#pragma clang fp contract(off)  // a score less the base: of the score as it was when the base was taken
         floatx4 dot[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -420,7 +423,7 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
             x[e] = dot[e >> 2][e & 3] * a.scale2;
             if constexpr (KIND != MLVC_KV_F16) {
                 x[e] *= ks[e >> 2][e & 3];
-                y[e] = x[e] + __builtin_amdgcn_logf(vs[e >> 2][e & 3]);
+                y[e] = __builtin_amdgcn_logf(vs[e >> 2][e & 3]);
             }
         }
         const bool ragged = j + kStep > to || !there[0] || !there[1];
@@ -434,36 +437,49 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
             for (int e = 0; e < 8; ++e)
                 if (!seen[e >> 2] || j + 16 * (e >> 2) + 4 * g + (e & 3) >= to) {
                     // Not seen: weight zero, and a value that is finite whatever lies there.
-                    x[e] = y[e] = -INFINITY;
+                    x[e] = -INFINITY, y[e] = 0.0f;
 #pragma unroll
                     for (int w = 0; w < C::VW; ++w) v[e][w] = 0;
                 }
         }
-        float top = x[0], topw = -INFINITY;
-#pragma unroll
-        for (int e = 1; e < 8; ++e) top = __builtin_elementwise_maximum(top, x[e]);
-        if constexpr (KIND != MLVC_KV_F16) {
-            topw = y[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) topw = __builtin_elementwise_maximum(topw, y[e]);
-        }
-        if (__any(top - m > kMost || topw - mw > kMost)) {
-            const float now = fmaxf(m, lifted(column_max(top)));
-            l *= __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
-            m = now;
-            const float noww = KIND == MLVC_KV_F16 ? now : fmaxf(mw, lifted(column_max(topw)));
-            const float keep = __builtin_amdgcn_exp2f(mw - (noww == -INFINITY ? 0.0f : noww));
-            mw = noww;
+        auto rescale = [&](float keep) {
 #pragma unroll
             for (int i = 0; i < C::DT; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[i][r] *= keep;
+        };
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top = __builtin_elementwise_maximum(top, x[e]);
+        if (__any(top - m > kMost)) {
+            const float now = fmaxf(m, lifted(column_max(top))), keep = __builtin_amdgcn_exp2f(m - (now == -INFINITY ? 0.0f : now));
+            l *= keep;
+            if constexpr (KIND == MLVC_KV_F16) rescale(keep);
+            else if (m != -INFINITY) mw += m - now;
+            m = now;
         }
-        const float base = m == -INFINITY ? 0.0f : m, basew = mw == -INFINITY ? 0.0f : mw;
+        const float base = m == -INFINITY ? 0.0f : m;
+        float basew = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] -= base;
+        if constexpr (KIND != MLVC_KV_F16) {
+            float topw = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[e] += x[e];
+                topw = __builtin_elementwise_maximum(topw, y[e]);
+            }
+            if (__any(topw - mw > kMost)) {
+                const float now = fmaxf(mw, lifted(column_max(topw)));
+                rescale(__builtin_amdgcn_exp2f(mw - (now == -INFINITY ? 0.0f : now)));
+                mw = now;
+            }
+            if (mw != -INFINITY) basew = mw;
+        }
         half8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float p = __builtin_amdgcn_exp2f(x[e] - base);
+            const float p = __builtin_amdgcn_exp2f(x[e]);
             l += p;
             const float w = KIND == MLVC_KV_F16 ? p : __builtin_amdgcn_exp2f(y[e] - basew);
             hi[e] = static_cast<_Float16>(w);
@@ -500,31 +516,27 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
     __syncthreads();
     for (int i = threadIdx.x; i < mine * (D / 4); i += C::WAVES * 64) {
         const int h = i / (D / 4), d = i % (D / 4) * 4;
-        float top = -INFINITY, topw = -INFINITY;
+        float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < C::WAVES; ++w) top = fmaxf(top, st[w * 16 + h]), topw = fmaxf(topw, st[(2 * C::WAVES + w) * 16 + h]);
-        const float base = top == -INFINITY ? 0.0f : top, basew = topw == -INFINITY ? 0.0f : topw;
+        for (int w = 0; w < C::WAVES; ++w) top = fmaxf(top, st[w * 16 + h]);
+        const float base = top == -INFINITY ? 0.0f : top;
         float total = 0.0f;
         floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < C::WAVES; ++w) {
-            total += st[(C::WAVES + w) * 16 + h] * __builtin_amdgcn_exp2f(st[w * 16 + h] - base);
-            const float f = __builtin_amdgcn_exp2f(st[(2 * C::WAVES + w) * 16 + h] - basew);
+            float f = __builtin_amdgcn_exp2f(st[w * 16 + h] - base);
+            total += st[(C::WAVES + w) * 16 + h] * f;
+            if constexpr (KIND != MLVC_KV_F16) f *= __builtin_amdgcn_exp2f(st[(2 * C::WAVES + w) * 16 + h]);
             const floatx4 v = *reinterpret_cast<const floatx4*>(joint + (w * mine + h) * D + d);
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = fmaf(v[r], f, o[r]);
         }
-        // From weights in powers above topw to powers above top. Where every value
-        // seen is zero (scale 0) there is no topw, and the sums are zero.
-        const float back = KIND == MLVC_KV_F16 ? 1.0f : topw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(basew - base);
         if (whole) {
-            const float f = total == 0.0f ? 0.0f : back / total;
+            const float f = total == 0.0f ? 0.0f : 1.0f / total;
             *reinterpret_cast<uint2*>(a.out + stream * a.out_stride + static_cast<std::int64_t>(q_head + h) * D + d) =
                 make_uint2(pack_rounded(o[0] * f, o[1] * f), pack_rounded(o[2] * f, o[3] * f));
         } else {
             const std::int64_t slot = static_cast<std::int64_t>(q_head + h) * (2 * a.shares + a.streams) + place_of_part;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] *= back;
             *reinterpret_cast<floatx4*>(a.part + slot * D + d) = o;
             if (d == 0) a.state[slot] = make_float2(top, total);
         }

@@ -134,3 +134,33 @@ def test_prompt_of_small_weights(dev, rng, queries, keys, q_heads, dim, causal):
                 want, tol = _weighed(f64(k[at]), f64(q[0, 0]), f64(v[at]), scale, 2.0 ** -11, LEAST)
                 within(got[i + r, head], want, tol, f"query {r} of {nq} on {nk}, head {head}")
         i, j = i + nq, j + nk
+
+
+# ------------------------------------------------------------ large scores
+
+def _far_apart(rng, n, heads, dim):
+    """Keys of one value throughout, different ones 16 apart at least; two largest ones, alike."""
+    size = rng.permutation(n).astype(np.float16) * np.float16(24)
+    order = np.argsort(size)
+    size[order[-2]] = size[order[-1]]
+    k = np.repeat(size, heads * dim).reshape(n, heads, dim)
+    return k, normal(rng, n, heads, dim), size
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("size", [0.5, 4.0, 60.0, 60000.0, -60000.0])
+@pytest.mark.parametrize("n", [900, 2600])
+def test_tokens_of_large_scores(dev, rng, kind, dim, size, n):
+    k, v, sizes = _far_apart(rng, n, 1, dim)
+    cache, table = _context(dev, rng, kind, k, v)
+    q = np.full((1, 4, dim), size, np.float16)
+    seen = sizes * np.sign(size)
+    at = np.flatnonzero(seen == seen.max())
+    v = stored64(v, kind)[at, 0]
+    want = v.mean(0)
+    got = Token(cache, q, table, [n], 1.0).run()
+    # Beside the result's rounding, a weight through the logarithm of its value's scale: an exponent of up to
+    # 2^6 in FP32, off by 2^-18 from the logarithm and 2^-19 from either of two sums.
+    for head in range(4):
+        within(got[0, head], want, np.abs(want) * 2.0 ** -11 + np.abs(v).mean(0) * 2.0 ** -17 + 2.0 ** -25)
