@@ -85,9 +85,10 @@ __device__ __forceinline__ std::uint32_t group_max(std::uint32_t x)
 // once a score is kMost above it; FP16 ends at 2^16.
 constexpr float kLift = 12.0f, kMost = 15.0f;
 
-// The base for a largest score. From 2^22 on scores are too coarse to lie 12
-// below one another, and the score itself is the base.
-__device__ __forceinline__ float lifted(float top) { return fabsf(top) < 0x1p22f ? top - kLift : top; }
+// The base for a largest score. From kCoarse on FP32's scores are too coarse to
+// lie 12 below one another, and the score itself is the base.
+constexpr float kCoarse = 0x1p22f;
+__device__ __forceinline__ float lifted(float top) { return fabsf(top) < kCoarse ? top - kLift : top; }
 
 // Sum over this lane and those before it: rows of 16 lanes by shifts, then
 // each row's total to the rows after it.

@@ -164,3 +164,23 @@ def test_tokens_of_large_scores(dev, rng, kind, dim, size, n):
     # 2^6 in FP32, off by 2^-18 from the logarithm and 2^-19 from either of two sums.
     for head in range(4):
         within(got[0, head], want, np.abs(want) * 2.0 ** -11 + np.abs(v).mean(0) * 2.0 ** -17 + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("size", [0.5, 4.0, 60.0, 60000.0, -60000.0])
+@pytest.mark.parametrize("queries,keys,q_heads", [([3], [900], 4), ([530], [1700], 64), ([1100], [1100], 64)])
+def test_prompt_of_large_scores(dev, rng, queries, keys, q_heads, dim, causal, size):
+    """Scores up to 2^36, further apart than FP32's rounding of them: the largest key's value, or the mean of two."""
+    n, nq = keys[0], queries[0]
+    k, v, sizes = _far_apart(rng, n, 2, dim)
+    q = np.full((nq, q_heads, dim), size, np.float16)
+    got = Prompt(dev, q, k, v, queries, keys, causal, 1.0).run()
+    for r in np.unique(np.r_[0, nq // 2, nq - 1, rng.integers(0, nq, 5)]):
+        seen = sizes[:n - nq + r + 1 if causal else n] * np.sign(size)
+        at = np.flatnonzero(seen == seen.max())
+        for head in (0, q_heads - 1):
+            # Alike weights, rounded to FP16 alike, over a sum that is not; then the result's rounding.
+            want = f64(v[at, head // (q_heads // 2)]).mean(0)
+            within(got[r, head], want, np.abs(want) * (2.0 ** -10 + 2.0 ** -20) + 2.0 ** -25, f"query {r}, head {head}")
+
