@@ -488,7 +488,9 @@ int mlvc_hip_attention_prompt(const mlvc_hip_attention_prompt_desc* desc, mlvc_h
 
 /* Attention of one query per stream on the stream's cached context: stream n
  * sees lengths[n] tokens, token j in page table[n][j / page_size]. A length of
- * zero gives zeros; tokens of pages outside the cache are not seen. Long
+ * zero gives zeros; tokens of pages outside the cache are not seen. An infinity
+ * among the values seen is the result, however small its weight, and NaN beside
+ * its opposite (an MLVC_KV_F16 cache; a quantised row that held one is NaN). Long
  * contexts are split over workgroups, which leave FP32 partials in the
  * workspace that a second kernel joins in a fixed order. Where a context is cut
  * follows from all lengths of the call: a stream's result may differ in its

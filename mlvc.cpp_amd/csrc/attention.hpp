@@ -90,6 +90,23 @@ constexpr float kLift = 12.0f, kMost = 15.0f;
 constexpr float kCoarse = 0x1p22f;
 __device__ __forceinline__ float lifted(float top) { return fabsf(top) < kCoarse ? top - kLift : top; }
 
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }
+
+// The infinities and NaN among the values of a sum with weights above 0. In
+// numbers of few bits a weight may be 0, and its product with one of them NaN:
+// every sum that holds one ends as infinite or NaN and is then decided by these.
+struct OddValues {
+    unsigned seen = 0;  // 1: +inf, 2: -inf, 4: NaN
+    __device__ void add(std::uint16_t v)
+    {
+        if ((v & 0x7c00u) == 0x7c00u) seen |= (v & 0x3ffu) ? 4u : (v & 0x8000u) ? 2u : 1u;
+    }
+    __device__ float sum(float otherwise) const
+    {
+        return seen == 0 ? otherwise : seen == 1 ? INFINITY : seen == 2 ? -INFINITY : __builtin_nanf("");
+    }
+};
+
 // Sum over this lane and those before it: rows of 16 lanes by shifts, then
 // each row's total to the rows after it.
 __device__ __forceinline__ int wave_scan(int x)

@@ -130,6 +130,28 @@ __device__ __forceinline__ void each_piece(const TokenArgs& a, int share, F&& fn
     }
 }
 
+// Row of token j of a stream's context, or -1 where its page is not in the cache.
+__device__ __forceinline__ std::int64_t token_row(const TokenArgs& a, int stream, int head, int j)
+{
+    const int page = a.table[static_cast<std::int64_t>(stream) * a.table_stride + j / a.page];
+    return page < 0 || page >= a.pages ? -1 : (static_cast<std::int64_t>(page) * a.heads + head) * a.page + j % a.page;
+}
+
+// Sums of FP16 values of tokens [first, last), N columns from d on, one of which came out as infinite or NaN.
+template <int N, typename T>
+__device__ __forceinline__ void decide_odd(const TokenArgs& a, int stream, int head, int first, int last, int d, T& sums)
+{
+    OddValues odd[N];
+    for (int j = first; j < last; ++j) {
+        const std::int64_t row = token_row(a, stream, head, j);
+        if (row < 0) continue;
+#pragma unroll
+        for (int r = 0; r < N; ++r) odd[r].add(reinterpret_cast<const std::uint16_t*>(a.v)[row * a.dim + d + r]);
+    }
+#pragma unroll
+    for (int r = 0; r < N; ++r) sums[r] = odd[r].sum(sums[r]);
+}
+
 // Any head size: one wave for a piece of one query head's context, 64 tokens
 // at a time, one token a lane for the scores and one value column a lane for
 // the sum.
@@ -151,11 +173,7 @@ __global__ __launch_bounds__(64) void token_any_kernel(TokenArgs a)
         float acc[kColumns] = {}, m = -INFINITY, l = 0.0f;
         for (int j0 = first; j0 < last; j0 += 64) {
             const int j = j0 + lane;
-            long long row = -1;
-            if (j < last) {
-                const int page = a.table[static_cast<std::int64_t>(stream) * a.table_stride + j / a.page];
-                if (page >= 0 && page < a.pages) row = (static_cast<long long>(page) * a.heads + head / a.group) * a.page + j % a.page;
-            }
+            const long long row = j < last ? token_row(a, stream, head / a.group, j) : -1;
             float s = -INFINITY;
             if (row >= 0) {
                 s = 0.0f;
@@ -182,6 +200,14 @@ __global__ __launch_bounds__(64) void token_any_kernel(TokenArgs a)
                 acc[c] = sum;
             }
             __syncthreads();
+        }
+        if constexpr (KIND == MLVC_KV_F16) {
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c) {
+                float sum[1] = {acc[c]};
+                if (c * 64 + lane < a.dim && !is_finite(sum[0])) decide_odd<1>(a, stream, head / a.group, first, last, c * 64 + lane, sum);
+                acc[c] = sum[0];
+            }
         }
         if (whole) {
             const float r = l == 0.0f ? 0.0f : 1.0f / l;
@@ -531,6 +557,8 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = fmaf(v[r], f, o[r]);
         }
+        if constexpr (KIND == MLVC_KV_F16)
+            if (!is_finite(o[0]) || !is_finite(o[1]) || !is_finite(o[2]) || !is_finite(o[3])) decide_odd<4>(a, stream, head, first, last, d, o);
         if (whole) {
             const float f = total == 0.0f ? 0.0f : 1.0f / total;
             *reinterpret_cast<uint2*>(a.out + stream * a.out_stride + static_cast<std::int64_t>(q_head + h) * D + d) =
@@ -615,6 +643,17 @@ __global__ __launch_bounds__(THREADS) void token_join_kernel(TokenArgs a)
                 l += st.y * f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sum[r] = fmaf(sums[i][at][r], f, sum[r]);
+            }
+            // A part that is infinite, with however small a weight.
+            if (!is_finite(sum[0]) || !is_finite(sum[1]) || !is_finite(sum[2]) || !is_finite(sum[3])) {
+                floatx4 odd = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int i = 0; i < parts; ++i) {
+                    const floatx4 v = *reinterpret_cast<const floatx4*>(a.part + (slot + i) * a.dim + d);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) odd[r] += is_finite(v[r]) ? 0.0f : v[r];
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum[r] = is_finite(sum[r]) ? sum[r] : odd[r];
             }
             const float f = l == 0.0f ? 0.0f : 1.0f / l;
             std::uint16_t* out = a.out + stream * a.out_stride + static_cast<std::int64_t>(head) * a.dim + d;

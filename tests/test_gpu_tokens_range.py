@@ -184,3 +184,64 @@ def test_prompt_of_large_scores(dev, rng, queries, keys, q_heads, dim, causal, s
             want = f64(v[at, head // (q_heads // 2)]).mean(0)
             within(got[r, head], want, np.abs(want) * (2.0 ** -10 + 2.0 ** -20) + 2.0 ** -25, f"query {r}, head {head}")
 
+
+
+# ------------------------------------------------------------ infinities
+
+def _with_odd_values(rng, n, heads, dim, peaked):
+    """Keys, values with infinities and NaN, the values without them, and what each column of head 0 holds:
+    {column: [(place, value), ...]}. One odd value's key has a score far below all others; peaked: the last
+    key's lies far above, so that every other weight is 0 in FP32."""
+    k, v = normal(rng, n, heads, dim), normal(rng, n, heads, dim)
+    k[n // 2] = -60
+    if peaked:
+        k[n - 1] = 60
+    odd = {5: [(3, np.inf)], 9: [(n - 1, -np.inf)], 20: [(n // 3, np.nan)], 30: [(6, np.inf), (n - 2, -np.inf)],
+           40: [(n // 2, -np.inf)], dim - 1: [(n // 2, np.inf), (0, np.inf)]}
+    clean = v.copy()
+    for column, places in odd.items():
+        for at, x in places:
+            v[at, 0, column], clean[at, 0, column] = x, 0
+    return k, v, clean, odd
+
+
+def _sum_of(seen):
+    """A weighted sum of such values: however small a weight, it is not 0."""
+    return np.float64(0) + sum(np.float64(x) for x in seen)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("n", [40, 900, 5000])
+@pytest.mark.parametrize("peaked", [False, True])
+@pytest.mark.parametrize("extra,shift", [(0, 0), (0, 1)])
+def test_tokens_of_infinite_values(dev, rng, dim, n, peaked, extra, shift):
+    """An FP16 cache: a seen infinity is the result, opposite ones and NaN are NaN, in their columns and head only."""
+    k, v, clean, odd = _with_odd_values(rng, n, 2, dim, peaked)
+    q = normal(rng, 1, 4, dim) * np.float16(0.1) + np.float16(4)
+    cache, table = _context(dev, rng, KV_F16, k, v)
+    got = Token(cache, q, table, [n], dim ** -0.5, extra=extra, shift=shift).run()
+    want, tol = attend64(f64(q), f64(k), f64(clean), dim ** -0.5, False)
+    with np.errstate(invalid="ignore"):
+        for column, places in odd.items():
+            want[0, :2, column] = _sum_of(x for _, x in places)
+    with np.errstate(invalid="ignore"):
+        within(got, want, tol)
+    same = np.isinf(want)
+    assert np.array_equal(np.isnan(want), np.isnan(got)) and np.array_equal(got[same], want[same])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("n", [40, 5000])
+def test_tokens_of_infinite_keys(dev, rng, dim, n):
+    """An FP16 cache: a key with an infinity scores +inf (NaN) or -inf (not there), by the sign of the query's value."""
+    k, v, q = normal(rng, n, 1, dim), normal(rng, n, 1, dim), normal(rng, 1, 4, dim)
+    k[7, 0, 3] = np.inf
+    q[0, :, 3] = [1, -1, 2, -2]
+    cache, table = _context(dev, rng, KV_F16, k, v)
+    got = Token(cache, q, table, [n], dim ** -0.5).run()
+    rest = np.arange(n) != 7
+    want, tol = attend64(f64(q), f64(k[rest]), f64(v[rest]), dim ** -0.5, False)
+    want[0, ::2] = np.nan
+    with np.errstate(invalid="ignore"):
+        within(got, want, tol)
+    assert np.isnan(got[0, ::2]).all()
