@@ -469,7 +469,9 @@ int mlvc_hip_kv_read(const mlvc_hip_kv_cache* cache, const mlvc_hip_kv_rows* row
  * with causal a query sees the keys up to its own place only. A query that
  * sees no key gives zeros. Query head h reads key head h * kv_heads / q_heads.
  * What a query does not see (keys past its place, other sequences' rows) never
- * reaches its output, infinities and NaN included. */
+ * reaches its output, infinities and NaN included. An infinity among the values
+ * that it sees is the result, however small its weight, and NaN beside its
+ * opposite. */
 typedef struct mlvc_hip_attention_prompt_desc {
     int sequences, q_heads, kv_heads, head_dim; /* q_heads a multiple of kv_heads; head_dim 1..512 */
     const void* q;

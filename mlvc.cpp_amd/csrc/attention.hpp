@@ -96,11 +96,10 @@ __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY;
 // numbers of few bits a weight may be 0, and its product with one of them NaN:
 // every sum that holds one ends as infinite or NaN and is then decided by these.
 struct OddValues {
-    unsigned seen = 0;  // 1: +inf, 2: -inf, 4: NaN
-    __device__ void add(std::uint16_t v)
-    {
-        if ((v & 0x7c00u) == 0x7c00u) seen |= (v & 0x3ffu) ? 4u : (v & 0x8000u) ? 2u : 1u;
-    }
+    unsigned seen = 0;
+    // 1: +inf, 2: -inf, 4: NaN, 0: neither.
+    __device__ static unsigned of(std::uint16_t v) { return (v & 0x7c00u) != 0x7c00u ? 0u : (v & 0x3ffu) ? 4u : (v & 0x8000u) ? 2u : 1u; }
+    __device__ void add(std::uint16_t v) { seen |= of(v); }
     __device__ float sum(float otherwise) const
     {
         return seen == 0 ? otherwise : seen == 1 ? INFINITY : seen == 2 ? -INFINITY : __builtin_nanf("");

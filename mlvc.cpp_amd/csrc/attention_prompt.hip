@@ -85,6 +85,14 @@ __global__ __launch_bounds__(64) void prompt_any_kernel(PromptArgs a)
         }
         __syncthreads();
     }
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+        const int d = c * 64 + lane;
+        if (d >= a.dim || is_finite(acc[c])) continue;
+        OddValues odd;
+        for (int j = 0; j < seen; ++j) odd.add(a.v[static_cast<std::int64_t>(sk.first + j) * a.v_stride + column + d]);
+        acc[c] = odd.sum(acc[c]);
+    }
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
     std::uint16_t* out = a.out + token * a.out_stride + static_cast<std::int64_t>(head) * a.dim;
 #pragma unroll
@@ -460,32 +468,6 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
                 acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, v), p[st], acc[dt], 0, 0, 0);
                 if constexpr (!CLEANED) __builtin_amdgcn_sched_barrier(0);
             }
-        if constexpr (CLEANED) {
-            // What was left out above: a query that sees an infinity or NaN gets
-            // it. Counted by products of 0 / 1 matrices, once for +inf and NaN,
-            // once for -inf and NaN.
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-                for (int sign = 0; sign < 2; ++sign) {
-                    floatx16 count = {};
-                    for (int st = 0; st < 2 * TT; ++st) {
-                        const u32x4 vf = value_fragment(tile_v, st, dt);
-                        half8 is, sees;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const std::uint32_t v = vf[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-                            const bool bad = (v & 0x7fffu) > 0x7c00u || v == (sign ? 0xfc00u : 0x7c00u);
-                            is[e] = static_cast<_Float16>(bad ? 1.0f : 0.0f);
-                            const int j = j0 + st * 16 + 8 * (e >> 2) + 4 * hi + (e & 3);
-                            sees[e] = static_cast<_Float16>(j < seen ? 1.0f : 0.0f);
-                        }
-                        count = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, count, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (count[r] > 0.0f) acc[dt][r] += sign ? -INFINITY : INFINITY;
-                }
-        }
     };
 
     // This group's buffers: K and V of one tile, then of the next.
@@ -522,7 +504,8 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     };
     // All groups take as many turns; `any` is at most `steps` tiles. First the
     // tiles that are seen whole; then those with masked keys, whose values get
-    // the weight 0, while all of them are finite; then, cleaned, the rest.
+    // the weight 0, while all of them are finite; then, cleaned of infinities and
+    // NaN, the rest.
     int round = 0, buffer = 0;
     for (; (round + 1) * C::KG <= clear; ++round, buffer ^= 1) {
         arrived([] {});
@@ -534,6 +517,7 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
         if (__any(flags[buffer * C::WAVES + lane % C::WAVES])) break;
         turn(step, buffer, std::true_type{}, std::false_type{});
     }
+    const int cleaned_from = round * C::KG * kKeys;
     for (; round * C::KG < steps; ++round, buffer ^= 1) {
         arrived([] {});
         turn(round * C::KG + key_group, buffer, std::true_type{}, std::true_type{});
@@ -573,6 +557,49 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
                     for (int e = 0; e < 4; ++e) acc[dt][4 * g + e] = acc[dt][4 * g + e] * mine + v[e] * other;
                 }
         }
+    }
+
+    // A query that sees an infinity or NaN gets it, however small the weight: the
+    // first place of each in a column decides, before the query's end or not. They
+    // are looked for where values were cleaned, and from the first key on where a
+    // sum shows that it met one (8160 tokens, 16 heads of 128, an infinity at the
+    // first key: 1.25 ms instead of 0.27; a sum that is finite costs its test).
+    bool odd = false;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd |= !is_finite(acc[dt][r]);
+    odd = __any(odd) != 0;
+    if (odd || cleaned_from < keys) {
+        constexpr int PER = D / 64;  // columns of a lane
+        int first[3][PER];
+        for (int kind = 0; kind < 3; ++kind)
+            for (int c = 0; c < PER; ++c) first[kind][c] = INT_MAX;
+#pragma unroll 4
+        for (int j = odd ? 0 : cleaned_from; j < keys; ++j) {
+            const std::uint16_t* const row = v0 + j * a.v_stride + lane * PER;
+            std::uint32_t v;
+            if constexpr (PER == 2) v = *reinterpret_cast<const std::uint32_t*>(row);
+            else v = *row;
+#pragma unroll
+            for (int c = 0; c < PER; ++c) {
+                const unsigned kind = OddValues::of(static_cast<std::uint16_t>(v >> 16 * c));
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                    if (kind == 1u << k) first[k][c] = min(first[k][c], j);
+            }
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int holder = (dt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3)) / PER;
+                OddValues seen_here;
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                    if (__shfl(first[k][(r & 3) % PER], holder) < seen) seen_here.seen |= 1u << k;
+                acc[dt][r] = seen_here.sum(acc[dt][r]);
+            }
     }
 
     const float sum = both_sum(l), r = sum == 0.0f ? 0.0f : 1.0f / sum;

@@ -245,3 +245,65 @@ def test_tokens_of_infinite_keys(dev, rng, dim, n):
     with np.errstate(invalid="ignore"):
         within(got, want, tol)
     assert np.isnan(got[0, ::2]).all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("peaked", [False, True])
+@pytest.mark.parametrize("queries,keys,q_heads", [
+    ([3], [3001], 4), ([4], [400], 4), ([130], [1300], 64), ([261], [261], 64), ([200, 77], [933, 1050], 64),
+    ([530], [530], 64), ([1100, 65], [1100, 2065], 64), ([4100], [4100], 32),
+])
+def test_prompt_of_infinite_values(dev, rng, queries, keys, q_heads, dim, causal, peaked):
+    """A seen infinity is the result, opposite ones and NaN are NaN, in their columns, sequence and key head
+    only and from their place on, in every tile shape and whatever the tile."""
+    parts = [_with_odd_values(rng, n, 2, dim, False) for n in keys]
+    for n, part in zip(keys, parts):
+        if peaked:
+            part[0][n // 4] = 60
+    k, v, clean = (np.concatenate([p[i] for p in parts]) for i in range(3))
+    q = normal(rng, sum(queries), q_heads, dim) * np.float16(0.1) + np.float16(4)
+    got = Prompt(dev, q, k, v, queries, keys, causal, dim ** -0.5).run()
+    i = j = 0
+    for nq, nk, part in zip(queries, keys, parts):
+        places = sorted({at for column in part[3].values() for at, _ in column} | {nk // 4})
+        rows = [r + nq - nk for at in places for r in (at - 1, at)] + [0, nq - 1] + rng.integers(0, nq, 4).tolist()
+        for r in sorted({r for r in rows if 0 <= r < nq}):
+            n = nk - nq + r + 1 if causal else nk
+            for head in (0, q_heads - 1):
+                at = slice(j, j + n), slice(head // (q_heads // 2), head // (q_heads // 2) + 1)
+                one = slice(i + r, i + r + 1), slice(head, head + 1)
+                want, tol = attend64(f64(q[one]), f64(k[at]), f64(clean[at]), dim ** -0.5, False)
+                with np.errstate(invalid="ignore"):
+                    if head == 0:
+                        for column, odd in part[3].items():
+                            seen = [x for place, x in odd if place < n]
+                            want[0, 0, column] = _sum_of(seen) if seen else want[0, 0, column]
+                    within(got[one], want, tol, f"query {r} of {nq} on {nk}, head {head}")
+                same = np.isinf(want)
+                assert np.array_equal(np.isnan(want), np.isnan(got[one])) and np.array_equal(got[one][same], want[same])
+        i, j = i + nq, j + nk
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("n,q_heads", [(40, 4), (900, 16), (1100, 64)])
+def test_prompt_of_infinite_keys(dev, rng, n, q_heads, dim, causal):
+    """A key with an infinity scores +inf (NaN) or -inf (not there), by the sign of the query's value."""
+    q, k, v = normal(rng, n, q_heads, dim), normal(rng, n, 2, dim), normal(rng, n, 2, dim)
+    place = n // 3
+    k[place, 0, 3] = np.inf
+    q[:, :, 3] = np.where(np.arange(n) % 2, 1, -1)[:, None]
+    got = Prompt(dev, q, k, v, [n], [n], causal, dim ** -0.5).run()
+    for r in (0, place - 1, place, place + 1, n - 2, n - 1):
+        seen = np.arange(r + 1 if causal else n)
+        rest = seen[seen != place]
+        for head in (0, q_heads - 1):
+            first = head < q_heads // 2
+            kv = slice(0, 1) if first else slice(1, 2)
+            use = rest if first else seen
+            want, tol = attend64(f64(q[r:r + 1, head:head + 1]), f64(k[use, kv]), f64(v[use, kv]), dim ** -0.5, False)
+            if first and place in seen and r % 2:
+                want[:] = np.nan
+            with np.errstate(invalid="ignore"):
+                within(got[r:r + 1, head:head + 1], want, tol, f"query {r}, head {head}")
