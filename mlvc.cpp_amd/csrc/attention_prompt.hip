@@ -619,12 +619,14 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 {
     const int tiles = (a.longest_q + C::ROWS - 1) / C::ROWS;
     // Tiles, at most, from what the host knows; a multiple of the XCDs' number.
-    // Many sequences go by turns where nearly all have as many tiles as the
-    // longest (70 of 200 tokens, 16 heads of 128: 59.7 us, one after the other
-    // 65), else one after the other (99 of 100 and one of 4080: 112 us, by
-    // turns 193; 200 of 30 to 240, heads of 64: 52 and 64).
+    // Many sequences go by turns where they fit a tile each or nearly all have as
+    // many tiles as the longest: a workgroup then finds its tile without reading
+    // past other sequences. us, by turns / one after the other: 1000 of one query,
+    // 16 heads of 64, 71 / 104, on 100 keys 115 / 154; 300 of 20 27 / 30; 200 of one
+    // query on 900 keys, heads of 128, 205 / 205; 70 of 200 59.8 / 63.3; one of 4080
+    // and 99 of 100 193 / 113; 200 of 30 to 240, heads of 64, 60 / 50.
     const std::int64_t by_longest = static_cast<std::int64_t>(tiles) * a.sequences, full = a.q_tokens / C::ROWS;
-    const bool by_turns = a.sequences == 1 || (a.sequences > 64 && by_longest <= full + a.sequences * 3LL / 4);
+    const bool by_turns = a.sequences == 1 || (a.sequences > 64 && (tiles == 1 || by_longest <= full + a.sequences * 3LL / 4));
     const std::int64_t most = by_turns ? by_longest : std::min(by_longest, full + a.sequences);
     const std::int64_t grid = (most * a.q_heads + kXcds - 1) / kXcds * kXcds;
     require(launchable(grid, C::WAVES * 64), "attention_prompt", "too many sequences, heads and queries in one call");

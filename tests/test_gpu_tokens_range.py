@@ -307,3 +307,25 @@ def test_prompt_of_infinite_keys(dev, rng, n, q_heads, dim, causal):
                 want[:] = np.nan
             with np.errstate(invalid="ignore"):
                 within(got[r:r + 1, head:head + 1], want, tol, f"query {r}, head {head}")
+
+
+# ------------------------------------------------------------ many short sequences
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("sequences,heads,most", [(65, 1, 1), (100, 2, 5), (70, 3, 32), (130, 8, 64), (200, 6, 128)])
+def test_prompt_many_sequences_of_one_tile(dev, rng, sequences, heads, most, dim, causal):
+    """More sequences than a wave has lanes that fit a tile each, empty ones among them, on more keys."""
+    queries = [int(n) for n in rng.integers(0, most + 1, sequences)]
+    queries[3], queries[sequences - 1] = most, 1
+    keys = [n + int(more) for n, more in zip(queries, rng.choice([0, 1, 60, 200], sequences))]
+    q = normal(rng, sum(queries), heads, dim)
+    k, v = normal(rng, sum(keys), 1, dim), normal(rng, sum(keys), 1, dim)
+    got = Prompt(dev, q, k, v, queries, keys, causal, dim ** -0.5).run()
+    i = j = 0
+    for nq, nk in zip(queries, keys):
+        a, b = slice(i, i + nq), slice(j, j + nk)
+        want, tol = attend64(f64(q[a, -1:]), f64(k[b]), f64(v[b]), dim ** -0.5, causal)
+        within(got[a, -1:], want, tol, f"{nq} on {nk}") if nq else None
+        i, j = i + nq, j + nk
+    assert np.isfinite(got).all()
