@@ -117,8 +117,9 @@ __device__ __forceinline__ std::uint32_t uniform(std::uint32_t x) { return __bui
 // synchronises before it turns to the next. The compiler does not see that this
 // is a load, so the wait states that the hardware leaves to it stand here too:
 // one after a scalar write of m0, five after a vector write of the buffer's
-// scalar registers (lanes made uniform just before); s_nop N makes N + 1. 8160
-// tokens at 16 heads of 64 take 174 us with all five and 172 with the one.
+// scalar registers (lanes made uniform just before); s_nop N makes N + 1. All
+// five instead of the one cost 1% at 8160 tokens, 16 heads of 64, and nothing
+// at heads of 128.
 __device__ __forceinline__ void lds_dma16(u32x4 buffer, std::uint32_t to, std::uint32_t at)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(buffer) : "memory", "m0");
@@ -186,12 +187,12 @@ struct PromptCfg {
 // there. By the number of keys a tile may see, most first: tile t of sequence n
 // has level base_n + t, in ROWS keys, and the tiles above a level are counted
 // for 64 levels at a time, one a lane (up to 64 sequences, one a lane too).
-// That takes 0.3 us. 8 ragged sequences (1 to 2040 tokens, 16 heads of 128) take
-// 57 us instead of 64.5, and where tiles just fit the CUs, ones that are not
-// there take no CU's turn: one sequence of 2000 and three of 100 tokens 37.7
-// instead of 52, of 300 and 20 tokens 9.4 instead of 13.5. More sequences follow
-// one another, each with its last tile first, 64 at a time. by_turns: sequence
-// after sequence within a tile number.
+// That takes 0.3 us. When it came, 8 ragged sequences (1 to 2040 tokens, 16 heads
+// of 128) took 57 us instead of 64.5 (54 now), and where tiles just fit the CUs,
+// ones that are not there take no CU's turn: one sequence of 2000 and three of 100
+// tokens 37.7 instead of 52, of 300 and 20 tokens 9.4 instead of 13.5. More
+// sequences follow one another, each with its last tile first, 64 at a time.
+// by_turns: sequence after sequence within a tile number.
 template <class C>
 __device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles, bool by_turns, int& n, int& tile, Span& sq, Span& sk)
 {
@@ -428,8 +429,8 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
             if (coarse) {
                 // One rounding of s factor - base would be of another number than the
                 // score that the base was taken from, by up to half a unit of its last
-                // place, and here that is a power of two. (The test costs 1%: 8160
-                // tokens, 16 heads of 64, 172.5 us instead of 170.5.)
+                // place, and here that is a power of two. (The test costs 1% at 8160
+                // tokens.)
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
@@ -641,22 +642,25 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 // groups take longer to start than they save on up to 512 keys.
 // us, the same work by the alternatives (16 query heads, causal):
 //   heads of 128               (4,1)  (4,2)  (2,4)  (1,4)  (8,1)
-//     10 on 1500                             20.6   17.4
-//     240                       11.8   13.0  11.1    8.9   18.3
-//     920                       23.0   21.2  17.9   19.8   30.8
-//     2040                      43.8   36.2  38.6   62.0   59.6
-//     4080                      95.2   87.4   116    184    113
-//     1..2040 packed            56.1   79.7   124    193   65.1
-//     4 x 2040                  85.8    105   159    264   91.9
-//     8160                       302    296   399    661    268
-//   heads of 64                (4,1)  (4,2)  (4,3)  (3,4)  (2,4)  (1,8)
-//     10 on 1500                                           13.2   11.7
-//     240                        9.2    9.0  11.4           8.0    7.6
-//     920                       17.2   14.7  16.1          11.2   15.9
-//     1400                                   20.2   17.9
-//     700 and 600, not causal                14.4   14.0
-//     920 on 4600, 460 on 3001  62.5   47.5  44.2   39.0   54.4
-//     8160                       176    184   188           218
+//     10 on 1500                31.3   24.7   20.0   17.7   39.4
+//     240                       10.9   11.9   10.5    9.1   14.9
+//     920                       22.9   20.8   17.5   20.6   28.8
+//     2040                      44.0   36.9   37.2   57.8   56.5
+//     4080                      93.3   84.1    112    173    109
+//     1..2040 packed            54.0   66.6   96.4    144   62.6
+//     4 x 2040                  83.7    101    145    235   86.7
+//     8160                       289    295    377    589    277
+//   heads of 64                (4,1)  (4,2)  (4,3)  (3,4)  (2,4)  (1,4)  (1,8)
+//     10 on 1500                22.1   18.2   17.4   14.7   12.9   11.5   11.6
+//     240                        8.0    8.2    9.4    8.6    7.4    6.5    7.6
+//     920                       15.9   14.3   14.4   13.0   10.9   14.6   15.7
+//     1400                      22.0   18.8   19.1   17.0   16.0   23.5   25.2
+//     2040                      29.7   24.8   23.8   23.4   22.7   35.8   37.9
+//     700 and 600, not causal   14.2   13.1   13.4   12.8   19.3   23.4   25.9
+//     920 on 4600, 460 on 3001  60.5   47.6   44.1   38.9   49.6   65.2   61.9
+//     4080                      58.6   51.9   52.7   62.5   64.9    105    105
+//     1..2040 packed            36.2   41.4   46.5   54.9   63.1   97.8    106
+//     8160                       172    182    178    193    215    343    326
 // 256 queries a workgroup halve the key traffic again, which pays where a
 // sequence is long enough for its last, partly seen tiles not to count.
 template <int D>

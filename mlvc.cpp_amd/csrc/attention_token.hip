@@ -310,11 +310,11 @@ __device__ __forceinline__ void columns(std::uint32_t a, std::uint32_t b, std::u
 // 2^-37 of the largest: 2^-21 of the values in a context of 65536.
 //
 // Bound by the bytes of the cache: 64 streams of 1 to 8160 tokens, 32 query
-// heads on 8 of 128, INT8, 0.55 GB in 112 us or 4.9 TB/s; one stream of 65280
-// in E4M3, 138 MB in 34.4 us, of them 6 for the launches and the join; 16
-// streams of 920 to 3001 tokens, 16 heads of 64, FP16, 128 MB in 30.6 us. A
+// heads on 8 of 128, INT8, 0.55 GB in 111 us or 5.0 TB/s; one stream of 65280
+// in E4M3, 138 MB in 34.1 us, of them 6 for the launches and the join; 16
+// streams of 920 to 3001 tokens, 16 heads of 64, FP16, 128 MB in 30.5 us. A
 // context of one workgroup is bound by the latency of its few steps: 920 tokens
-// 8.2 us, of them 4 for an empty launch.
+// 8.4 us, of them 4 for an empty launch.
 template <int KIND_, int D_, int WAVES_, int OCC_>
 struct TokenCfg {
     static constexpr int KIND = KIND_, D = D_, WAVES = WAVES_, OCC = OCC_;
@@ -672,18 +672,24 @@ struct Plan {
 // Whether a context goes to one workgroup of eight waves, without a cut. Up to
 // 1024 tokens it is done before a second kernel would start; longer ones are
 // not cut where enough workgroups keep the GPU busy through the longest: half
-// one a CU up to 2048 tokens, three a CU up to 4096. us, whole / cut:
-//   1 x 920, 4 heads of 64, INT8      8.2 / 11.4
-//   200 x 512..1024, 8 of 128, INT8    75 / 91      (1600 workgroups)
-//   16 x 1000..2000, 8 of 128, INT8  20.6 / 20.3    (128)
-//   64 x 1000..2000, 4 of 64, FP16   20.0 / 25.3    (256)
-//   64 x 1..2000, 8 of 128, INT8     41.4 / 39.4    (512)
-//   16 x 1000..2000, 4 of 64, FP16   14.4 / 13.2    (64)
-//   200 x 1..4080, 8 of 128, INT8     172 / 183     (1600)
-//   200 x 1..4080, 4 of 64, E4M3     56.2 / 65.1    (800)
-//   64 x 2040..4080, 4 of 64, FP16   42.4 / 45.6    (256)
-//   64 x 1..4080, 8 of 128, INT8     73.0 / 64.4    (512)
-//   200 x 4080..8160, 4 of 64, FP16   238 / 228     (800)
+// one a CU up to 2048 tokens, three a CU up to 4096. The lengths themselves are
+// on the device: a batch of very different ones, which a cut would even out,
+// and the shortest of the contexts that are cut lose by the rule. us, whole /
+// cut, the one taken marked *:
+//   1 x 920, 4 heads of 64, INT8      8.7*/ 10.2
+//   200 x 512..1024, 8 of 128, INT8  75.7*/ 83.9    (1600 workgroups)
+//   16 x 1..1300, 4 of 64, E4M3       9.7 / 12.5*   (64)
+//   16 x 1000..2000, 4 of 64, FP16   15.4 / 13.5*   (64)
+//   16 x 1000..2000, 8 of 128, INT8  20.6*/ 19.7    (128)
+//   64 x 1000..2000, 4 of 64, FP16   19.5*/ 24.2    (256)
+//   48 x 1..2000, 8 of 128, INT8     32.6*/ 29.6    (384)
+//   64 x 1..2000, 8 of 128, INT8     41.0*/ 37.7    (512)
+//   64 x 1000..2000, 8 of 128, INT8  46.8*/ 49.6    (512)
+//   200 x 1..4080, 8 of 128, INT8     174*/ 177     (1600)
+//   200 x 1..4080, 4 of 64, E4M3     56.7*/ 57.3    (800)
+//   64 x 2040..4080, 4 of 64, FP16   40.8 / 45.5*   (256)
+//   64 x 1..4080, 8 of 128, INT8     71.9 / 62.1*   (512)
+//   200 x 4080..8160, 4 of 64, FP16   239 / 227*    (800)
 bool whole(int longest, std::int64_t workgroups)
 {
     const std::int64_t cus = conv::cu_count();
