@@ -388,7 +388,7 @@ int mlvc_hip_y1_tail(const mlvc_hip_y1_tail_desc* desc, mlvc_hip_stream s);
  * There the softmax's weights go to the matrix cores as FP16, a second
  * rounding: for scores below 2^22 a weight is off by at most 2^-11 of itself or
  * 2^-37 of the largest in attention_prompt, by 2^-22 (8-bit caches: 2^-17) or
- * 2^-37 in attention_token. Other heads and rows take plain FP32 kernels, 20 to
+ * 2^-37 in attention_token. Other heads and rows take plain FP32 kernels, up to
  * 240 times slower in attention (8160 tokens, 16 heads of 96: 30 ms; of 128:
  * 0.3). Norm, rotation and cache have fast kernels for heads of 40 to 256, a
  * multiple of 8, and plain ones 2 to 7 times slower beside them. */
