@@ -524,6 +524,126 @@ typedef struct mlvc_hip_attention_token_desc {
 size_t mlvc_hip_attention_token_workspace_bytes(const mlvc_hip_attention_token_desc* desc);
 int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip_stream s);
 
+/* ---- several tokens a step, in bounded memory ----
+ * The steps of a decoder that drafts tokens and keeps the right ones, without
+ * the host in between: mlvc_hip_kv_plan hands out pages and slots, kv_write
+ * fills them, attention_drafts looks at the cache, mlvc_hip_kv_keep moves the
+ * drafts that are kept behind the context and gives the lengths that the next
+ * plan starts from. With a window, contexts of any age hold the pages of the
+ * window and of the first `sinks` tokens only.
+ *
+ * Window and sinks, in all of them: a token at place p sees a token at place j
+ * if p - j < window (and j - p < window, where it sees later ones at all) or
+ * j < sinks. Window 0: no window. */
+
+/* Page tables, slots and positions of a step, from the streams' lengths on the
+ * device. Stream n has `past[n]` tokens in the cache and gets fresh[n] more, or
+ * has ended (fresh[n] = -1: no tokens, and all of its pages go back). In order:
+ *   1. pages go back to the pool: those behind the context's last token (of
+ *      drafts that were not kept), and with a window those that hold neither a
+ *      sink nor a token that the first of the new ones or a later one sees;
+ *   2. streams take the pages that their new tokens need beyond what they hold,
+ *      stream by stream, from the top of the stack free_pages; the first one
+ *      that the pool does not suffice for and those behind it that need a page
+ *      get none (lacking counts them), nor does a stream whose tokens go beyond
+ *      its table row;
+ *   3. lengths[n] = past[n] + fresh[n] (past[n] for a stream that got no pages),
+ *      starts = 0, then the sums of fresh; token t, the i-th new one of stream
+ *      n, has slots[t], the slot of place past[n] + i, and positions[t] = past[n]
+ *      + i, or with `seen` past[n] + the number of other drafts that it sees: a
+ *      tree's depth. Rows past the last token, and the tokens of streams that got
+ *      no pages, have slot -1 (kv_write skips it); rows past the last token have
+ *      position 0.
+ * Pages that go back and are taken again come in the order that makes a second
+ * call with the same lengths give the same table: a step can be planned anew.
+ * The caller fills `table` with -1, `held` with 0 and free_pages with the pool's
+ * pages before the first call, and leaves them, page_size, window and sinks as
+ * they are between calls. Entries of the table that hold no page are -1. */
+typedef struct mlvc_hip_kv_plan_desc {
+    int streams, pages, page_size; /* as the cache's */
+    int tokens;                    /* rows of slots, positions and seen; later tokens are left out */
+    int window, sinks;
+    int32_t* table;                /* [streams][table_stride] */
+    int table_stride;
+    int32_t* held;                 /* [streams][2]: entries of the table in use, those before a window apart */
+    int32_t* free_pages;           /* [pages] */
+    int32_t* free_count;           /* [1] */
+    const int32_t* past;           /* [streams] */
+    const int32_t* fresh;          /* [streams] */
+    const uint64_t* seen;          /* [tokens] as in attention_drafts, or NULL */
+    int32_t* lengths;              /* [streams]; not `past` or `fresh` */
+    int32_t* starts;               /* [streams + 1] */
+    int32_t* slots;                /* [tokens] */
+    int32_t* positions;            /* [tokens], or NULL */
+    int32_t* lacking;              /* [1] */
+} mlvc_hip_kv_plan_desc;
+int mlvc_hip_kv_plan(const mlvc_hip_kv_plan_desc* desc, mlvc_hip_stream s);
+
+/* Attention of packed sequences as mlvc_hip_attention_prompt, under a window:
+ * places are those of the keys, a query's counted from the sequence's last key
+ * back. With window 0 it is mlvc_hip_attention_prompt. Cost follows the keys
+ * that are seen, not the sequence. */
+typedef struct mlvc_hip_attention_window_desc {
+    mlvc_hip_attention_prompt_desc prompt;
+    int window, sinks;
+} mlvc_hip_attention_window_desc;
+int mlvc_hip_attention_window(const mlvc_hip_attention_window_desc* desc, mlvc_hip_stream s);
+
+/* Attention of each stream's last tokens, 1 to 64 drafts, on its cached context.
+ * Stream n's drafts are rows starts[n] .. starts[n + 1] of q and out; their keys
+ * and values are in the cache already, as the last of its lengths[n] tokens. A
+ * draft sees the context before the drafts, and of the drafts those whose bit is
+ * set in its `seen` (bit j: the stream's j-th draft, its own bit included; NULL:
+ * itself and those before it). With a window, a draft's place is the context's
+ * length plus the number of other drafts that it sees. One draft a stream is the
+ * ordinary step under a window. Drafts past `longest_q` or the 64th are not
+ * computed, and seen by none; their rows of out stay as they are, as do those
+ * past the last stream's. A draft that sees nothing gives zeros. Pages, lengths,
+ * infinities, the workspace and the order of sums are as in
+ * mlvc_hip_attention_token; a weight of the softmax is off by at most 2^-11 of
+ * itself or 2^-37 of the largest. */
+typedef struct mlvc_hip_attention_drafts_desc {
+    const mlvc_hip_kv_cache* cache;
+    int streams, q_heads;          /* q_heads a multiple of the cache's heads */
+    int q_tokens;                  /* rows of q and out: starts beyond are cut to them */
+    int longest_q;                 /* at least the most drafts of a stream, 1..64 */
+    const void* q;                 /* [q_tokens][q_heads][head_dim] FP16 */
+    void* out;
+    int64_t q_stride, out_stride;  /* halves from token to token */
+    const int32_t* starts;         /* [streams + 1], ascending, device memory */
+    const uint64_t* seen;          /* [q_tokens], device memory, or NULL */
+    const int32_t* table;          /* [streams][table_stride], device memory */
+    int table_stride;
+    const int32_t* lengths;        /* [streams], with the drafts, device memory */
+    int longest;                   /* at least the longest context; later tokens are not seen */
+    int window, sinks;
+    float scale;
+    void* workspace;               /* 16-byte aligned; mlvc_hip_attention_drafts_workspace_bytes */
+    size_t workspace_bytes;
+} mlvc_hip_attention_drafts_desc;
+/* Depends on streams, q_heads, longest_q, longest, window, sinks and the cache's
+ * layout only (0: none needed), and grows with streams, longest_q and longest. */
+size_t mlvc_hip_attention_drafts_workspace_bytes(const mlvc_hip_attention_drafts_desc* desc);
+int mlvc_hip_attention_drafts(const mlvc_hip_attention_drafts_desc* desc, mlvc_hip_stream s);
+
+/* Keeps a path of each stream's drafts: draft kept[n][i] moves to the i-th place
+ * behind the context, its stored values and scales as they are, and
+ * lengths_out[n] becomes the context's length with the kept drafts. A number
+ * that is no draft of the stream (-1) ends its list. The same draft may stand
+ * twice. Rows whose page is not in the cache are not moved. */
+typedef struct mlvc_hip_kv_keep_desc {
+    const mlvc_hip_kv_cache* cache;
+    int streams;
+    const int32_t* table;       /* [streams][table_stride], device memory */
+    int table_stride;
+    const int32_t* starts;      /* [streams + 1]: stream n has starts[n + 1] - starts[n] drafts */
+    const int32_t* lengths;     /* [streams], with the drafts */
+    const int32_t* kept;        /* [streams][kept_stride] */
+    int kept_stride;            /* 0..64 */
+    int32_t* lengths_out;       /* [streams]; not `lengths` */
+} mlvc_hip_kv_keep_desc;
+int mlvc_hip_kv_keep(const mlvc_hip_kv_keep_desc* desc, mlvc_hip_stream s);
+
 #ifdef __cplusplus
 }
 #endif

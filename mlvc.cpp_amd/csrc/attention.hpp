@@ -17,8 +17,10 @@ inline void require(bool ok, const char* op, const char* what)
     if (!ok) throw std::runtime_error(std::string(op) + ": " + what);
 }
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0; }
-inline bool aligned2(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 1u) == 0; }
+template <int BYTES>
+bool aligned_to(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & (BYTES - 1u)) == 0; }
+inline bool aligned16(const void* p) { return aligned_to<16>(p); }
+inline bool aligned2(const void* p) { return aligned_to<2>(p); }
 
 // 16-byte aligned rows of halves.
 inline bool vector_rows(const void* p, std::int64_t stride) { return aligned16(p) && stride % 8 == 0; }

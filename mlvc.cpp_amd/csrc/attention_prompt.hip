@@ -25,6 +25,7 @@ struct PromptArgs {
     const std::int32_t* k_starts;
     int sequences, q_heads, group, dim, q_tokens, k_tokens, longest_q, causal, negate, cus;
     float scale2;  // |scale| log2(e); negate: scale is negative
+    int window, sinks;  // window 0: none
 };
 
 // Rows [first, first + count) of a sequence, cut to the tensor.
@@ -53,44 +54,57 @@ __global__ __launch_bounds__(64) void prompt_any_kernel(PromptArgs a)
     const Span sq = span(a.q_starts, lo, a.q_tokens), sk = span(a.k_starts, lo, a.k_tokens);
     const int i = token - sq.first;
     if (i < 0 || i >= sq.count || i >= a.longest_q) return;
-    const int seen = a.causal ? min(sk.count, max(0, sk.count - sq.count + i + 1)) : sk.count;
+    const std::int64_t place = static_cast<std::int64_t>(sk.count) - sq.count + i;
+    const int end = a.causal ? static_cast<int>(min(static_cast<std::int64_t>(sk.count), max(std::int64_t{0}, place + 1))) : sk.count;
+    // Keys seen: two ranges, the sinks before the window (those behind it if
+    // they reach further) and the window.
+    int from[2] = {0, 0}, to[2] = {0, end};
+    if (a.window) {
+        const int sinks = min(a.sinks, end);
+        from[1] = static_cast<int>(min(static_cast<std::int64_t>(end), max(std::int64_t{0}, place - a.window + 1)));
+        to[1] = static_cast<int>(min(static_cast<std::int64_t>(end), max(std::int64_t{0}, place + a.window)));
+        to[0] = min(sinks, from[1]);
+        if (sinks > from[1]) to[1] = max(to[1], sinks);
+    }
     const std::uint16_t* q = a.q + token * a.q_stride + static_cast<std::int64_t>(head) * a.dim;
     for (int d = lane; d < a.dim; d += 64) qs[d] = h2f(q[d]) * (a.negate ? -a.scale2 : a.scale2);
     __syncthreads();
     const std::int64_t column = static_cast<std::int64_t>(head / a.group) * a.dim;
     constexpr int kColumns = kMaxHeadDim / 64;
     float acc[kColumns] = {}, m = -INFINITY, l = 0.0f;
-    for (int j0 = 0; j0 < seen; j0 += 64) {
-        float s = -INFINITY;
-        if (j0 + lane < seen) {
-            const std::uint16_t* k = a.k + static_cast<std::int64_t>(sk.first + j0 + lane) * a.k_stride + column;
-            s = 0.0f;
-            for (int d = 0; d < a.dim; ++d) s = fmaf(qs[d], h2f(k[d]), s);
-        }
-        const float top = fmaxf(m, group_max<64>(s)), base = top == -INFINITY ? 0.0f : top;
-        const float p = __builtin_amdgcn_exp2f(s - base), keep = __builtin_amdgcn_exp2f(m - base);
-        m = top;
-        l = l * keep + group_sum<64>(p);
-        ps[lane] = p;
-        __syncthreads();
-        const int n = min(64, seen - j0);
-        const std::uint16_t* v = a.v + static_cast<std::int64_t>(sk.first + j0) * a.v_stride + column;
+    for (int range = 0; range < 2; ++range)
+        for (int j0 = from[range], seen = to[range]; j0 < seen; j0 += 64) {
+            float s = -INFINITY;
+            if (j0 + lane < seen) {
+                const std::uint16_t* k = a.k + static_cast<std::int64_t>(sk.first + j0 + lane) * a.k_stride + column;
+                s = 0.0f;
+                for (int d = 0; d < a.dim; ++d) s = fmaf(qs[d], h2f(k[d]), s);
+            }
+            const float top = fmaxf(m, group_max<64>(s)), base = top == -INFINITY ? 0.0f : top;
+            const float p = __builtin_amdgcn_exp2f(s - base), keep = __builtin_amdgcn_exp2f(m - base);
+            m = top;
+            l = l * keep + group_sum<64>(p);
+            ps[lane] = p;
+            __syncthreads();
+            const int n = min(64, seen - j0);
+            const std::uint16_t* v = a.v + static_cast<std::int64_t>(sk.first + j0) * a.v_stride + column;
 #pragma unroll
-        for (int c = 0; c < kColumns; ++c) {
-            const int d = c * 64 + lane;
-            if (d >= a.dim) break;
-            float sum = acc[c] * keep;
-            for (int j = 0; j < n; ++j) sum = fmaf(ps[j], h2f(v[j * a.v_stride + d]), sum);
-            acc[c] = sum;
+            for (int c = 0; c < kColumns; ++c) {
+                const int d = c * 64 + lane;
+                if (d >= a.dim) break;
+                float sum = acc[c] * keep;
+                for (int j = 0; j < n; ++j) sum = fmaf(ps[j], h2f(v[j * a.v_stride + d]), sum);
+                acc[c] = sum;
+            }
+            __syncthreads();
         }
-        __syncthreads();
-    }
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) {
         const int d = c * 64 + lane;
         if (d >= a.dim || is_finite(acc[c])) continue;
         OddValues odd;
-        for (int j = 0; j < seen; ++j) odd.add(a.v[static_cast<std::int64_t>(sk.first + j) * a.v_stride + column + d]);
+        for (int range = 0; range < 2; ++range)
+            for (int j = from[range]; j < to[range]; ++j) odd.add(a.v[static_cast<std::int64_t>(sk.first + j) * a.v_stride + column + d]);
         acc[c] = odd.sum(acc[c]);
     }
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
@@ -630,7 +644,7 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
     const bool by_turns = a.sequences == 1 || (a.sequences > 64 && (tiles == 1 || by_longest <= full + a.sequences * 3LL / 4));
     const std::int64_t most = by_turns ? by_longest : std::min(by_longest, full + a.sequences);
     const std::int64_t grid = (most * a.q_heads + kXcds - 1) / kXcds * kXcds;
-    require(launchable(grid, C::WAVES * 64), "attention_prompt", "too many sequences, heads and queries in one call");
+    require(launchable(grid, C::WAVES * 64), a.window ? "attention_window" : "attention_prompt", "too many sequences, heads and queries in one call");
     prompt_kernel<C><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles, by_turns);
 }
 
@@ -685,10 +699,10 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
     else launch_prompt<PromptCfg<D, 4, 1, 64, D == 64 ? 3 : 2>>(a, s);
 }
 
-void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
+void attention_prompt(const mlvc_hip_attention_prompt_desc* d, int window, int sinks, const char* op, hipStream_t s)
 {
-    const char* op = "attention_prompt";
     require(d != nullptr, op, "no descriptor");
+    require(window >= 0 && sinks >= 0, op, "window and sinks must not be negative");
     require(d->sequences >= 0 && d->q_tokens >= 0 && d->k_tokens >= 0 && d->longest_q >= 0, op, "negative size");
     require(d->head_dim >= 1 && d->head_dim <= kMaxHeadDim, op, "head_dim must be 1..512");
     require(d->kv_heads >= 1 && d->q_heads >= 1 && d->q_heads <= 65535 && d->q_heads % d->kv_heads == 0, op,
@@ -714,18 +728,20 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
     a.q_tokens = d->q_tokens, a.k_tokens = d->k_tokens, a.longest_q = std::min(d->longest_q, d->q_tokens), a.causal = d->causal != 0;
     a.cus = conv::cu_count();
     a.scale2 = std::fabs(d->scale) * 1.4426950408889634f, a.negate = d->scale < 0.0f;
+    // A window that reaches from end to end is none.
+    a.window = window < static_cast<std::int64_t>(d->q_tokens) + d->k_tokens ? window : 0, a.sinks = sinks;
     // The matrix-core kernel addresses a tile's rows by 32-bit byte offsets,
     // and scales masked scores (-inf) by the factor, which must not be 0.
     constexpr std::int64_t kFarthest = std::int64_t{1} << 23;
     const bool rows = vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride) && vector_rows(d->k, d->k_stride) &&
                       vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f;
-    if (rows && d->head_dim == 128) launch_prompt<128>(a, s);
-    else if (rows && d->head_dim == 64) launch_prompt<64>(a, s);
+    if (rows && !a.window && d->head_dim == 128) launch_prompt<128>(a, s);
+    else if (rows && !a.window && d->head_dim == 64) launch_prompt<64>(a, s);
     else {
         require(launchable(d->q_tokens, 64), op, "too many sequences, heads and queries in one call");
         prompt_any_kernel<<<dim3(static_cast<unsigned>(d->q_tokens), static_cast<unsigned>(d->q_heads)), 64, 0, s>>>(a);
     }
-    check(hipGetLastError(), "attention_prompt launch");
+    check(hipGetLastError(), window ? "attention_window launch" : "attention_prompt launch");
 }
 
 }  // namespace
@@ -733,7 +749,16 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, hipStream_t s)
 
 using namespace mlvc_hip;
 
-extern "C" int mlvc_hip_attention_prompt(const mlvc_hip_attention_prompt_desc* desc, mlvc_hip_stream s)
+extern "C" {
+
+int mlvc_hip_attention_prompt(const mlvc_hip_attention_prompt_desc* desc, mlvc_hip_stream s)
 {
-    return guard([&] { attention_prompt(desc, to_stream(s)); });
+    return guard([&] { attention_prompt(desc, 0, 0, "attention_prompt", to_stream(s)); });
 }
+
+int mlvc_hip_attention_window(const mlvc_hip_attention_window_desc* desc, mlvc_hip_stream s)
+{
+    return guard([&] { attention_prompt(desc ? &desc->prompt : nullptr, desc ? desc->window : 0, desc ? desc->sinks : 0, "attention_window", to_stream(s)); });
+}
+
+}  // extern "C"

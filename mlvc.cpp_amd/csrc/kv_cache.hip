@@ -252,6 +252,104 @@ void run(const mlvc_hip_kv_cache* c, const mlvc_hip_kv_rows* r, hipStream_t s)
     check(hipGetLastError(), WRITE ? "kv_write launch" : "kv_read launch");
 }
 
+struct KeepArgs {
+    std::uint8_t* cache[2];  // k, v
+    float* scale[2];
+    const std::int32_t* table;
+    const std::int32_t* starts;
+    const std::int32_t* lengths;
+    const std::int32_t* kept;
+    std::int32_t* lengths_out;
+    int streams, heads, row_bytes, page, pages, table_stride, kept_stride, quantised;
+};
+
+constexpr int kMostKept = 64;
+
+// A workgroup for the kept rows of one head of a stream. The places they go to
+// may be those of others that move too, so a group of columns is read for all
+// rows before any of it is written; columns do not meet.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void kv_keep_kernel(KeepArgs a)
+{
+    __shared__ std::int64_t from[kMostKept], to[kMostKept];
+    __shared__ int kept_count;
+    const int head = blockIdx.x % a.heads, stream = blockIdx.x / a.heads, tid = threadIdx.x;
+    if (tid < 64) {
+        const int drafts = max(a.starts[stream + 1] - a.starts[stream], 0), past = max(a.lengths[stream], 0) - drafts;
+        const int draft = tid < a.kept_stride ? a.kept[static_cast<std::int64_t>(stream) * a.kept_stride + tid] : -1;
+        const unsigned long long ends = ~__ballot(draft >= 0 && draft < drafts);
+        const int count = ends ? __builtin_ctzll(ends) : 64;
+        auto row = [&](int i) -> std::int64_t {
+            const std::int64_t place = static_cast<std::int64_t>(past) + i;
+            if (place < 0 || place >= static_cast<std::int64_t>(a.table_stride) * a.page) return -1;
+            const int entry = static_cast<int>(static_cast<unsigned>(place) / static_cast<unsigned>(a.page));
+            const int page = a.table[static_cast<std::int64_t>(stream) * a.table_stride + entry];
+            return page < 0 || page >= a.pages ? -1 : (static_cast<std::int64_t>(page) * a.heads + head) * a.page + (place - static_cast<std::int64_t>(entry) * a.page);
+        };
+        const bool moves = tid < count && draft != tid;
+        const std::int64_t f = moves ? row(draft) : -1, t = moves ? row(tid) : -1;
+        from[tid] = t < 0 ? -1 : f;
+        to[tid] = t;
+        if (tid == 0) {
+            kept_count = count;
+            if (head == 0) a.lengths_out[stream] = max(past + count, 0);
+        }
+    }
+    __syncthreads();
+    const int count = kept_count;
+    if (count == 0) return;
+    const int pieces = a.row_bytes / static_cast<int>(sizeof(T)), columns = kBlock / count;  // of a turn
+    const int row = tid / columns, column = tid - row * columns;
+    const bool mine = row < count && from[min(row, kMostKept - 1)] >= 0;
+    for (int c = 0; c < pieces; c += columns) {
+        const bool here = mine && c + column < pieces;
+        T k{}, v{};
+        if (here) {
+            const std::int64_t at = from[row] * a.row_bytes + static_cast<std::int64_t>(c + column) * sizeof(T);
+            k = *reinterpret_cast<const T*>(a.cache[0] + at), v = *reinterpret_cast<const T*>(a.cache[1] + at);
+        }
+        __syncthreads();
+        if (here) {
+            const std::int64_t at = to[row] * a.row_bytes + static_cast<std::int64_t>(c + column) * sizeof(T);
+            *reinterpret_cast<T*>(a.cache[0] + at) = k, *reinterpret_cast<T*>(a.cache[1] + at) = v;
+        }
+    }
+    if (a.quantised && tid < kMostKept) {  // one wave: reads before writes
+        const bool here = tid < count && from[tid] >= 0;
+        const float k = here ? a.scale[0][from[tid]] : 0.0f, v = here ? a.scale[1][from[tid]] : 0.0f;
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (here) a.scale[0][to[tid]] = k, a.scale[1][to[tid]] = v;
+    }
+}
+
+void kv_keep(const mlvc_hip_kv_keep_desc* d, hipStream_t s)
+{
+    const char* op = "kv_keep";
+    require(d != nullptr, op, "no descriptor");
+    check_cache(d->cache, op);
+    require(d->streams >= 0 && d->table_stride >= 0, op, "negative size");
+    require(d->kept_stride >= 0 && d->kept_stride <= kMostKept, op, "kept_stride must be 0..64");
+    if (d->streams == 0) return;
+    require(d->starts && d->lengths && d->lengths_out && (d->kept || d->kept_stride == 0) && (d->table || d->table_stride == 0), op, "null tensor");
+    require(d->lengths_out != d->lengths && d->lengths_out != d->starts, op, "lengths_out must not be lengths or starts");
+    for (const std::int32_t* p : {d->table, d->starts, d->lengths, d->kept, static_cast<const std::int32_t*>(d->lengths_out)})
+        require(aligned_to<4>(p), op, "a tensor is not aligned to its values");
+    const mlvc_hip_kv_cache* c = d->cache;
+    const std::int64_t grid = static_cast<std::int64_t>(d->streams) * c->heads;
+    require(launchable(grid, kBlock), op, "too many streams and heads in one call");
+    KeepArgs a{};
+    a.cache[0] = static_cast<std::uint8_t*>(c->k), a.cache[1] = static_cast<std::uint8_t*>(c->v);
+    a.scale[0] = c->k_scale, a.scale[1] = c->v_scale;
+    a.table = d->table, a.starts = d->starts, a.lengths = d->lengths, a.kept = d->kept, a.lengths_out = d->lengths_out;
+    a.streams = d->streams, a.heads = c->heads, a.page = c->page_size, a.pages = c->pages, a.table_stride = d->table_stride;
+    a.kept_stride = d->kept_stride, a.quantised = c->kind != MLVC_KV_F16;
+    a.row_bytes = c->head_dim * (a.quantised ? 1 : 2);
+    if (a.row_bytes % 16 == 0) kv_keep_kernel<u32x4><<<static_cast<unsigned>(grid), kBlock, 0, s>>>(a);
+    else kv_keep_kernel<uint2><<<static_cast<unsigned>(grid), kBlock, 0, s>>>(a);
+    check(hipGetLastError(), "kv_keep launch");
+}
+
 size_t values_of_cache(const mlvc_hip_kv_cache* c)
 {
     return static_cast<size_t>(c->pages) * c->heads * c->page_size;
@@ -284,6 +382,11 @@ int mlvc_hip_kv_write(const mlvc_hip_kv_cache* cache, const mlvc_hip_kv_rows* ro
 int mlvc_hip_kv_read(const mlvc_hip_kv_cache* cache, const mlvc_hip_kv_rows* rows, mlvc_hip_stream s)
 {
     return guard([&] { run<false>(cache, rows, to_stream(s)); });
+}
+
+int mlvc_hip_kv_keep(const mlvc_hip_kv_keep_desc* desc, mlvc_hip_stream s)
+{
+    return guard([&] { kv_keep(desc, to_stream(s)); });
 }
 
 }  // extern "C"

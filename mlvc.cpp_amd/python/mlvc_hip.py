@@ -461,6 +461,35 @@ class TokenAttention(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class KvPlan(C.Structure):
+    """mlvc_hip_kv_plan_desc"""
+    _fields_ = [(f, C.c_int) for f in ("streams", "pages", "page_size", "tokens", "window", "sinks")] + [
+        ("table", C.c_void_p), ("table_stride", C.c_int)] + [
+        (f, C.c_void_p) for f in ("held", "free_pages", "free_count", "past", "fresh", "seen", "lengths", "starts", "slots",
+                                  "positions", "lacking")]
+
+
+class WindowAttention(C.Structure):
+    """mlvc_hip_attention_window_desc"""
+    _fields_ = [("prompt", PromptAttention), ("window", C.c_int), ("sinks", C.c_int)]
+
+
+class DraftAttention(C.Structure):
+    """mlvc_hip_attention_drafts_desc; keep the KvCache that `cache` points to."""
+    _fields_ = [("cache", C.POINTER(KvCache))] + [(f, C.c_int) for f in ("streams", "q_heads", "q_tokens", "longest_q")] + [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("starts", C.c_void_p),
+        ("seen", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int), ("lengths", C.c_void_p)] + [
+        (f, C.c_int) for f in ("longest", "window", "sinks")] + [
+        ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class KvKeep(C.Structure):
+    """mlvc_hip_kv_keep_desc; keep the KvCache that `cache` points to."""
+    _fields_ = [("cache", C.POINTER(KvCache)), ("streams", C.c_int), ("table", C.c_void_p), ("table_stride", C.c_int),
+                ("starts", C.c_void_p), ("lengths", C.c_void_p), ("kept", C.c_void_p), ("kept_stride", C.c_int),
+                ("lengths_out", C.c_void_p)]
+
+
 def _bind_attention(lib) -> None:
     lib.mlvc_hip_qk_norm_rope.argtypes = [C.POINTER(QkNormRope), C.c_void_p]
     lib.mlvc_hip_rope_frequencies.argtypes = [C.c_int, C.c_double, C.c_int, C.c_double, C.c_double, C.c_void_p,
@@ -473,6 +502,12 @@ def _bind_attention(lib) -> None:
     lib.mlvc_hip_attention_token_workspace_bytes.argtypes = [C.POINTER(TokenAttention)]
     lib.mlvc_hip_attention_token_workspace_bytes.restype = C.c_size_t
     lib.mlvc_hip_attention_token.argtypes = [C.POINTER(TokenAttention), C.c_void_p]
+    lib.mlvc_hip_kv_plan.argtypes = [C.POINTER(KvPlan), C.c_void_p]
+    lib.mlvc_hip_attention_window.argtypes = [C.POINTER(WindowAttention), C.c_void_p]
+    lib.mlvc_hip_attention_drafts_workspace_bytes.argtypes = [C.POINTER(DraftAttention)]
+    lib.mlvc_hip_attention_drafts_workspace_bytes.restype = C.c_size_t
+    lib.mlvc_hip_attention_drafts.argtypes = [C.POINTER(DraftAttention), C.c_void_p]
+    lib.mlvc_hip_kv_keep.argtypes = [C.POINTER(KvKeep), C.c_void_p]
 
 
 def _device_check(rc: int) -> None:
@@ -517,3 +552,23 @@ def attention_token_workspace_bytes(desc: TokenAttention) -> int:
 
 def attention_token(desc: TokenAttention, stream=None) -> None:
     _device_check(device_lib().mlvc_hip_attention_token(desc, stream))
+
+
+def kv_plan(desc: KvPlan, stream=None) -> None:
+    _device_check(device_lib().mlvc_hip_kv_plan(desc, stream))
+
+
+def attention_window(desc: WindowAttention, stream=None) -> None:
+    _device_check(device_lib().mlvc_hip_attention_window(desc, stream))
+
+
+def attention_drafts_workspace_bytes(desc: DraftAttention) -> int:
+    return device_lib().mlvc_hip_attention_drafts_workspace_bytes(desc)
+
+
+def attention_drafts(desc: DraftAttention, stream=None) -> None:
+    _device_check(device_lib().mlvc_hip_attention_drafts(desc, stream))
+
+
+def kv_keep(desc: KvKeep, stream=None) -> None:
+    _device_check(device_lib().mlvc_hip_kv_keep(desc, stream))
