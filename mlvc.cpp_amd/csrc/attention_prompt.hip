@@ -271,7 +271,36 @@ __device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles,
     return true;
 }
 
-template <class C>
+// Under a window: the key tiles that a workgroup's queries see, [0, sinks) and
+// [from, to), and of the latter those that all of them see whole, [clear_from,
+// clear_to). They are taken in the order clear, sinks, before, behind.
+struct WindowTiles {
+    int sinks, from, to, clear_from, clear_to;
+    __device__ int clear() const { return clear_to - clear_from; }
+    __device__ int steps() const { return sinks + to - from; }
+    __device__ int at(int step) const
+    {
+        if (step < clear()) return clear_from + step;
+        step -= clear();
+        if (step < sinks) return step;
+        step += from - sinks;
+        return step < clear_from ? step : step + clear();
+    }
+};
+
+// Keys that the queries first .. last see of a window, and of the sinks; places
+// are those of their sequence's keys.
+struct Sight {
+    int from, to, sinks;
+    __device__ Sight(const PromptArgs& a, int first, int last, int count)
+    {
+        from = min(max(first - a.window + 1, 0), count);
+        to = max(min(last + (a.causal ? 1 : a.window), count), from);
+        sinks = max(min(a.sinks, a.causal ? min(last + 1, count) : count), 0);
+    }
+};
+
+template <class C, bool WINDOW>
 __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArgs a, int tiles, bool by_turns)
 {
     constexpr int D = C::D, KS = D / 16, DT = D / 32, kKeys = C::KEYS, TT = kKeys / 32;
@@ -313,7 +342,18 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     const int behind = sk.count - sq.count;  // keys before the first query
     const int last = min(q0 + C::ROWS, nq) - 1;
     const int keys = a.causal ? max(0, min(sk.count, behind + last + 1)) : sk.count;  // seen by any query here
-    const int steps = (keys + kKeys - 1) / kKeys;
+    WindowTiles wt{};
+    if constexpr (WINDOW) {
+        const Sight all(a, behind + q0, behind + last, sk.count);
+        const int sink_tiles = (all.sinks + kKeys - 1) / kKeys;
+        wt.from = all.from / kKeys;
+        wt.to = max(max(wt.from, sink_tiles), all.to > all.from ? (all.to + kKeys - 1) / kKeys : 0);
+        wt.sinks = min(sink_tiles, wt.from);
+        const int low = max(behind + last - a.window + 1, 0), high = min(behind + q0 + (a.causal ? 1 : a.window), sk.count);
+        wt.clear_from = min((low + kKeys - 1) / kKeys, wt.to);
+        wt.clear_to = max(high < 0 ? 0 : high / kKeys, wt.clear_from);
+    }
+    const int steps = WINDOW ? wt.steps() : (keys + kKeys - 1) / kKeys;
 
     // This wave's queries, as B fragments.
     const int w0 = q0 + row_group * 32, i_query = w0 + column, at_query = min(i_query, nq - 1);
@@ -332,12 +372,16 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     // Tiles that every query of the workgroup sees whole, and keys that any of this wave's sees.
     const int clear = (a.causal ? max(0, min(sk.count, behind + q0 + 1)) : sk.count) / kKeys;
     const int any = w0 >= nq ? 0 : a.causal ? max(0, min(sk.count, behind + min(w0 + 32, nq))) : sk.count;
+    // Under a window: keys that any of this wave's queries sees, and those of this lane's.
+    const Sight of_wave(a, behind + w0, behind + min(w0 + 32, nq) - 1, sk.count), of_lane(a, behind + at_query, behind + at_query, sk.count);
+    auto lane_sees = [&](int j) { return static_cast<unsigned>(j - of_lane.from) < static_cast<unsigned>(of_lane.to - of_lane.from) || j < of_lane.sinks; };
 
     const std::int64_t kv = static_cast<std::int64_t>(head / a.group) * D;
     const std::uint16_t* const k0 = a.k + sk.first * a.k_stride + kv;
     const std::uint16_t* const v0 = a.v + sk.first * a.v_stride + kv;
     // A tile's DMA instructions are dealt to the waves of its group.
     const int first_row = row_group * C::DMA_ROWS + lane / C::PIECES;
+    auto tile_of = [&](int step) { return WINDOW ? wt.at(step) : step; };
     auto stage = [&](const std::uint16_t* x, std::int64_t stride, int step, std::uint32_t to) {
         const std::uint32_t stride2 = static_cast<std::uint32_t>(stride) * 2u;
         const std::uint64_t p = reinterpret_cast<std::uint64_t>(x + static_cast<std::int64_t>(step) * kKeys * stride);
@@ -413,8 +457,10 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (j0 + tt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen) s[tt][r] = -INFINITY;
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = j0 + tt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3);
+                        if (WINDOW ? !lane_sees(j) : j >= seen) s[tt][r] = -INFINITY;
+                    }
             }
             // The NaN-propagating maximum of three is one instruction; a score that
             // is NaN leaves the maximum where it was, and its query becomes NaN.
@@ -489,8 +535,9 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     std::uint16_t* const tiles_of_group = lds + key_group * 4 * C::TILE;
     const std::uint32_t to = uniform(lds_address(tiles_of_group));
     auto stage_both = [&](int step, int buffer) {
-        stage(k0, a.k_stride, step, to + buffer * C::TILE * 4);
-        stage(v0, a.v_stride, step, to + buffer * C::TILE * 4 + C::TILE * 2);
+        const int tile = tile_of(step);
+        stage(k0, a.k_stride, tile, to + buffer * C::TILE * 4);
+        stage(v0, a.v_stride, tile, to + buffer * C::TILE * 4 + C::TILE * 2);
     };
     if (key_group < steps) stage_both(key_group, 0);
     // Whether the pieces of V that this wave staged hold an infinity or NaN.
@@ -515,14 +562,18 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     auto turn = [&](int step, int buffer, auto masked, auto cleaned) {
         if (step + C::KG < steps) stage_both(step + C::KG, buffer ^ 1);
         const std::uint16_t* const tile = tiles_of_group + buffer * 2 * C::TILE;
-        if (!masked || step * kKeys < any) compute(step, tile, tile + C::TILE, masked, cleaned);
+        if constexpr (WINDOW) {
+            if (masked && step >= steps) return;
+            const int t = tile_of(step), j = t * kKeys;
+            if (!masked || (w0 < nq && ((j < of_wave.to && j + kKeys > of_wave.from) || j < of_wave.sinks))) compute(t, tile, tile + C::TILE, masked, cleaned);
+        } else if (!masked || step * kKeys < any) compute(step, tile, tile + C::TILE, masked, cleaned);
     };
     // All groups take as many turns; `any` is at most `steps` tiles. First the
     // tiles that are seen whole; then those with masked keys, whose values get
     // the weight 0, while all of them are finite; then, cleaned of infinities and
     // NaN, the rest.
     int round = 0, buffer = 0;
-    for (; (round + 1) * C::KG <= clear; ++round, buffer ^= 1) {
+    for (; (round + 1) * C::KG <= (WINDOW ? wt.clear() : clear); ++round, buffer ^= 1) {
         arrived([] {});
         turn(round * C::KG + key_group, buffer, std::false_type{}, std::false_type{});
     }
@@ -585,7 +636,53 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
 #pragma unroll
         for (int r = 0; r < 16; ++r) odd |= !is_finite(acc[dt][r]);
     odd = __any(odd) != 0;
-    if (odd || cleaned_from < keys) {
+    if constexpr (WINDOW) {
+        // The wave's window moves by a key from query to query: where its first keys,
+        // which only some of the queries see, hold an infinity or NaN is kept bit by
+        // bit, of the keys behind them and of the sinks the first place.
+        if (odd || cleaned_from < steps * kKeys) {
+            constexpr int PER = D / 64;
+            int first[2][3][PER];
+            unsigned edge[3][PER];
+            for (int kind = 0; kind < 3; ++kind)
+                for (int c = 0; c < PER; ++c) first[0][kind][c] = first[1][kind][c] = INT_MAX, edge[kind][c] = 0;
+            const int low = behind + w0 - a.window + 1;  // of the wave's first query, before the first key or not
+            for (int part = 0; part < 2; ++part)
+#pragma unroll 4
+                for (int j = part ? of_wave.from : 0; j < (part ? of_wave.to : of_wave.sinks); ++j) {
+                    const std::uint16_t* const row = v0 + j * a.v_stride + lane * PER;
+                    std::uint32_t v;
+                    if constexpr (PER == 2) v = *reinterpret_cast<const std::uint32_t*>(row);
+                    else v = *row;
+#pragma unroll
+                    for (int c = 0; c < PER; ++c) {
+                        const unsigned kind = OddValues::of(static_cast<std::uint16_t>(v >> 16 * c));
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) {
+                            if (kind != 1u << k) continue;
+                            if (part && j - low < 31) edge[k][c] |= 1u << (j - low);
+                            else first[part][k][c] = min(first[part][k][c], j);
+                        }
+                    }
+                }
+            const int mine = max(at_query - w0, 0), width = behind + at_query + (a.causal ? 1 : a.window) - (low + mine);
+            const unsigned wide = width >= 32 ? ~0u : (1u << width) - 1;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int holder = (dt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3)) / PER;
+                    OddValues seen_here;
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+                        const bool sink = __shfl(first[0][k][(r & 3) % PER], holder) < of_lane.sinks, in = __shfl(first[1][k][(r & 3) % PER], holder) < of_lane.to;
+                        const unsigned at_edge = __shfl(edge[k][(r & 3) % PER], holder) >> mine & wide;
+                        if (sink || in || at_edge) seen_here.seen |= 1u << k;
+                    }
+                    acc[dt][r] = seen_here.sum(acc[dt][r]);
+                }
+        }
+    } else if (odd || cleaned_from < keys) {
         constexpr int PER = D / 64;  // columns of a lane
         int first[3][PER];
         for (int kind = 0; kind < 3; ++kind)
@@ -629,7 +726,7 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
                            pack_rounded(acc[dt][4 * g + 2] * r, acc[dt][4 * g + 3] * r));
 }
 
-template <class C>
+template <class C, bool WINDOW>
 void launch_prompt(const PromptArgs& a, hipStream_t s)
 {
     const int tiles = (a.longest_q + C::ROWS - 1) / C::ROWS;
@@ -645,7 +742,7 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
     const std::int64_t most = by_turns ? by_longest : std::min(by_longest, full + a.sequences);
     const std::int64_t grid = (most * a.q_heads + kXcds - 1) / kXcds * kXcds;
     require(launchable(grid, C::WAVES * 64), a.window ? "attention_window" : "attention_prompt", "too many sequences, heads and queries in one call");
-    prompt_kernel<C><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles, by_turns);
+    prompt_kernel<C, WINDOW><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles, by_turns);
 }
 
 // Workgroups of 128 queries, two a CU, read each key tile once for 128 queries
@@ -677,7 +774,7 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 //     8160                       172    182    178    193    215    343    326
 // 256 queries a workgroup halve the key traffic again, which pays where a
 // sequence is long enough for its last, partly seen tiles not to count.
-template <int D>
+template <int D, bool WINDOW>
 void launch_prompt(const PromptArgs& a, hipStream_t s)
 {
     const std::int64_t cus = conv::cu_count();
@@ -686,17 +783,17 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
         return a.q_heads * std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / queries) + a.sequences);
     };
     if (workgroups(32) <= cus) {
-        if constexpr (D == 128) launch_prompt<PromptCfg<D, 1, 4, 32, 2>>(a, s);
-        else if (a.k_tokens > 512LL * a.sequences) launch_prompt<PromptCfg<64, 1, 8, 32, 2>>(a, s);
-        else launch_prompt<PromptCfg<64, 1, 4, 64, 2>>(a, s);
+        if constexpr (D == 128) launch_prompt<PromptCfg<D, 1, 4, 32, 2>, WINDOW>(a, s);
+        else if (a.k_tokens > 512LL * a.sequences) launch_prompt<PromptCfg<64, 1, 8, 32, 2>, WINDOW>(a, s);
+        else launch_prompt<PromptCfg<64, 1, 4, 64, 2>, WINDOW>(a, s);
     }
-    else if (workgroups(64) <= cus) launch_prompt<PromptCfg<D, 2, 4, D == 64 ? 64 : 32, 2>>(a, s);
-    else if (D == 64 && workgroups(96) <= cus) launch_prompt<PromptCfg<64, 3, 4, 64, 3>>(a, s);
-    else if (D == 64 && workgroups(128) <= cus) launch_prompt<PromptCfg<64, 4, 3, 64, 3>>(a, s);
-    else if (workgroups(128) <= 2 * cus) launch_prompt<PromptCfg<D, 4, 2, 64, 2>>(a, s);
+    else if (workgroups(64) <= cus) launch_prompt<PromptCfg<D, 2, 4, D == 64 ? 64 : 32, 2>, WINDOW>(a, s);
+    else if (D == 64 && workgroups(96) <= cus) launch_prompt<PromptCfg<64, 3, 4, 64, 3>, WINDOW>(a, s);
+    else if (D == 64 && workgroups(128) <= cus) launch_prompt<PromptCfg<64, 4, 3, 64, 3>, WINDOW>(a, s);
+    else if (workgroups(128) <= 2 * cus) launch_prompt<PromptCfg<D, 4, 2, 64, 2>, WINDOW>(a, s);
     else if (D == 128 && a.longest_q >= 4096 && workgroups(128) >= 4 * cus && static_cast<std::int64_t>(a.longest_q) * a.sequences <= 2 * static_cast<std::int64_t>(a.q_tokens))
-        launch_prompt<PromptCfg<128, 8, 1, 64, 2>>(a, s);
-    else launch_prompt<PromptCfg<D, 4, 1, 64, D == 64 ? 3 : 2>>(a, s);
+        launch_prompt<PromptCfg<128, 8, 1, 64, 2>, WINDOW>(a, s);
+    else launch_prompt<PromptCfg<D, 4, 1, 64, D == 64 ? 3 : 2>, WINDOW>(a, s);
 }
 
 void attention_prompt(const mlvc_hip_attention_prompt_desc* d, int window, int sinks, const char* op, hipStream_t s)
@@ -735,8 +832,10 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, int window, int s
     constexpr std::int64_t kFarthest = std::int64_t{1} << 23;
     const bool rows = vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride) && vector_rows(d->k, d->k_stride) &&
                       vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f;
-    if (rows && !a.window && d->head_dim == 128) launch_prompt<128>(a, s);
-    else if (rows && !a.window && d->head_dim == 64) launch_prompt<64>(a, s);
+    // The kernel under a window counts places in 32 bits.
+    const bool fast = rows && (!a.window || static_cast<std::int64_t>(d->q_tokens) + d->k_tokens < (std::int64_t{1} << 30));
+    if (fast && d->head_dim == 128) a.window ? launch_prompt<128, true>(a, s) : launch_prompt<128, false>(a, s);
+    else if (fast && d->head_dim == 64) a.window ? launch_prompt<64, true>(a, s) : launch_prompt<64, false>(a, s);
     else {
         require(launchable(d->q_tokens, 64), op, "too many sequences, heads and queries in one call");
         prompt_any_kernel<<<dim3(static_cast<unsigned>(d->q_tokens), static_cast<unsigned>(d->q_heads)), 64, 0, s>>>(a);

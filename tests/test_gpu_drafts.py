@@ -204,6 +204,70 @@ def test_window_heads_and_strides(dev, rng, dim, q_heads, kv_heads, extra, shift
     _window(dev, rng, [70, 9], [200, 9], q_heads, kv_heads, dim, causal, 40, 6, extra, shift)
 
 
+@pytest.mark.parametrize("queries,keys,q_heads,dim,causal,window,sinks", [
+    ([240], [240], 16, 64, True, 80, 4), ([700, 600], [700, 600], 16, 64, False, 100, 0), ([1500], [1500], 16, 64, True, 333, 70),
+    ([10], [1500], 16, 64, True, 700, 4), ([10], [1500], 16, 128, False, 1, 300), ([920], [920], 16, 128, True, 500, 1),
+    ([2040], [2040], 16, 128, True, 129, 64), ([1, 1200, 333, 64, 700], [1, 1300, 333, 900, 700], 16, 128, True, 256, 9),
+    ([3000, 700], [3000, 900], 16, 64, True, 64, 130), ([4097], [4097], 16, 128, True, 640, 0), ([1100, 40], [1100, 2000], 5, 64, False, 65, 65),
+    ([30] * 70, [100] * 70, 3, 64, True, 33, 2), ([200] * 66, [230] * 66, 2, 128, False, 50, 3),
+])
+def test_window_tiles(dev, rng, queries, keys, q_heads, dim, causal, window, sinks):
+    """Every shape of workgroup, windows that begin and end inside tiles, tiles of sinks beside them."""
+    _window(dev, rng, queries, keys, q_heads, 1, dim, causal, window, sinks)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("queries,keys,q_heads,dim,window,sinks", [
+    ([70], [70], 2, 64, 20, 3), ([200, 33], [300, 33], 2, 128, 40, 70), ([900], [900], 16, 64, 31, 5), ([520], [700], 16, 128, 300, 0),
+    ([300], [300], 2, 96, 33, 2), ([1200], [1200], 16, 128, 1, 66),
+])
+def test_window_of_infinite_values(dev, rng, queries, keys, q_heads, dim, window, sinks, causal):
+    """Infinities and NaN among the values reach the queries that see them, and no others."""
+    q, k, v = normal(rng, sum(queries), q_heads, dim), normal(rng, sum(keys), 1, dim), normal(rng, sum(keys), 1, dim)
+    for value in (np.inf, -np.inf, np.nan):
+        for _ in range(max(2, sum(keys) // 60)):
+            v[rng.integers(0, sum(keys)), 0, rng.integers(0, dim)] = value
+    v[0, 0, 1], v[min(sinks, 60), 0, 2] = np.inf, -np.inf
+    got = Window(Prompt(dev, q, k, v, queries, keys, causal, dim ** -0.5), window, sinks).run()
+    i = j = 0
+    for nq, nk in zip(queries, keys):
+        want, tol = masked64(f64(q[i:i + nq]), f64(k[j:j + nk]), f64(v[j:j + nk]), dim ** -0.5, window_seen(nq, nk, causal, window, sinks))
+        assert np.array_equal(np.isnan(got[i:i + nq]), np.isnan(want)) and np.array_equal(np.isinf(got[i:i + nq]), np.isinf(want))
+        inf = np.isinf(want)
+        assert np.array_equal(got[i:i + nq][inf] > 0, want[inf] > 0)
+        within(got[i:i + nq], want, tol)
+        i, j = i + nq, j + nk
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_window_peaked_and_small_weights(dev, rng, dim):
+    """Scores far apart, and many small weights beside a large one among the sinks."""
+    for spread in (20.0, 0.01):
+        _window(dev, rng, [300], [500], 2, 1, dim, True, 200, 40, spread=spread)
+    n = 1500
+    q, k, v = np.zeros((3, 1, dim), np.float16), np.zeros((n, 1, dim), np.float16), normal(rng, n, 1, dim)
+    q[..., 0], k[0, 0, 0] = 1, 16           # the first key weighs e^16 times the others
+    v[0] = 0
+    got = Window(Prompt(dev, q, k, v, [3], [n], True, 1.0), 1200, 1).run()
+    want, tol = masked64(f64(q), f64(k), f64(v), 1.0, window_seen(3, n, True, 1200, 1))
+    within(got, want, tol)
+
+
+def test_window_strides_past_32_bits(dev, rng):
+    """Keys 2^31 halves and more from the first."""
+    dim, n, stride = 64, 40, 1 << 26
+    base = dev.alloc(2 * (n * stride + dim))
+    rows = normal(rng, n, 1, dim)
+    for i in range(n):
+        dev.check(dev.lib.mlvc_hip_memcpy_h2d(base.value + 2 * i * stride, rows[i].ctypes.data, 2 * dim, None))
+    q = normal(rng, n, 1, dim)
+    p = Prompt(dev, q, rows, rows, [n], [n], True, 0.125)
+    p.desc.k = p.desc.v = base.value
+    p.desc.k_stride = p.desc.v_stride = stride
+    want, tol = masked64(f64(q), f64(rows), f64(rows), 0.125, window_seen(n, n, True, 9, 2))
+    within(Window(p, 9, 2).run(), want, tol)
+
+
 def test_window_of_none_is_the_prompt(dev, rng):
     q, k, v = (normal(rng, 300, 2, 64) for _ in range(3))
     for causal in (False, True):
