@@ -80,6 +80,18 @@ __device__ __forceinline__ std::uint32_t group_max(std::uint32_t x)
     else return x;
 }
 
+// Maximum (sum) of a lane's value and that of the lane 32 away, in both.
+__device__ __forceinline__ float both_max(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_sum(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // Weights go to the matrix cores in FP16, as 2^(score - m) with a base m of the
 // running softmax that lies kLift powers of two below a score: FP16's numbers
 // end at 2^-24, so with the largest weight at 2^12 or more one of 2^-26 of it

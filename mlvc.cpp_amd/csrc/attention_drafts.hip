@@ -30,8 +30,9 @@ struct DraftArgs {
     const std::int32_t* lengths;
     int table_stride, pages, page, heads, q_heads, group, dim, longest, longest_q, q_tokens, streams, window, sinks;
     float scale2;
-    float* part;    // [heads][rows][2 shares + streams][dim], a row for each draft and query head of a group
-    float2* state;  // [heads][rows][2 shares + streams]: base, l
+    float* part;    // [heads][rows][places][dim], a row for each draft and query head of a group
+    float2* state;  // [heads][rows][places]: base, l
+    int places;     // of a row's parts: shares and streams
     int shares;     // workgroups of a key head and a block of rows that the GPU holds at once; 0: a context goes to one workgroup
     int blocks;     // of rows
     bool spare;     // small shares behind the large ones
@@ -71,6 +72,14 @@ struct Sight {
     __device__ bool operator()(int j) const
     {
         return j < past ? j >= from || j < sinks : j - past < kMostDrafts && (drafts >> (j - past) & 1);
+    }
+    // Of the 32 tokens from j on, one a bit; those before `length` that are there.
+    __device__ __forceinline__ unsigned step(int j, int length, bool here0, bool here1) const
+    {
+        auto below = [&](int end) { return end <= j ? 0u : end - j >= 32 ? ~0u : (1u << (end - j)) - 1; };
+        const unsigned context = (~below(from) | below(sinks)) & below(past);
+        const unsigned long long later = past - j >= 64 ? 0 : past >= j ? drafts << (past - j) : j - past >= 64 ? 0 : drafts >> (j - past);
+        return (context | (static_cast<unsigned>(later) & ~below(past))) & below(length) & (here0 ? ~0u : 0xffff0000u) & (here1 ? ~0u : 0xffffu);
     }
 };
 
@@ -223,6 +232,33 @@ __device__ __forceinline__ void decide_odd(const DraftArgs& a, const View& w, co
     for (int r = 0; r < 4; ++r) sums[r] = odd[r].sum(sums[r]);
 }
 
+// Rows of the cache of a stream's tiles of 16 tokens (each in one page), those of
+// 64 tiles at a time, one a lane: the table is read once for 32 steps, and no
+// step waits for it.
+struct Tiles {
+    const DraftArgs& a;
+    const View& w;
+    int stream, head, first = -64;
+    std::int64_t mine = -1;
+    __device__ Tiles(const DraftArgs& a_, const View& w_, int stream_, int head_) : a(a_), w(w_), stream(stream_), head(head_) {}
+    // Of the tiles of a step, from its first token on; -1 for one that is not there.
+    __device__ __forceinline__ void find(int token, std::int64_t* row)
+    {
+        const int tile = token / 16;
+        if (static_cast<unsigned>(tile - first) >= 64u) {
+            first = tile;
+            const int at = token + 16 * static_cast<int>(threadIdx.x & 63);
+            mine = at < w.length ? token_row(a, stream, head, at) : -1;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int lane = tile + t - first;
+            row[t] = static_cast<std::int64_t>(static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), lane))) << 32 |
+                                               static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(mine), lane)));
+        }
+    }
+};
+
 // Heads of D values. The rows of a key head are its drafts times the query heads
 // that share it; a workgroup takes NB blocks of 16 of them, and a part of one
 // stream's context; its waves take consecutive runs of the part, 32 tokens a
@@ -259,8 +295,9 @@ struct DraftCfg {
     static constexpr int DT = D / 16;                  // tiles of O^T
     static constexpr int KS = D / 32;                  // products of a score
     static constexpr int ROWS = NB * 16;
-    static constexpr size_t JOINT = (WAVES * 16 * D + 2 * WAVES * 16) * sizeof(float), QUERIES = NB > 1 ? KS * NB * 1024 : 0;
-    static constexpr size_t LDS = JOINT > QUERIES ? JOINT : QUERIES;
+    static_assert(NB <= 2);
+    static constexpr size_t LDS = (WAVES * 16 * D + 2 * WAVES * 16) * sizeof(float);
+    static_assert(NB == 1 || KS * NB * 1024 <= LDS);
 };
 
 template <class C>
@@ -277,24 +314,14 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
     if (mine <= 0) return;
 
     const int from = first + (last - first) * wave / WAVES, to = first + (last - first) * (wave + 1) / WAVES;
-    typedef const __attribute__((address_space(4))) std::int32_t* scalar_table;
-    const scalar_table table = (scalar_table)(a.table + static_cast<std::int64_t>(stream) * a.table_stride);
-
-    // Rows of the two tiles (16 tokens each, in one page) of a step, row 0 for a
-    // tile that is not there.
+    // Rows of the two tiles of a step, row 0 for a tile that is not there.
+    Tiles tiles(a, w, stream, head);
     std::int64_t row[2];
     bool there[2];
     auto locate = [&](int j) {
-        int at = static_cast<int>(static_cast<unsigned>(j) / static_cast<unsigned>(a.page)), in_page = j - at * a.page;
+        tiles.find(j, row);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            int page = -1;
-            if (j + 16 * t < w.length) page = table[at];
-            there[t] = page >= 0 && page < a.pages;
-            row[t] = there[t] ? (static_cast<std::int64_t>(page) * a.heads + head) * a.page + in_page : 0;
-            in_page += 16;
-            if (in_page == a.page) in_page = 0, ++at;
-        }
+        for (int t = 0; t < 2; ++t) there[t] = row[t] >= 0, row[t] = there[t] ? row[t] : 0;
     };
     u32x4 k[2][C::KL];
     std::uint32_t v[8][C::VW];
@@ -352,7 +379,7 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
 #pragma unroll
         for (int i = 0; i < KS; ++i) q[i] = __builtin_bit_cast(half8, query(0, i, lane));
     } else {
-        for (int i = threadIdx.x; i < KS * NB * 64; i += WAVES * 64) queries[i] = query(i >> 6 & (NB - 1), i >> 6 >> (NB == 4 ? 2 : 1), i & 63);
+        for (int i = threadIdx.x; i < KS * NB * 64; i += WAVES * 64) queries[i] = query(i >> 6 & 1, i >> 7, i & 63);
     }
     if (wave == 0) {
         const unsigned long long mask = mask_of(a, w, lane);
@@ -416,10 +443,10 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
         }
         const bool masked = j + kStep > w.past || !there[0] || !there[1] || (j < clear_from && j + kStep > w.sinks);
         const bool here[2] = {there[0], there[1]};
-        if (step + 1 < to) {
-            locate(w.token(step + 1));
-            fetch_k();
-        }
+        // The last step asks for itself again: so that there are always as many loads,
+        // and the wait for K leaves V on its way.
+        locate(w.token(min(step + 1, to - 1)));
+        fetch_k();
         if (masked) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -444,14 +471,11 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
             float x[8], p[8], wt[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = dot[b][e >> 2][e & 3] * factor[e];
-            unsigned unseen = 0;
+            unsigned see = ~0u;
             if (masked) {
-                const Sight sight = sights[draft[b]];
+                see = sights[draft[b]].step(j, w.length, here[0], here[1]) >> 4 * g;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int at = j + 16 * (e >> 2) + 4 * g + (e & 3);
-                    if (!here[e >> 2] || at >= w.length || !sight(at)) unseen |= 1u << e, x[e] = -INFINITY;
-                }
+                for (int e = 0; e < 8; ++e) x[e] = see >> (16 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY;
             }
             auto weigh = [&] {
 #pragma unroll
@@ -462,7 +486,7 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
                 if (KIND != MLVC_KV_F16 && masked) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (unseen >> e & 1) wt[e] = 0.0f;
+                        wt[e] = see >> (16 * (e >> 2) + (e & 3)) & 1 ? wt[e] : 0.0f;
                 }
             };
             weigh();
@@ -503,7 +527,7 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
                 }
             }
         }
-        if (step + 1 < to) fetch_v();
+        fetch_v();
     }
     if (KIND == MLVC_KV_F16 && met) *odd_met = 1;
 
@@ -546,11 +570,319 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
                 *reinterpret_cast<uint2*>(a.out + (w.start + of) * a.out_stride + static_cast<std::int64_t>(head * a.group + at - of * a.group) * D + d) =
                     make_uint2(pack_rounded(sum[0] * f, sum[1] * f), pack_rounded(sum[2] * f, sum[3] * f));
             } else {
-                const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + at) * (2 * a.shares + a.streams) + place;
+                const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + at) * a.places + place;
                 *reinterpret_cast<floatx4*>(a.part + slot * D + d) = sum;
                 if (d == 0) a.state[slot] = make_float2(top, total);
             }
         }
+    }
+}
+
+// More rows than 32: RG x KG waves take RG * 32 rows. The KG groups of waves take
+// every KG-th step of the part, and put their states together at the end. The
+// waves of a group unpack the step's rows of the cache to halves in LDS, once for
+// all of them, while the next step's are on their way to registers; each wave
+// holds 32 rows as columns of S^T = K Q^T (32x32x16 products, keys as rows), so
+// that a lane's scores all belong to one row, and rounded to halves they are the
+// B operand of O^T += V^T P^T as they stand. 16-byte pieces of a row are permuted
+// in LDS (piece ^ f(row)) against bank conflicts; V is read transposing.
+template <int KIND_, int D_, int RG_, int KG_>
+struct TileCfg {
+    static constexpr int KIND = KIND_, D = D_, RG = RG_, KG = KG_, WAVES = RG * KG, ROWS = RG * 32, OCC = 2;
+    static constexpr int BYTES = KIND == MLVC_KV_F16 ? 2 : 1;
+    static constexpr int TILE = kStep * D;                     // halves of K or V of a step
+    static constexpr int LOADS = 2 * kStep * D * BYTES / 1024; // of a wave, for K and V of a step
+    static constexpr int MINE = (LOADS + RG - 1) / RG;         // of each wave of a group
+    static constexpr int DEPTH = KIND == MLVC_KV_F16 ? 1 : 2;     // steps on their way
+    static constexpr int WORDS = D / 8 + 1;                    // 16-byte words of a lane's state
+    static constexpr size_t TILES = KG * 2 * 2 * TILE * 2, SCALES = KG * 2 * 2 * kStep * sizeof(float),
+                            JOINT = static_cast<size_t>(KG - 1) * WORDS * RG * 64 * 16;
+    static constexpr size_t LDS = TILES + SCALES > JOINT ? TILES + SCALES : JOINT;
+    __host__ __device__ static constexpr int swizzle(int t)
+    {
+        return D == 128 ? 4 * (t & 3) + (t >> 2 & 3) : 4 * (t >> 1 & 1) + (t >> 2 & 3);
+    }
+};
+
+template <class C>
+__device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight* sights, int* odd_met, int head, int block, int stream, const View& w,
+                                           int first, int last, bool whole, int place)
+{
+    constexpr int D = C::D, KIND = C::KIND, RG = C::RG, KG = C::KG, KS = D / 16, DT = D / 32, RB = D * C::BYTES;
+    constexpr float kBase0 = -3.402823466e38f;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RG, kg = wave / RG, column = lane & 31, hi = lane >> 5;
+    const int rows = w.queries * a.group, row0 = block * C::ROWS, mine = min(C::ROWS, rows - row0);
+    if (mine <= 0) return;
+    std::uint16_t* const tiles = reinterpret_cast<std::uint16_t*>(lds) + kg * 4 * C::TILE;      // [buffer][K, V][TILE]
+    float* const scales = reinterpret_cast<float*>(lds + C::TILES) + kg * 4 * kStep;            // [buffer][scale_k, scale_v][kStep]
+
+    // A step that is on its way: its first token, whether its tiles are there, its rows as they lie in the cache.
+    struct Coming {
+        int j = 0;
+        bool there[2] = {false, false};
+        u32x4 raw[C::MINE];
+        float scale = 0.0f;
+    };
+    Tiles table(a, w, stream, head);
+    Coming coming[C::DEPTH];
+    auto fetch = [&](int step, Coming& c) {
+        std::int64_t row[2];
+        c.j = w.token(step);
+        table.find(c.j, row);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) c.there[t] = row[t] >= 0, row[t] = c.there[t] ? row[t] : 0;
+#pragma unroll
+        for (int i = 0; i < C::MINE; ++i) {
+            const int n = rg + i * RG;
+            if (C::LOADS % RG != 0 && n >= C::LOADS) continue;
+            const bool is_v = n >= C::LOADS / 2;
+            const int byte = (n - (is_v ? C::LOADS / 2 : 0)) * 1024, t = byte / RB / 16;
+            c.raw[i] = *reinterpret_cast<const u32x4*>((is_v ? a.v : a.k) + (t ? row[1] : row[0]) * RB + (byte - t * 16 * RB) + lane * 16);
+        }
+        if constexpr (KIND != MLVC_KV_F16) c.scale = (hi ? a.v_scale : a.k_scale)[(lane & 16 ? row[1] : row[0]) + (lane & 15)];
+    };
+    // Always as many loads, the last step's again past the end: so that the wait
+    // for a step leaves the next one's on their way.
+    if (first < last)
+#pragma unroll
+        for (int i = 0; i < C::DEPTH; ++i) fetch(min(first + i * KG + kg, last - 1), coming[i]);
+
+    if (wave == 0) {
+        const unsigned long long mask = mask_of(a, w, lane);
+        const int depth = depth_of(mask, lane);
+        Sight s;
+        s.past = w.past, s.sinks = w.sinks;
+        s.from = a.window ? max(w.past + depth - a.window + 1, 0) : 0;
+        s.drafts = mask;
+        if (a.window && a.window < kMostDrafts)
+            for (int e = 0; e < kMostDrafts; ++e) {
+                const int other = __builtin_amdgcn_readlane(depth, e);
+                if (depth - other >= a.window && w.past + other >= a.sinks) s.drafts &= ~(1ull << e);
+            }
+        sights[lane] = s;
+        if (lane == 0) *odd_met = 0;
+    }
+    // This lane's row: of a draft and a query head.
+    const int at_row = row0 + min(rg * 32 + column, mine - 1), draft = static_cast<int>(static_cast<unsigned>(at_row) / static_cast<unsigned>(a.group));
+    const bool has_rows = rg * 32 < mine, my_row = rg * 32 + column < mine;
+    const std::int64_t token = w.start + draft, at_head = static_cast<std::int64_t>(head * a.group + at_row - draft * a.group) * D;
+    half8 q[KS];
+    {
+        const std::uint16_t* x = a.q + token * a.q_stride + at_head + hi * 8;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) q[i] = __builtin_bit_cast(half8, *reinterpret_cast<const u32x4*>(x + i * 16));
+    }
+    const int clear_from = a.window ? max(w.past + min(w.drafts, kMostDrafts) - a.window, 0) : 0;
+
+    // Places of this lane's pieces: of K, pieces 2 ks + hi of row lane & 31; of V,
+    // the transposing read of 16 lanes takes 4 halves of each of 4 rows (4 hi + 8 e
+    // + 0..3 of a 16-row step) a lane and returns one column's four.
+    int kat[KS], vat[DT][2];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) kat[i] = column * D + ((2 * i + hi) ^ C::swizzle(column)) * 8;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = 8 * e + 4 * hi + ((lane & 15) >> 2);
+            vat[dt][e] = r * D + ((4 * dt + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ C::swizzle(r)) * 8 + (lane & 1) * 4;
+        }
+    floatx16 acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[dt][r] = 0.0f;
+    float base = kBase0, l = 0.0f;
+    bool met = false;
+    __syncthreads();
+    const Sight sight = sights[draft];
+
+    // The step that came in, as halves in LDS; what rows that do not see it must
+    // not meet is zeroed.
+    auto unpack = [&](const Coming& c, int buffer, bool masked) {
+        std::uint16_t* const tile = tiles + buffer * 2 * C::TILE;
+#pragma unroll
+        for (int i = 0; i < C::MINE; ++i) {
+            const int n = rg + i * RG;
+            if (C::LOADS % RG != 0 && n >= C::LOADS) continue;
+            const bool is_v = n >= C::LOADS / 2;
+            const int byte = (n - (is_v ? C::LOADS / 2 : 0)) * 1024 + lane * 16, r = byte / RB, piece = byte % RB / 16 * (2 / C::BYTES);
+            std::uint16_t* const to = tile + (is_v ? C::TILE : 0) + r * D;
+            const bool gone = masked && is_v && (!(r & 16 ? c.there[1] : c.there[0]) || c.j + r >= w.length);
+            auto put = [&](int at, u32x4 x) {
+                if (masked && is_v) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const std::uint32_t odd = KIND == MLVC_KV_INT8 ? 0u : ((x[e] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((x[e] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+                        if (KIND == MLVC_KV_F16) met |= !gone && odd;
+                        x[e] = gone ? 0u : x[e] & ~odd;
+                    }
+                }
+                *reinterpret_cast<u32x4*>(to + (at ^ C::swizzle(r)) * 8) = x;
+            };
+            if constexpr (KIND == MLVC_KV_F16) {
+                put(piece, c.raw[i]);
+            } else {
+                put(piece, __builtin_bit_cast(u32x4, eight<KIND>(c.raw[i][0], c.raw[i][1])));
+                put(piece + 1, __builtin_bit_cast(u32x4, eight<KIND>(c.raw[i][2], c.raw[i][3])));
+            }
+        }
+        if (KIND != MLVC_KV_F16 && rg == 0)
+            scales[buffer * 2 * kStep + lane] = hi ? __builtin_elementwise_maximum(c.scale, 0x1p-40f) : c.scale * a.scale2;
+    };
+    auto compute = [&](int buffer, int j, bool masked, bool here0, bool here1) {
+#pragma clang fp contract(off)  // a score less the base: of the score as it was when the base was taken
+        const std::uint16_t* const tile_k = tiles + buffer * 2 * C::TILE;
+        const std::uint16_t* const tile_v = tile_k + C::TILE;
+        floatx16 s;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8*>(tile_k + kat[i]), q[i], i ? s : floatx16{}, 0, 0, 0);
+        float x[16], scale[16], p[16], wt[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            floatx4 f = {a.scale2, a.scale2, a.scale2, a.scale2}, t = {1.0f, 1.0f, 1.0f, 1.0f};
+            if constexpr (KIND != MLVC_KV_F16) {
+                f = *reinterpret_cast<const floatx4*>(scales + buffer * 2 * kStep + 8 * g + 4 * hi);
+                t = *reinterpret_cast<const floatx4*>(scales + buffer * 2 * kStep + kStep + 8 * g + 4 * hi);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * g + e] = s[4 * g + e] * f[e], scale[4 * g + e] = t[e];
+        }
+        if (masked) {
+            const unsigned see = sight.step(j, w.length, here0, here1) >> 4 * hi;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool seen = see >> (8 * (r >> 2) + (r & 3)) & 1;
+                x[r] = seen ? x[r] : -INFINITY, scale[r] = seen ? scale[r] : 1.0f;
+            }
+        }
+        auto weigh = [&] {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                p[r] = __builtin_amdgcn_exp2f(x[r] - base);
+                wt[r] = KIND == MLVC_KV_F16 ? p[r] : p[r] * scale[r];
+            }
+        };
+        weigh();
+        float top = wt[0];
+#pragma unroll
+        for (int r = 1; r < 15; r += 2) top = fmaxf(fmaxf(top, wt[r]), wt[r + 1]);
+        top = fmaxf(top, wt[15]);
+        if (__any(top > 0x1p15f)) {
+            top = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, KIND == MLVC_KV_F16 ? x[r] : x[r] + __builtin_amdgcn_logf(scale[r]));
+            const float now = fmaxf(base, lifted(both_max(top))), keep = __builtin_amdgcn_exp2f(base - now);
+            l *= keep;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[dt][r] *= keep;
+            base = now;
+            weigh();
+        }
+        float sum[4] = {};
+        half8 weights[2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[r & 3] += p[r], weights[r >> 3][r & 7] = static_cast<_Float16>(wt[r]);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                u32x2 v[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    v[e] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                         (__attribute__((address_space(3))) s16x4*)(tile_v + vat[dt][e] + h * 16 * D)));
+                acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, u32x4{v[0][0], v[0][1], v[1][0], v[1][1]}), weights[h], acc[dt], 0, 0, 0);
+            }
+    };
+    const int turns = (last - first + KG - 1) / KG;
+    auto take_turn = [&](int turn, Coming& c) {
+        const int step = first + turn * KG + kg, buffer = turn & 1, j = c.j;
+        const bool here0 = c.there[0], here1 = c.there[1];
+        const bool masked = j + kStep > w.past || !here0 || !here1 || (j < clear_from && j + kStep > w.sinks);
+        unpack(c, buffer, masked);
+        fetch(min(step + C::DEPTH * KG, last - 1), c);
+        __syncthreads();
+        if (step < last && has_rows) compute(buffer, j, masked, here0, here1);
+    };
+    for (int turn = 0; turn < turns; turn += C::DEPTH) {
+        take_turn(turn, coming[0]);
+        if constexpr (C::DEPTH > 1)
+            if (turn + 1 < turns) take_turn(turn + 1, coming[1]);
+    }
+    if (KIND == MLVC_KV_F16 && met) *odd_met = 1;
+
+    // The other groups hand their states to the first, lane by lane.
+    __syncthreads();
+    l = both_sum(l);
+    if constexpr (KG > 1) {
+        floatx4* const states = reinterpret_cast<floatx4*>(lds) + rg * 64 + lane;
+        if (kg > 0 && has_rows) {
+            floatx4* const to = states + (kg - 1) * C::WORDS * RG * 64;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    to[(dt * 4 + g) * RG * 64] = floatx4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+            to[DT * 4 * RG * 64] = floatx4{base, l, 0.0f, 0.0f};
+        }
+        __syncthreads();
+        if (kg > 0 || !has_rows) return;
+#pragma unroll
+        for (int n = 0; n < KG - 1; ++n) {
+            const floatx4* const from = states + n * C::WORDS * RG * 64;
+            const floatx4 st = from[DT * 4 * RG * 64];
+            const float now = fmaxf(base, st[0]), old = __builtin_amdgcn_exp2f(base - now), f = __builtin_amdgcn_exp2f(st[0] - now);
+            base = now;
+            l = l * old + st[1] * f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const floatx4 v = from[(dt * 4 + g) * RG * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[dt][4 * g + e] = acc[dt][4 * g + e] * old + v[e] * f;
+                }
+        }
+    }
+    if (!my_row) return;
+    if constexpr (KIND == MLVC_KV_F16) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                floatx4 v = {acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+                if (*odd_met || !is_finite(v[0]) || !is_finite(v[1]) || !is_finite(v[2]) || !is_finite(v[3])) {
+                    decide_odd(a, w, sight, stream, head, first, last, dt * 32 + 8 * g + 4 * hi, v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[dt][4 * g + e] = v[e];
+                }
+            }
+    }
+    if (whole) {
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        std::uint16_t* const out = a.out + token * a.out_stride + at_head + 4 * hi;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<uint2*>(out + dt * 32 + 8 * g) = make_uint2(pack_rounded(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f),
+                                                                              pack_rounded(acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f));
+    } else {
+        const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + at_row) * a.places + place;
+        float* const part = a.part + slot * D + 4 * hi;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<floatx4*>(part + dt * 32 + 8 * g) = floatx4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+        if (hi == 0) a.state[slot] = make_float2(base, l);
     }
 }
 
@@ -565,14 +897,18 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void drafts_kernel(DraftArgs
     __shared__ int odd_met;
     const int turn = blockIdx.x / kXcds, block = turn % a.blocks, item = a.blocks == 1 ? blockIdx.x : turn / a.blocks * kXcds + blockIdx.x % kXcds;
     const int head = item % a.heads, rest = item / a.heads;
+    auto take = [&](int stream, const View& w, int first, int last, bool whole, int place) {
+        if constexpr (requires { C::NB; }) draft_piece<C>(a, lds, sights, &odd_met, head, block, stream, w, first, last, whole, place);
+        else tile_piece<C>(a, lds, sights, &odd_met, head, block, stream, w, first, last, whole, place);
+    };
     if constexpr (SHARES)
         each_piece(a, rest, [&](int stream, int first, int last, bool whole, int place) {
-            draft_piece<C>(a, lds, sights, &odd_met, head, block, stream, View(a, stream), first, last, whole, place);
+            take(stream, View(a, stream), first, last, whole, place);
             __syncthreads();  // before the next piece's queries and states
         });
     else if (rest < a.streams) {
         const View w(a, rest);
-        draft_piece<C>(a, lds, sights, &odd_met, head, block, rest, w, 0, w.steps, true, 0);
+        take(rest, w, 0, w.steps, true, 0);
     }
 }
 
@@ -600,7 +936,7 @@ __global__ __launch_bounds__(LANES* ROWS* GROUPS) void drafts_join_kernel(DraftA
     const Shares shares(a.shares, total, a.spare);
     const int first = w.steps ? shares.holder(start) : 0, parts = w.steps ? shares.holder(start + w.steps - 1) - first + 1 : 0;
     if (parts == 1) return;  // written by the share that holds it
-    const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + row) * (2 * a.shares + a.streams) + first + stream;
+    const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + row) * a.places + first + stream;
     const int d = at * 4;
     float base = kBase0, l = 0.0f;
     floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -650,14 +986,6 @@ __global__ __launch_bounds__(LANES* ROWS* GROUPS) void drafts_join_kernel(DraftA
         make_uint2(pack_rounded(sum[0] * f, sum[1] * f), pack_rounded(sum[2] * f, sum[3] * f));
 }
 
-// How a call is laid out; from what the host knows.
-struct Plan {
-    int nb, blocks, shares;
-    bool fast, spare;
-    std::int64_t row_count;  // rows of all key heads
-    size_t part_bytes, bytes;
-};
-
 void check_desc(const mlvc_hip_attention_drafts_desc* d, const char* op)
 {
     require(d != nullptr, op, "no descriptor");
@@ -670,56 +998,101 @@ void check_desc(const mlvc_hip_attention_drafts_desc* d, const char* op)
     require(std::isfinite(d->scale), op, "scale must be finite");
 }
 
-// Whether a context goes to one workgroup, without a cut.
-bool whole(std::int64_t longest, std::int64_t workgroups)
-{
-    const std::int64_t cus = conv::cu_count();
-    return longest <= 1024 || (longest <= 2048 && 2 * workgroups >= cus) || (longest <= 4096 && workgroups >= 3 * cus);
-}
+// Workgroups: rows of one, and how many fit a CU.
+enum Shape { kOne8, kOne4, kTwo4, kTile21, kTile22, kTile41, kTile42 };
+constexpr int kRows[] = {16, 16, 32, 64, 64, 128, 128}, kPerCu[] = {1, 3, 2, 4, 2, 2, 1};
 
+// How a call is laid out; from what the host knows.
+struct Plan {
+    Shape shape;
+    int blocks, shares;
+    bool fast;
+    std::int64_t row_count;  // rows of all key heads
+    size_t part_bytes, bytes;
+};
+
+// Contexts of few steps go to one workgroup each, whole: by 8 waves for 16 rows
+// while there are no more workgroups than CUs, then to workgroups of as many rows
+// as still let all of them run at once. Others are cut into shares: for 16 rows
+// while a wave has few steps, as more rows take longer to start and to join; else
+// for as many as let each cached row be unpacked for all rows of a head, or for
+// two workgroups of them. Shapes with more rows than 32 unpack into LDS; a CU
+// holds four of two waves, which leave the most independent of each other, where
+// there are enough contexts for the parts they leave not to count. us, E4M3 or
+// INT8, 32 / 8 heads of 128 where not said otherwise, the one taken marked *:
+//   whole                            One8  One4  Two4  Tile22
+//     1 x 16 drafts, 920 tokens, 16 / 4 of 64
+//                                    9.6*        14.1  19.6
+//     1 x 64, 920                    14.7*       20.2  26.8
+//     8 x 16, 500 to 2000            20.7*       28.8  48.7
+//     16 x 16, 200 to 1000           26.7        20.4* 28.4
+//     32 x 16, 500 to 2000           67.6        38.6* 50.2
+//     64 x 16, 200 to 1000           96.4        48.7  38.3*
+//   shares                           One4  Two4  Tile21 Tile22 Tile41 Tile42
+//     1 x 16, 4000                   17.5* 17.9         20.8
+//     1 x 8, 65280                   45.9  40.4* 45.4   42.8
+//     1 x 16, 65280                  77.8  50.3  53.8   51.6*  64.6   68.8
+//     64 x 8, 16 to 8160             165   141*  142    151    197    242
+//     64 x 16, 16 to 8160            256   192   172*   179    226    263
+//     16 x 64, 920 to 3001, 16 / 16 of 64, FP16
+//                                    58.6  51.9  43.9   39.9*  46.1   49.9
+//     8 x 32, 4000 to 8160, FP16     151   90.1  75.0   70.9   73.9   67.2*
+//     1 x 64, 65280                  223   128   130    132    123*   129
+//     64 x 64, 64 to 8160            906   599   524    563    476*   537
 Plan plan(const mlvc_hip_attention_drafts_desc* d)
 {
     Plan p{};
     const mlvc_hip_kv_cache* c = d->cache;
-    const std::int64_t rows = static_cast<std::int64_t>(d->longest_q) * (d->q_heads / c->heads), blocks = (rows + 15) / 16;
+    const std::int64_t rows = static_cast<std::int64_t>(d->longest_q) * (d->q_heads / c->heads), cus = conv::cu_count();
     p.row_count = rows * c->heads;
     p.fast = c->head_dim == 64 || c->head_dim == 128;
-    p.nb = blocks <= 1 ? 1 : blocks == 2 ? 2 : 4;
-    p.blocks = static_cast<int>((blocks + p.nb - 1) / p.nb);
-    p.spare = p.nb == 1;
     if (!p.fast) return p;
     // Tokens that a stream's drafts see at most, and those beside them in their steps.
     std::int64_t longest = d->longest;
-    if (d->window) longest = std::min(longest, static_cast<std::int64_t>(d->window) + kMostDrafts + std::min(d->sinks, d->longest) + 2 * kStep);
+    if (d->window) longest = std::min(longest, static_cast<std::int64_t>(d->window) + d->longest_q + std::min(d->sinks, d->longest) + 2 * kStep);
+    auto workgroups = [&](Shape shape) { return (rows + kRows[shape] - 1) / kRows[shape] * c->heads * d->streams; };
+    auto take = [&](Shape shape) { p.shape = shape, p.blocks = static_cast<int>((rows + kRows[shape] - 1) / kRows[shape]); };
+    take(workgroups(kOne4) <= cus                                     ? kOne8
+         : rows <= 16                                                 ? kOne4
+         : rows <= 32 || workgroups(kTwo4) <= 2 * cus                 ? kTwo4
+         : rows <= 64 || workgroups(kTile22) <= 4 * cus               ? kTile22
+                                                                      : kTile41);
     if (longest <= 1024) return p;
-    const std::int64_t of_stream = static_cast<std::int64_t>(c->heads) * p.blocks;
-    const int shares = static_cast<int>(std::max<std::int64_t>(1, (p.nb == 1 ? 3 : 1) * conv::cu_count() / of_stream));
-    const size_t slots = (2 * static_cast<size_t>(shares) + d->streams) * p.row_count;
+    // Parts: each share leaves one a row, and one for each context that begins in
+    // it. Asked for whether this call cuts or not and for the shape that leaves the
+    // most, so that what is enough for a batch is enough for a smaller one.
+    const size_t slots = 256 * static_cast<size_t>(cus) + (d->streams + 2) * static_cast<size_t>(p.row_count);
     p.part_bytes = slots * c->head_dim * sizeof(float);
-    // Asked for whether this call cuts or not, so that what is enough for a
-    // batch is enough for a smaller one.
     p.bytes = p.part_bytes + slots * sizeof(float2);
-    if (!whole(longest, d->streams * of_stream)) p.shares = shares;
+    const std::int64_t whole = workgroups(p.shape);
+    if ((longest <= 2048 && 2 * whole >= cus) || (longest <= 4096 && whole >= 3 * cus)) return p;
+    const bool bytes = c->kind != MLVC_KV_F16, many = static_cast<std::int64_t>(c->heads) * d->streams >= cus;
+    take(rows <= 16 || workgroups(kOne4) * (longest / kStep) <= 48 * cus ? kOne4
+         : rows <= 32                                                    ? kTwo4
+         : rows <= 64                                                    ? (bytes && many ? kTile21 : kTile22)
+                                                                         : (bytes ? kTile41 : kTile42));
+    p.shares = static_cast<int>(std::max<std::int64_t>(1, kPerCu[p.shape] * cus / (static_cast<std::int64_t>(c->heads) * p.blocks)));
     return p;
 }
 
-template <class C, bool SHARES>
+template <class C>
 void launch_drafts(const DraftArgs& a, unsigned grid, hipStream_t s)
 {
-    drafts_kernel<C, SHARES><<<grid, C::WAVES * 64, C::LDS, s>>>(a);
+    if (a.shares) drafts_kernel<C, true><<<grid, C::WAVES * 64, C::LDS, s>>>(a);
+    else drafts_kernel<C, false><<<grid, C::WAVES * 64, C::LDS, s>>>(a);
 }
 
 template <int KIND, int D>
-void launch_drafts(const DraftArgs& a, int nb, unsigned grid, hipStream_t s)
+void launch_drafts(const DraftArgs& a, Shape shape, unsigned grid, hipStream_t s)
 {
-    if (a.shares) {
-        if (nb == 1) launch_drafts<DraftCfg<KIND, D, 1, 4, 3>, true>(a, grid, s);
-        else if (nb == 2) launch_drafts<DraftCfg<KIND, D, 2, 8, 2>, true>(a, grid, s);
-        else launch_drafts<DraftCfg<KIND, D, 4, D == 64 ? 8 : 4, D == 64 ? 2 : 1>, true>(a, grid, s);
-    } else {
-        if (nb == 1) launch_drafts<DraftCfg<KIND, D, 1, 8, 2>, false>(a, grid, s);
-        else if (nb == 2) launch_drafts<DraftCfg<KIND, D, 2, 8, 2>, false>(a, grid, s);
-        else launch_drafts<DraftCfg<KIND, D, 4, D == 64 ? 8 : 4, D == 64 ? 2 : 1>, false>(a, grid, s);
+    switch (shape) {
+    case kOne8: return launch_drafts<DraftCfg<KIND, D, 1, 8, 2>>(a, grid, s);
+    case kOne4: return launch_drafts<DraftCfg<KIND, D, 1, 4, 3>>(a, grid, s);
+    case kTwo4: return launch_drafts<DraftCfg<KIND, D, 2, 4, 2>>(a, grid, s);
+    case kTile21: return launch_drafts<TileCfg<KIND, D, 2, 1>>(a, grid, s);
+    case kTile22: return launch_drafts<TileCfg<KIND, D, 2, 2>>(a, grid, s);
+    case kTile41: return launch_drafts<TileCfg<KIND, D, 4, 1>>(a, grid, s);
+    case kTile42: return launch_drafts<TileCfg<KIND, D, 4, 2>>(a, grid, s);
     }
 }
 
@@ -727,8 +1100,8 @@ template <int KIND>
 void launch_drafts(const DraftArgs& a, const Plan& p, bool fast, unsigned grid, hipStream_t s)
 {
     if (!fast) drafts_any_kernel<KIND><<<grid, 64, 0, s>>>(a);
-    else if (a.dim == 64) launch_drafts<KIND, 64>(a, p.nb, grid, s);
-    else launch_drafts<KIND, 128>(a, p.nb, grid, s);
+    else if (a.dim == 64) launch_drafts<KIND, 64>(a, p.shape, grid, s);
+    else launch_drafts<KIND, 128>(a, p.shape, grid, s);
 }
 
 template <int LANES>
@@ -763,7 +1136,7 @@ void attention_drafts(const mlvc_hip_attention_drafts_desc* d, hipStream_t s)
     const std::int64_t all_rows = static_cast<std::int64_t>(d->streams) * p.row_count;
     std::int64_t grid = all_rows;
     if (fast) {
-        const std::int64_t items = static_cast<std::int64_t>(d->cache->heads) * (p.shares ? (p.spare ? 2 : 1) * p.shares : d->streams);
+        const std::int64_t items = static_cast<std::int64_t>(d->cache->heads) * (p.shares ? (p.shape == kOne4 ? 2 : 1) * p.shares : d->streams);
         grid = p.blocks == 1 ? items : (items + kXcds - 1) / kXcds * kXcds * p.blocks;
     }
     require(launchable(grid, fast ? 512 : 64) && launchable(all_rows, 256) &&
@@ -786,7 +1159,8 @@ void attention_drafts(const mlvc_hip_attention_drafts_desc* d, hipStream_t s)
     a.scale2 = d->scale * 1.4426950408889634f;
     a.part = static_cast<float*>(d->workspace);
     a.state = reinterpret_cast<float2*>(static_cast<char*>(d->workspace) + p.part_bytes);
-    a.shares = p.shares, a.blocks = p.blocks, a.spare = p.spare;
+    a.shares = p.shares, a.blocks = p.blocks, a.spare = p.shape == kOne4;
+    a.places = (a.spare ? 2 : 1) * a.shares + a.streams;
     const unsigned n = static_cast<unsigned>(grid);
     if (c->kind == MLVC_KV_F16) launch_drafts<MLVC_KV_F16>(a, p, fast, n, s);
     else if (c->kind == MLVC_KV_E4M3) launch_drafts<MLVC_KV_E4M3>(a, p, fast, n, s);

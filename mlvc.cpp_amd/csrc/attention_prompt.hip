@@ -143,18 +143,6 @@ __device__ __forceinline__ std::uint32_t lds_address(const void* p)
     return static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) const void*)p));
 }
 
-// Maximum (sum) of a lane's value and that of the lane 32 away, in both.
-__device__ __forceinline__ float both_max(float x)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float both_sum(float x)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // Heads of D values, rows on 16 bytes. A workgroup of RG x KG waves takes
 // RG * 32 queries of a head. A wave holds 32 of them as columns of S^T = K Q^T
 // (32x32x16 products, keys as rows), so that

@@ -321,6 +321,95 @@ def test_drafts_in_a_chain_on_long_contexts(dev, rng, kind, dim, window, sinks):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_heads,heads,counts,lengths,window,sinks", [
+    # Whole contexts: 16 rows of many streams, 32 rows, 64, 128.
+    (4, 2, [1, 3, 2] * 50, [5, 300, 77] * 50, 0, 0),
+    (4, 1, [8, 5, 6] * 35, [205, 70, 33] * 35, 64, 40),
+    (16, 8, [20, 17, 1] * 11, [150, 64, 40] * 11, 0, 0),
+    (16, 8, [64, 40, 33, 50, 1] * 13, [70, 130, 64, 96, 33] * 13, 50, 3),
+    # Cut ones: 32 rows, 64, 64 of many streams, 128.
+    (4, 2, [15, 9] * 20, [2600, 31] + [77, 40] * 19, 0, 0),
+    (6, 2, [20, 16] * 20, [2600, 31] + [77, 40] * 19, 0, 0),
+    (16, 8, [20] * 33, [2300] + [60] * 31 + [2100], 0, 0),
+    (4, 2, [64, 3, 33], [8300, 40, 700], 0, 0),
+    (4, 2, [64, 3, 33], [9000, 40, 8700], 8400, 100),
+])
+def test_drafts_shapes(dev, rng, kind, dim, q_heads, heads, counts, lengths, window, sinks):
+    """Every number of rows a workgroup takes, contexts whole and cut."""
+    _drafts(dev, rng, kind, q_heads, heads, dim, 16, counts, lengths, window, sinks)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_heads,drafts,n", [(2, 3, 700), (4, 16, 700), (6, 40, 300), (2, 5, 1500), (4, 60, 6000), (2, 20, 9000)])
+def test_drafts_of_zero_values_and_far_scores(dev, rng, kind, dim, q_heads, drafts, n):
+    """Zero rows of V that weigh most, rows of far smaller values beside large ones, scores far apart."""
+    ctx = Contexts(dev, rng, Cache, kind, 1, dim, 16, [n])
+    k, v = ctx.k[0], ctx.v[0]
+    v[: n // 3] *= np.float16(2.0 ** -12)
+    top = rng.permutation(n)[: n // 4]
+    v[top] = 0
+    k[top] *= np.float16(3)
+    k[n // 2:] *= np.float16(8)
+    ctx.cache.write(k, v, ctx.slots(0, np.arange(n)))
+    q = normal(rng, drafts, q_heads, dim)
+    masks = tree(rng, drafts)
+    got = Drafts(ctx.cache, q, [drafts], masks, ctx.table, [n], 0.2).run()
+    want, tol = masked64(f64(q), stored64(k, kind), stored64(v, kind), 0.2, drafts_seen(n, masks, 0, 0), tops_of(v, kind))
+    within(got, want, tol)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("q_heads,drafts,dim", [(2, 3, 64), (4, 8, 128), (6, 40, 128), (4, 64, 64)])
+def test_drafts_of_large_scores(dev, rng, kind, q_heads, drafts, dim):
+    """Scores of 2^22 and more, whose last place is more than the weights' own: the largest decides."""
+    n = 260
+    ctx = Contexts(dev, rng, Cache, kind, 1, dim, 16, [n])
+    k = np.zeros((n, 1, dim), np.float16)
+    k[:, 0, 0] = rng.permutation(n) + 1     # whole multiples of a power of two once scaled: one key far above the others
+    k[:, 0, 1] = n                          # the rows' largest value: quantised alike
+    ctx.cache.write(k, ctx.v[0], ctx.slots(0, np.arange(n)))
+    q = np.zeros((drafts, q_heads, dim), np.float16)
+    q[..., 0] = 256
+    masks = tree(rng, drafts)
+    got = Drafts(ctx.cache, q, [drafts], masks, ctx.table, [n], 2.0 ** 18).run()
+    sk, sv, seen = stored64(k, kind), stored64(ctx.v[0], kind), drafts_seen(n, masks, 0, 0)
+    for i in range(drafts):
+        see = np.flatnonzero(seen[i])
+        best = see[sk[see, 0, 0] == sk[see, 0, 0].max()]
+        want = sv[best, 0].mean(0)
+        tol = np.abs(sv[best, 0]).max(0) * 2.0 ** -9 + 2.0 ** -24
+        for h in range(q_heads):
+            within(got[i, h], want, tol, f"draft {i}")
+
+
+@pytest.mark.parametrize("q_heads,drafts,dim,n", [(2, 3, 64, 200), (4, 8, 128, 900), (6, 40, 128, 300), (4, 64, 64, 3000), (4, 30, 128, 5000), (2, 9, 96, 100)])
+def test_drafts_of_infinite_values(dev, rng, q_heads, drafts, dim, n):
+    """Infinities and NaN among the values of an FP16 cache reach the drafts that see them, and no others."""
+    ctx = Contexts(dev, rng, Cache, KV_F16, 1, dim, 16, [n, n])
+    trees = [tree(rng, drafts), tree(rng, drafts)]
+    for stream in range(2):
+        v = ctx.v[stream]
+        for value in (np.inf, -np.inf, np.nan):
+            if stream == 0:
+                v[rng.integers(0, n - drafts), 0, rng.integers(0, dim)] = value
+            for _ in range(3):
+                v[n - drafts + rng.integers(0, drafts), 0, rng.integers(0, dim)] = value
+        ctx.cache.write(ctx.k[stream], v, ctx.slots(stream, np.arange(n)))
+    q = normal(rng, 2 * drafts, q_heads, dim)
+    for window in (0, 70):
+        got = Drafts(ctx.cache, q, [drafts] * 2, trees[0] + trees[1], ctx.table, [n, n], 0.1, window, 3).run()
+        for i in range(2):
+            want, tol = masked64(f64(q[i * drafts:(i + 1) * drafts]), f64(ctx.k[i]), f64(ctx.v[i]), 0.1, drafts_seen(n, trees[i], window, 3))
+            g = got[i * drafts:(i + 1) * drafts]
+            assert np.array_equal(np.isnan(g), np.isnan(want)) and np.array_equal(np.isinf(g), np.isinf(want))
+            inf = np.isinf(want)
+            assert np.array_equal(g[inf] > 0, want[inf] > 0)
+            within(g, want, tol)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
 def test_one_draft_is_the_token_step(dev, rng, kind, dim):
     ctx = Contexts(dev, rng, Cache, kind, 2, dim, 16, [1, 500, 37, 1300])
     q = normal(rng, 4, 8, dim)
