@@ -78,93 +78,193 @@ __device__ __forceinline__ int chain_or_depth(const PlanArgs& a, int token, int 
     return __popcll(others);
 }
 
-// Sum over this thread and those before it in the workgroup; `total` in all.
-__device__ std::int64_t scan(std::int64_t x, std::int64_t* waves, std::int64_t& total)
+constexpr int kMostThreads = 1024;
+constexpr int kTokensHere = 4096;  // tokens that the one workgroup takes too
+constexpr int kAtOnce = 4;         // pages of a thread that are on their way at once
+
+// Three sums over this thread and those before it in the workgroup, of 32, 32 and
+// 64 bits, and their totals.
+struct Sums {
+    int a, b;
+    std::int64_t c;
+};
+__device__ __forceinline__ Sums scan(int a, int b, int c, Sums (&waves)[kMostThreads / 64], Sums& total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const std::int64_t up = __shfl_up(x, o);
-        if (lane >= o) x += up;
-    }
-    __syncthreads();  // before the last scan's sums
-    if (lane == 63) waves[wave] = x;
+    Sums s{wave_scan(a), wave_scan(b), (static_cast<std::int64_t>(wave_scan(c >> 16)) << 16) + wave_scan(c & 0xffff)};
+    if (lane == 63) waves[wave] = s;
     __syncthreads();
-    std::int64_t before = 0;
-    total = 0;
+    total = {};
     for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) {
-        if (w < wave) before += waves[w];
-        total += waves[w];
+        const Sums x = waves[w];
+        if (w == wave) s.a += total.a, s.b += total.b, s.c += total.c;
+        total.a += x.a, total.b += x.b, total.c += x.c;
     }
-    return before + x;
+    return s;
 }
 
 __device__ __forceinline__ int capped(std::int64_t x) { return static_cast<int>(min(x, static_cast<std::int64_t>(INT_MAX))); }
 
-constexpr int kMostThreads = 1024;
+// The first of n ascending sums that is above x.
+__device__ __forceinline__ int above(const int* sums, int n, int x)
+{
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (sums[mid] > x) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
 
-// One workgroup, a stream a thread; more streams than threads by turns.
+// Calls take(several) for a thread's entries of n that are dealt to all threads,
+// a few at once; several(f) calls f(u, e) for each of them. What the first of its
+// calls reads is on its way for all before the next one uses it.
+template <class F>
+__device__ __forceinline__ void each_entry(int n, int threads, F&& take)
+{
+    if (n <= threads) {
+        const int e = threadIdx.x;
+        if (e < n) take([&](auto&& f) { f(0, e); });
+        return;
+    }
+    for (int e0 = threadIdx.x; e0 < n; e0 += kAtOnce * threads)
+        take([&](auto&& f) {
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (e0 + u * threads < n) f(u, e0 + u * threads);
+        });
+}
+
+// Slot and position of the i-th new token, the t-th of all, of a stream with a row of the table.
+__device__ __forceinline__ void place_token(const PlanArgs& a, int t, const std::int32_t* row, int past, int i, int drafts, bool served)
+{
+    const unsigned place = static_cast<unsigned>(past) + i, entry = place / static_cast<unsigned>(a.page);
+    const int page = served ? row[entry] : -1;
+    a.slots[t] = page < 0 ? -1 : page * a.page + static_cast<int>(place - entry * a.page);
+    if (a.positions) a.positions[t] = past + chain_or_depth(a, t, i, drafts);
+}
+
+// One workgroup, a stream a thread; more streams than threads by turns. Entries
+// that change, and tokens, are dealt to all threads by the sums before them.
 __global__ __launch_bounds__(kMostThreads) void plan_kernel(PlanArgs a)
 {
-    __shared__ std::int64_t waves[kMostThreads / 64];
+    __shared__ Sums waves[kMostThreads / 64];
+    __shared__ int upto[kMostThreads], first[3][kMostThreads], count[2][kMostThreads];
+    __shared__ int taken_here, lacking_here;
     const int tid = threadIdx.x, threads = blockDim.x;
     auto row_of = [&](int n) { return n < a.streams ? Row(a, a.past[n], a.fresh[n], a.held[n]) : Row(); };
-    const std::int64_t count = min(max(*a.free_count, 0), a.pages);
+    auto table = [&](int n) { return a.table + static_cast<std::int64_t>(n) * a.table_stride; };
+    const bool one_turn = a.streams <= threads;
+    Row r = row_of(tid);
+    const int held = min(max(*a.free_count, 0), a.pages);
+    if (tid == 0) lacking_here = 0;
 
     // Pages that go back: the first entry on top.
-    std::int64_t returned = 0;
-    for (int b = 0; b < a.streams; b += threads) {
-        std::int64_t total;
-        scan(row_of(b + tid).returned(), waves, total);
-        returned += total;
-    }
-    const std::int64_t top = min(count + returned, static_cast<std::int64_t>(a.pages));
-    std::int64_t carry = 0;
-    if (returned > 0)
-        for (int b = 0; b < a.streams; b += threads) {
-            const Row r = row_of(b + tid);
-            std::int64_t total, at = scan(r.returned(), waves, total) - r.returned() + carry;
-            carry += total;
-            std::int32_t* const row = a.table + static_cast<std::int64_t>(b + tid) * a.table_stride;
-            for (int k = 0; k < 3; ++k)
-                for (int e = 0; e < r.count[k]; ++e, ++at) {
-                    const std::int64_t to = count + returned - 1 - at;
-                    if (to < a.pages) a.free_pages[to] = row[r.first[k] + e];
-                    row[r.first[k] + e] = -1;
-                }
+    Sums total, sums = scan(r.returned(), r.need, r.fresh, waves, total);
+    std::int64_t returned = total.a;
+    if (!one_turn)
+        for (int b = threads; b < a.streams; b += threads) {
+            Sums more;
+            __syncthreads();
+            scan(row_of(b + tid).returned(), 0, 0, waves, more);
+            returned += more.a;
         }
-    __syncthreads();
+    const int top = static_cast<int>(min(held + returned, static_cast<std::int64_t>(a.pages)));
+    if (returned > 0) {
+        std::int64_t before = 0;
+        for (int b = 0; b < a.streams; b += threads) {
+            Row back = r;
+            Sums all = total, here = sums;
+            if (!one_turn) {
+                back = row_of(b + tid);
+                __syncthreads();
+                here = scan(back.returned(), 0, 0, waves, all);
+            }
+            upto[tid] = here.a;
+            for (int k = 0; k < 3; ++k) first[k][tid] = back.first[k];
+            for (int k = 0; k < 2; ++k) count[k][tid] = back.count[k];
+            __syncthreads();
+            const int here_streams = min(threads, a.streams - b);
+            each_entry(all.a, threads, [&](auto&& several) {
+                std::int32_t* entry[kAtOnce];
+                std::int32_t page[kAtOnce];
+                several([&](int u, int e) {
+                    const int i = above(upto, here_streams, e);
+                    int k = 0, at = e - (i ? upto[i - 1] : 0);
+                    if (at >= count[0][i]) at -= count[0][i], k = 1;
+                    if (k == 1 && at >= count[1][i]) at -= count[1][i], k = 2;
+                    entry[u] = table(b + i) + first[k][i] + at;
+                    page[u] = *entry[u];
+                });
+                several([&](int u, int e) {
+                    const std::int64_t to = held + returned - 1 - (before + e);
+                    if (to < a.pages) a.free_pages[to] = page[u];
+                    *entry[u] = -1;
+                });
+            });
+            before += all.a;
+        }
+    }
 
-    // Pages that are taken, and the lengths. `held` changes last: a turn reads its own streams' only.
-    std::int64_t needed = 0, tokens = 0, taken = 0;
-    int lacking = 0;
+    // Pages that are taken, the lengths, and where few the tokens. `held` changes
+    // last: a turn reads its own streams' only.
+    std::int64_t needed = 0, tokens = 0;
+    int taken = 0;
     for (int b = 0; b < a.streams; b += threads) {
         const int n = b + tid;
-        const Row r = row_of(n);
-        std::int64_t total, all_fresh, none;
-        const std::int64_t upto = scan(r.need, waves, total) + needed, until = scan(r.fresh, waves, all_fresh) + tokens;
-        const bool served = r.fits && (r.need == 0 || upto <= top);
+        __syncthreads();  // what the last turn left in LDS is read; what went back is there
+        if (!one_turn) {
+            r = row_of(n);
+            sums = scan(0, r.need, r.fresh, waves, total);
+        }
+        const std::int64_t until = needed + sums.b;
+        const bool served = r.fits && (r.need == 0 || until <= top);
         const int got = served ? r.need : 0;
+        upto[tid] = sums.b, first[0][tid] = r.back;
+        if (tid == 0) taken_here = 0;
+        __syncthreads();
+        if (got) atomicMax(&taken_here, sums.b);
+        const unsigned long long short_of = __ballot(!served);
+        if ((tid & 63) == 0 && short_of) atomicAdd(&lacking_here, __popcll(short_of));
         if (n < a.streams) {
-            std::int32_t* const row = a.table + static_cast<std::int64_t>(n) * a.table_stride;
-            for (int e = 0; e < got; ++e) {
-                const int page = a.free_pages[top - 1 - (upto - r.need + e)];
-                row[r.back + e] = page >= 0 && page < a.pages ? page : -1;
-            }
             a.lengths[n] = r.past + (served ? r.fresh : 0);
-            a.starts[n + 1] = capped(until);
+            a.starts[n + 1] = capped(tokens + sums.c);
             a.held[n] = make_int2(r.front, r.back + got);
         }
-        scan(got, waves, none);
-        taken += none;
-        scan(n < a.streams && !served, waves, none);
-        lacking += static_cast<int>(none);
-        needed += total, tokens += all_fresh;
+        __syncthreads();
+        // The streams that are served are those up to the last sum within the pool.
+        const int now = taken_here, here_streams = min(threads, a.streams - b);
+        each_entry(now, threads, [&](auto&& several) {
+            std::int32_t page[kAtOnce];
+            several([&](int u, int e) { page[u] = a.free_pages[top - 1 - needed - e]; });
+            several([&](int u, int e) {
+                const int i = above(upto, here_streams, e);
+                table(b + i)[first[0][i] + e - (i ? upto[i - 1] : 0)] = page[u] >= 0 && page[u] < a.pages ? page[u] : -1;
+            });
+        });
+        taken += now;
+        needed += total.b, tokens += total.c;
+        if (a.slots_here) {  // one turn
+            __syncthreads();
+            first[0][tid] = r.past, first[1][tid] = served, first[2][tid] = r.fresh;
+            upto[tid] = capped(sums.c);
+            __syncthreads();
+            for (int t = tid; t < a.tokens; t += threads) {
+                if (t >= total.c) {
+                    a.slots[t] = -1;
+                    if (a.positions) a.positions[t] = 0;
+                    continue;
+                }
+                const int i = above(upto, here_streams, t);
+                place_token(a, t, table(i), first[0][i], t - (i ? upto[i - 1] : 0), first[2][i], first[1][i]);
+            }
+        }
     }
     if (tid == 0) {
         a.starts[0] = 0;
-        *a.free_count = static_cast<std::int32_t>(top - taken);
-        *a.lacking = lacking;
+        *a.free_count = top - taken;
+        *a.lacking = lacking_here;
     }
 }
 
@@ -172,24 +272,13 @@ __global__ __launch_bounds__(256) void slots_kernel(PlanArgs a)
 {
     const int t = blockIdx.x * 256 + threadIdx.x;
     if (t >= a.tokens) return;
-    int slot = -1, position = 0;
-    if (t < a.starts[a.streams]) {
-        int lo = 0, hi = a.streams;  // the stream that starts at or before the token, and ends behind it
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (a.starts[mid] <= t) lo = mid;
-            else hi = mid;
-        }
-        const int past = max(a.past[lo], 0), i = t - a.starts[lo];
-        if (a.lengths[lo] > past) {
-            const unsigned place = static_cast<unsigned>(past) + i, entry = place / static_cast<unsigned>(a.page);
-            const int page = a.table[static_cast<std::int64_t>(lo) * a.table_stride + entry];
-            if (page >= 0) slot = page * a.page + static_cast<int>(place - entry * a.page);
-        }
-        position = past + chain_or_depth(a, t, i, a.starts[lo + 1] - a.starts[lo]);
+    if (t >= a.starts[a.streams]) {
+        a.slots[t] = -1;
+        if (a.positions) a.positions[t] = 0;
+        return;
     }
-    a.slots[t] = slot;
-    if (a.positions) a.positions[t] = position;
+    const int n = above(a.starts + 1, a.streams, t), start = a.starts[n], past = max(a.past[n], 0);
+    place_token(a, t, a.table + static_cast<std::int64_t>(n) * a.table_stride, past, t - start, a.starts[n + 1] - start, a.lengths[n] > past);
 }
 
 void kv_plan(const mlvc_hip_kv_plan_desc* d, hipStream_t s)
@@ -217,10 +306,13 @@ void kv_plan(const mlvc_hip_kv_plan_desc* d, hipStream_t s)
     a.free_pages = d->free_pages, a.free_count = d->free_count, a.past = d->past, a.fresh = d->fresh;
     a.seen = reinterpret_cast<const unsigned long long*>(d->seen);
     a.lengths = d->lengths, a.starts = d->starts, a.slots = d->slots, a.positions = d->positions, a.lacking = d->lacking;
-    const int threads = std::min(kMostThreads, std::max(64, (d->streams + 63) / 64 * 64));
+    // A stream a thread, and enough of them for the pages and the tokens.
+    const std::int64_t work = std::max<std::int64_t>(d->streams, d->tokens / 4);
+    const int threads = static_cast<int>(std::min<std::int64_t>(kMostThreads, std::max<std::int64_t>(64, (work + 63) / 64 * 64)));
+    a.slots_here = d->streams > 0 && d->streams <= threads && d->tokens <= kTokensHere;
     plan_kernel<<<1, threads, 0, s>>>(a);
     check(hipGetLastError(), "kv_plan launch");
-    if (d->tokens == 0) return;
+    if (d->tokens == 0 || a.slots_here) return;
     slots_kernel<<<(d->tokens + 255u) / 256u, 256, 0, s>>>(a);
     check(hipGetLastError(), "kv_plan slots launch");
 }
