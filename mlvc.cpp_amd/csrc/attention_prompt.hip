@@ -733,6 +733,13 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
     prompt_kernel<C, WINDOW><<<static_cast<unsigned>(grid), C::WAVES * 64, C::LDS, s>>>(a, tiles, by_turns);
 }
 
+// Workgroups of so many queries, at most, from what the host knows.
+std::int64_t workgroups_of(const PromptArgs& a, int queries)
+{
+    const std::int64_t by_longest = static_cast<std::int64_t>((a.longest_q + queries - 1) / queries) * a.sequences;
+    return a.q_heads * std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / queries) + a.sequences);
+}
+
 // Workgroups of 128 queries, two a CU, read each key tile once for 128 queries
 // and balance well; they need two of them for every CU. Fewer queries are
 // given more waves by key groups, at first beside as many queries, then fewer:
@@ -762,26 +769,59 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 //     8160                       172    182    178    193    215    343    326
 // 256 queries a workgroup halve the key traffic again, which pays where a
 // sequence is long enough for its last, partly seen tiles not to count.
-template <int D, bool WINDOW>
+template <int D>
 void launch_prompt(const PromptArgs& a, hipStream_t s)
 {
     const std::int64_t cus = conv::cu_count();
-    auto workgroups = [&](int queries) {  // at most, from what the host knows
-        const std::int64_t by_longest = static_cast<std::int64_t>((a.longest_q + queries - 1) / queries) * a.sequences;
-        return a.q_heads * std::min(by_longest, static_cast<std::int64_t>(a.q_tokens / queries) + a.sequences);
-    };
+    auto workgroups = [&](int queries) { return workgroups_of(a, queries); };
     if (workgroups(32) <= cus) {
-        if constexpr (D == 128) launch_prompt<PromptCfg<D, 1, 4, 32, 2>, WINDOW>(a, s);
-        else if (a.k_tokens > 512LL * a.sequences) launch_prompt<PromptCfg<64, 1, 8, 32, 2>, WINDOW>(a, s);
-        else launch_prompt<PromptCfg<64, 1, 4, 64, 2>, WINDOW>(a, s);
+        if constexpr (D == 128) launch_prompt<PromptCfg<D, 1, 4, 32, 2>, false>(a, s);
+        else if (a.k_tokens > 512LL * a.sequences) launch_prompt<PromptCfg<64, 1, 8, 32, 2>, false>(a, s);
+        else launch_prompt<PromptCfg<64, 1, 4, 64, 2>, false>(a, s);
     }
-    else if (workgroups(64) <= cus) launch_prompt<PromptCfg<D, 2, 4, D == 64 ? 64 : 32, 2>, WINDOW>(a, s);
-    else if (D == 64 && workgroups(96) <= cus) launch_prompt<PromptCfg<64, 3, 4, 64, 3>, WINDOW>(a, s);
-    else if (D == 64 && workgroups(128) <= cus) launch_prompt<PromptCfg<64, 4, 3, 64, 3>, WINDOW>(a, s);
-    else if (workgroups(128) <= 2 * cus) launch_prompt<PromptCfg<D, 4, 2, 64, 2>, WINDOW>(a, s);
+    else if (workgroups(64) <= cus) launch_prompt<PromptCfg<D, 2, 4, D == 64 ? 64 : 32, 2>, false>(a, s);
+    else if (D == 64 && workgroups(96) <= cus) launch_prompt<PromptCfg<64, 3, 4, 64, 3>, false>(a, s);
+    else if (D == 64 && workgroups(128) <= cus) launch_prompt<PromptCfg<64, 4, 3, 64, 3>, false>(a, s);
+    else if (workgroups(128) <= 2 * cus) launch_prompt<PromptCfg<D, 4, 2, 64, 2>, false>(a, s);
     else if (D == 128 && a.longest_q >= 4096 && workgroups(128) >= 4 * cus && static_cast<std::int64_t>(a.longest_q) * a.sequences <= 2 * static_cast<std::int64_t>(a.q_tokens))
-        launch_prompt<PromptCfg<128, 8, 1, 64, 2>, WINDOW>(a, s);
-    else launch_prompt<PromptCfg<D, 4, 1, 64, D == 64 ? 3 : 2>, WINDOW>(a, s);
+        launch_prompt<PromptCfg<128, 8, 1, 64, 2>, false>(a, s);
+    else launch_prompt<PromptCfg<D, 4, 1, 64, D == 64 ? 3 : 2>, false>(a, s);
+}
+
+// Under a window a workgroup's keys are few and as many in each, so that 256
+// queries gain nothing, and key groups less: two beside 64 queries while those
+// workgroups fit the GPU at once, four beside 32 or 64 while they fit the CUs.
+// us, a window of w (16 query heads, 4 sinks, causal):
+//   heads of 128              (1,4,32) (2,4,32) (2,2,32) (4,2,64) (4,1,64) (8,1,64)
+//     10 on 1500, w 700         12.1     13.3     14.9     17.6     21.6     24.8
+//     240, w 80                  9.2     10.7     10.0     12.6     13.3     16.0
+//     920, w 256                19.9     13.0     12.6     17.0     18.4     27.8
+//     2040, w 512               45.6     29.7     21.0     21.8     24.5     34.4
+//     8160, w 64                 110     81.1     46.0     54.1     37.8     46.2
+//     8160, w 1024               237      144      104      110     94.2      103
+//     8160, w 4080               490      299      252      237      229      252
+//     32640, w 1024              998      588      433      437      371      414
+//   heads of 64               (1,4,64) (1,4,32) (2,4,64) (2,2,32) (4,2,64) (4,1,64)
+//     240, w 80                  6.3      6.6      7.4      7.7      9.1     10.4
+//     10 on 1500, w 700         10.0      8.4     10.9     11.5     13.4     16.1
+//     920, w 300                15.4      8.5      9.8     10.6     12.5     15.6
+//     700 and 600, w 100 both ways
+//                               21.1     14.5     16.0     10.6     11.7     14.5
+//     2040, w 300               29.6     15.6     18.6     12.9     12.9     15.9
+//     1..2040 packed, w 240 both ways
+//                               99.4     53.9     61.1     31.3     38.8     30.1
+//     8160, w 500                133     68.8     78.0     39.8     57.3     41.4
+template <int D>
+void launch_window(const PromptArgs& a, hipStream_t s)
+{
+    const std::int64_t cus = conv::cu_count(), by_64 = workgroups_of(a, 64);
+    if (workgroups_of(a, 32) <= (D == 64 ? 2 : 1) * cus) {
+        if (D == 64 && a.window <= (a.causal ? 256 : 128)) launch_prompt<PromptCfg<64, 1, 4, 64, 2>, true>(a, s);
+        else launch_prompt<PromptCfg<D, 1, 4, 32, 2>, true>(a, s);
+    }
+    else if (D == 128 && by_64 <= cus) launch_prompt<PromptCfg<128, 2, 4, 32, 2>, true>(a, s);
+    else if (by_64 <= 2 * cus) launch_prompt<PromptCfg<D, 2, 2, 32, 2>, true>(a, s);
+    else launch_prompt<PromptCfg<D, 4, 1, 64, D == 64 ? 3 : 2>, true>(a, s);
 }
 
 void attention_prompt(const mlvc_hip_attention_prompt_desc* d, int window, int sinks, const char* op, hipStream_t s)
@@ -822,8 +862,8 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, int window, int s
                       vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f;
     // The kernel under a window counts places in 32 bits.
     const bool fast = rows && (!a.window || static_cast<std::int64_t>(d->q_tokens) + d->k_tokens < (std::int64_t{1} << 30));
-    if (fast && d->head_dim == 128) a.window ? launch_prompt<128, true>(a, s) : launch_prompt<128, false>(a, s);
-    else if (fast && d->head_dim == 64) a.window ? launch_prompt<64, true>(a, s) : launch_prompt<64, false>(a, s);
+    if (fast && d->head_dim == 128) a.window ? launch_window<128>(a, s) : launch_prompt<128>(a, s);
+    else if (fast && d->head_dim == 64) a.window ? launch_window<64>(a, s) : launch_prompt<64>(a, s);
     else {
         require(launchable(d->q_tokens, 64), op, "too many sequences, heads and queries in one call");
         prompt_any_kernel<<<dim3(static_cast<unsigned>(d->q_tokens), static_cast<unsigned>(d->q_heads)), 64, 0, s>>>(a);
