@@ -38,6 +38,9 @@ struct DraftArgs {
     bool spare;     // small shares behind the large ones
 };
 
+// The first place that a token at `place` sees under a window.
+__device__ __forceinline__ int first_seen(int place, int window) { return place >= window ? place - window + 1 : 0; }
+
 // A stream's context. Its steps: those that hold sinks, then those from the
 // window's first token on.
 struct View {
@@ -54,7 +57,7 @@ struct View {
         tokens = max(tokens, 0);
         past = tokens - drafts;
         length = static_cast<int>(min(static_cast<std::int64_t>(min(tokens, a.longest)), held));
-        const int first = a.window ? max(past - a.window + 1, 0) / kStep : 0;
+        const int first = a.window ? first_seen(past, a.window) / kStep : 0;
         sinks = a.window ? min(a.sinks, length) : 0;
         sink_steps = (sinks + kStep - 1) / kStep;
         const int all = (length + kStep - 1) / kStep;
@@ -115,7 +118,7 @@ __global__ __launch_bounds__(64) void drafts_any_kernel(DraftArgs a)
         const unsigned long long mine = mask_of(a, w, lane), mask = __shfl(mine, draft);
         const int depth = depth_of(mine, lane), depth_i = __shfl(depth, draft);
         sight.past = w.past;
-        sight.from = a.window ? max(w.past + depth_i - a.window + 1, 0) : 0;
+        sight.from = a.window ? first_seen(w.past + depth_i, a.window) : 0;
         sight.sinks = w.sinks;
         sight.drafts = mask & __ballot(!a.window || depth_i - depth < a.window || w.past + depth < a.sinks);
     }
@@ -386,7 +389,7 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
         const int depth = depth_of(mask, lane);
         Sight s;
         s.past = w.past, s.sinks = w.sinks;
-        s.from = a.window ? max(w.past + depth - a.window + 1, 0) : 0;
+        s.from = a.window ? first_seen(w.past + depth, a.window) : 0;
         s.drafts = mask;
         if (a.window && a.window < kMostDrafts)
             for (int e = 0; e < kMostDrafts; ++e) {
@@ -654,7 +657,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
         const int depth = depth_of(mask, lane);
         Sight s;
         s.past = w.past, s.sinks = w.sinks;
-        s.from = a.window ? max(w.past + depth - a.window + 1, 0) : 0;
+        s.from = a.window ? first_seen(w.past + depth, a.window) : 0;
         s.drafts = mask;
         if (a.window && a.window < kMostDrafts)
             for (int e = 0; e < kMostDrafts; ++e) {
@@ -912,20 +915,20 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void drafts_kernel(DraftArgs
     }
 }
 
-// Puts the parts of ROWS rows of a stream and key head together: LANES threads
-// hold a part's row, four values each, and GROUPS of them take every GROUPS-th
-// part, each with a base of its own; they are put together in LDS.
+// Puts the parts of a stream's and key head's rows together, ROWS at a time:
+// LANES threads hold a part's row, four values each, and GROUPS of them take every
+// GROUPS-th part, each with a base of its own; they are put together in LDS.
+// `turns` workgroups take a stream's and key head's rows by turns.
 template <int LANES, int ROWS, int GROUPS>
-__global__ __launch_bounds__(LANES* ROWS* GROUPS) void drafts_join_kernel(DraftArgs a, int row_blocks)
+__global__ __launch_bounds__(LANES* ROWS* GROUPS) void drafts_join_kernel(DraftArgs a, int turns)
 {
     __shared__ floatx4 sums[GROUPS][ROWS][LANES];
     __shared__ float2 states[GROUPS][ROWS];
     constexpr float kBase0 = -3.402823466e38f;
-    const int lane = threadIdx.x & 63, row_block = blockIdx.x % row_blocks, rest = blockIdx.x / row_blocks, head = rest % a.heads, stream = rest / a.heads;
-    const int at = threadIdx.x % LANES, r = threadIdx.x / LANES % ROWS, group = threadIdx.x / (LANES * ROWS);
+    const int lane = threadIdx.x & 63, rest = blockIdx.x / turns, head = rest % a.heads, stream = rest / a.heads;
+    const int at = threadIdx.x % LANES, r = threadIdx.x / LANES % ROWS, group = threadIdx.x / (LANES * ROWS), d = at * 4;
     const View w(a, stream);
-    const int row = row_block * ROWS + r, rows = w.queries * a.group;
-    if (row_block * ROWS >= rows) return;
+    const int rows = w.queries * a.group;
     int total = 0, start = 0;
     for (int b = 0; b < a.streams; b += 64) {
         const int mine = b + lane < a.streams ? View(a, b + lane).steps : 0;
@@ -936,11 +939,11 @@ __global__ __launch_bounds__(LANES* ROWS* GROUPS) void drafts_join_kernel(DraftA
     const Shares shares(a.shares, total, a.spare);
     const int first = w.steps ? shares.holder(start) : 0, parts = w.steps ? shares.holder(start + w.steps - 1) - first + 1 : 0;
     if (parts == 1) return;  // written by the share that holds it
-    const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + row) * a.places + first + stream;
-    const int d = at * 4;
-    float base = kBase0, l = 0.0f;
-    floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (row < rows) {
+    for (int row0 = blockIdx.x % turns * ROWS; row0 < rows; row0 += turns * ROWS) {
+        const int row = min(row0 + r, rows - 1);
+        const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + row) * a.places + first + stream;
+        float base = kBase0, l = 0.0f;
+        floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int i = group; i < parts; i += GROUPS) {
             const floatx4 v = *reinterpret_cast<const floatx4*>(a.part + (slot + i) * a.dim + d);
@@ -951,39 +954,43 @@ __global__ __launch_bounds__(LANES* ROWS* GROUPS) void drafts_join_kernel(DraftA
 #pragma unroll
             for (int c = 0; c < 4; ++c) sum[c] = sum[c] * old + v[c] * f;
         }
-    }
-    sums[group][r][at] = sum;
-    if (at == 0) states[group][r] = make_float2(base, l);
-    __syncthreads();
-    if (group != 0 || row >= rows) return;
-    float top = kBase0;
+        if constexpr (GROUPS > 1) {
+            __syncthreads();  // the last rows' sums are read
+            sums[group][r][at] = sum;
+            if (at == 0) states[group][r] = make_float2(base, l);
+            __syncthreads();
+            if (group != 0) continue;
+            float top = kBase0;
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, states[i][r].x);
-    l = 0.0f;
-    sum = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, states[i][r].x);
+            l = 0.0f;
+            sum = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) {
-        const float2 st = states[i][r];
-        const float f = __builtin_amdgcn_exp2f(st.x - top);
-        l += st.y * f;
+            for (int i = 0; i < GROUPS; ++i) {
+                const float2 st = states[i][r];
+                const float f = __builtin_amdgcn_exp2f(st.x - top);
+                l += st.y * f;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sum[c] = fmaf(sums[i][r][at][c], f, sum[c]);
-    }
-    // A part that is infinite, with however small a weight.
-    if (!is_finite(sum[0]) || !is_finite(sum[1]) || !is_finite(sum[2]) || !is_finite(sum[3])) {
-        floatx4 odd = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i = 0; i < parts; ++i) {
-            const floatx4 v = *reinterpret_cast<const floatx4*>(a.part + (slot + i) * a.dim + d);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) odd[c] += is_finite(v[c]) ? 0.0f : v[c];
+                for (int c = 0; c < 4; ++c) sum[c] = fmaf(sums[i][r][at][c], f, sum[c]);
+            }
         }
+        // A part that is infinite, with however small a weight.
+        if (!is_finite(sum[0]) || !is_finite(sum[1]) || !is_finite(sum[2]) || !is_finite(sum[3])) {
+            floatx4 odd = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < parts; ++i) {
+                const floatx4 v = *reinterpret_cast<const floatx4*>(a.part + (slot + i) * a.dim + d);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sum[c] = is_finite(sum[c]) ? sum[c] : odd[c];
+                for (int c = 0; c < 4; ++c) odd[c] += is_finite(v[c]) ? 0.0f : v[c];
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] = is_finite(sum[c]) ? sum[c] : odd[c];
+        }
+        if (row0 + r >= rows) continue;
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        const int of = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(a.group));
+        *reinterpret_cast<uint2*>(a.out + (w.start + of) * a.out_stride + static_cast<std::int64_t>(head * a.group + row - of * a.group) * a.dim + d) =
+            make_uint2(pack_rounded(sum[0] * f, sum[1] * f), pack_rounded(sum[2] * f, sum[3] * f));
     }
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    const int of = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(a.group));
-    *reinterpret_cast<uint2*>(a.out + (w.start + of) * a.out_stride + static_cast<std::int64_t>(head * a.group + row - of * a.group) * a.dim + d) =
-        make_uint2(pack_rounded(sum[0] * f, sum[1] * f), pack_rounded(sum[2] * f, sum[3] * f));
 }
 
 void check_desc(const mlvc_hip_attention_drafts_desc* d, const char* op)
@@ -1107,14 +1114,15 @@ void launch_drafts(const DraftArgs& a, const Plan& p, bool fast, unsigned grid, 
 template <int LANES>
 void launch_join(const DraftArgs& a, hipStream_t s)
 {
-    // A row for 256 threads where there are few, eight rows where there are many.
+    // A row for 256 threads where there are few; else eight at a time, by no more
+    // workgroups than find where the parts lie in one turn of the GPU.
     const int rows = a.longest_q * a.group;
-    const std::int64_t all = static_cast<std::int64_t>(rows) * a.heads * a.streams;
-    if (all > 4096) {
-        const int blocks = (rows + 7) / 8;
-        drafts_join_kernel<LANES, 8, 1><<<static_cast<unsigned>(static_cast<std::int64_t>(blocks) * a.heads * a.streams), LANES * 8, 0, s>>>(a, blocks);
+    const std::int64_t of_head = static_cast<std::int64_t>(a.heads) * a.streams;
+    if (rows * of_head > 4096) {
+        const int turns = static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>((rows + 7) / 8, 8 * conv::cu_count() / of_head)));
+        drafts_join_kernel<LANES, 8, 1><<<static_cast<unsigned>(turns * of_head), LANES * 8, 0, s>>>(a, turns);
     } else {
-        drafts_join_kernel<LANES, 1, 256 / LANES><<<static_cast<unsigned>(all), 256, 0, s>>>(a, rows);
+        drafts_join_kernel<LANES, 1, 256 / LANES><<<static_cast<unsigned>(rows * of_head), 256, 0, s>>>(a, rows);
     }
     check(hipGetLastError(), "attention_drafts join launch");
 }

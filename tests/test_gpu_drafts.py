@@ -268,6 +268,17 @@ def test_window_strides_past_32_bits(dev, rng):
     within(Window(p, 9, 2).run(), want, tol)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 40])
+@pytest.mark.parametrize("causal", [False, True])
+def test_window_of_all_sinks_is_the_prompt(dev, rng, dim, causal):
+    """Sinks that reach to the last key."""
+    q, k, v = normal(rng, 150, 2, dim), normal(rng, 200, 1, dim), normal(rng, 200, 1, dim)
+    p = Prompt(dev, q, k, v, [150], [200], causal, 0.1)
+    for sinks in (200, 2 ** 31 - 1):
+        want, tol = masked64(f64(q), f64(k), f64(v), 0.1, window_seen(150, 200, causal, 0, 0))
+        within(Window(p, 1, sinks).run(), want, tol)
+
+
 def test_window_of_none_is_the_prompt(dev, rng):
     q, k, v = (normal(rng, 300, 2, 64) for _ in range(3))
     for causal in (False, True):
@@ -500,6 +511,19 @@ def test_drafts_unseen_places_do_not_reach(dev, rng, kind, dim, window):
         within(got[at:at + count][clean], want[clean], tol[clean], f"stream {i}")
         assert np.isnan(got[at:at + count][~clean]).all()  # those that see it
         at += count
+
+
+@pytest.mark.parametrize("dim", [64, 128, 40])
+def test_drafts_of_the_widest_window(dev, rng, dim):
+    """A window and sinks of 2^31 - 1, more drafts than tokens among the streams: nothing is cut."""
+    counts, lengths = [5, 9, 20], [300, 4, 40]
+    ctx = Contexts(dev, rng, Cache, KV_INT8, 1, dim, 16, lengths)
+    q = normal(rng, sum(counts), 4, dim)
+    masks = [m for n in counts for m in tree(rng, n)]
+    got = [Drafts(ctx.cache, q, counts, masks, ctx.table, lengths, 0.1, *w).run().view(np.uint16)
+           for w in ((0, 0), (2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1))]
+    for g in got[1:]:
+        assert np.array_equal(g, got[0])
 
 
 @pytest.mark.parametrize("kind", KINDS)
