@@ -1009,6 +1009,17 @@ void check_desc(const mlvc_hip_attention_drafts_desc* d, const char* op)
 enum Shape { kOne8, kOne4, kTwo4, kTile21, kTile22, kTile41, kTile42 };
 constexpr int kRows[] = {16, 16, 32, 64, 64, 128, 128}, kPerCu[] = {1, 3, 2, 4, 2, 2, 1};
 
+// Parts of a call for each CU, at most: those of its workgroups' rows, twice where
+// there are small shares behind the large ones.
+constexpr int kParts = 256;
+constexpr bool enough_parts()
+{
+    for (int i = kOne8; i <= kTile42; ++i)
+        if (kRows[i] * kPerCu[i] * (i == kOne4 ? 2 : 1) > kParts) return false;
+    return true;
+}
+static_assert(enough_parts());
+
 // How a call is laid out; from what the host knows.
 struct Plan {
     Shape shape;
@@ -1068,7 +1079,7 @@ Plan plan(const mlvc_hip_attention_drafts_desc* d)
     // Parts: each share leaves one a row, and one for each context that begins in
     // it. Asked for whether this call cuts or not and for the shape that leaves the
     // most, so that what is enough for a batch is enough for a smaller one.
-    const size_t slots = 256 * static_cast<size_t>(cus) + (d->streams + 2) * static_cast<size_t>(p.row_count);
+    const size_t slots = kParts * static_cast<size_t>(cus) + (d->streams + 2) * static_cast<size_t>(p.row_count);
     p.part_bytes = slots * c->head_dim * sizeof(float);
     p.bytes = p.part_bytes + slots * sizeof(float2);
     const std::int64_t whole = workgroups(p.shape);
