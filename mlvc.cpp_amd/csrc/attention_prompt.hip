@@ -362,7 +362,11 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     const int any = w0 >= nq ? 0 : a.causal ? max(0, min(sk.count, behind + min(w0 + 32, nq))) : sk.count;
     // Under a window: keys that any of this wave's queries sees, and those of this lane's.
     const Sight of_wave(a, behind + w0, behind + min(w0 + 32, nq) - 1, sk.count), of_lane(a, behind + at_query, behind + at_query, sk.count);
-    auto lane_sees = [&](int j) { return static_cast<unsigned>(j - of_lane.from) < static_cast<unsigned>(of_lane.to - of_lane.from) || j < of_lane.sinks; };
+    // Of 32 keys from j on, one a bit.
+    auto lane_sees = [&](int j) {
+        auto below = [&](int end) { return end <= j ? 0u : end - j >= 32 ? ~0u : (1u << (end - j)) - 1; };
+        return (below(of_lane.to) & ~below(of_lane.from)) | below(of_lane.sinks);
+    };
 
     const std::int64_t kv = static_cast<std::int64_t>(head / a.group) * D;
     const std::uint16_t* const k0 = a.k + sk.first * a.k_stride + kv;
@@ -443,12 +447,18 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
         {
             if constexpr (MASKED) {
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
+                for (int tt = 0; tt < TT; ++tt) {
+                    // A bit spread over a word chooses between a score's bits and those of
+                    // -inf: two operations a score, four for its place against three ends.
+                    const unsigned see = WINDOW ? lane_sees(j0 + tt * 32) >> 4 * hi : 0u;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int j = j0 + tt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3);
-                        if (WINDOW ? !lane_sees(j) : j >= seen) s[tt][r] = -INFINITY;
+                        if constexpr (WINDOW) {
+                            const unsigned all = __builtin_amdgcn_sbfe(see, 8 * (r >> 2) + (r & 3), 1);
+                            s[tt][r] = __uint_as_float((__float_as_uint(s[tt][r]) & all) | (0xff800000u & ~all));
+                        } else if (j0 + tt * 32 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen) s[tt][r] = -INFINITY;
                     }
+                }
             }
             // The NaN-propagating maximum of three is one instruction; a score that
             // is NaN leaves the maximum where it was, and its query becomes NaN.
