@@ -588,7 +588,7 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
 // holds 32 rows as columns of S^T = K Q^T (32x32x16 products, keys as rows), so
 // that a lane's scores all belong to one row, and rounded to halves they are the
 // B operand of O^T += V^T P^T as they stand. 16-byte pieces of a row are permuted
-// in LDS (piece ^ f(row)) against bank conflicts; V is read transposing.
+// in LDS against bank conflicts; V is read transposing.
 template <int KIND_, int D_, int RG_, int KG_>
 struct TileCfg {
     static constexpr int KIND = KIND_, D = D_, RG = RG_, KG = KG_, WAVES = RG * KG, ROWS = RG * 32, OCC = 2;
@@ -601,9 +601,16 @@ struct TileCfg {
     static constexpr size_t TILES = KG * 2 * 2 * TILE * 2, SCALES = KG * 2 * 2 * kStep * sizeof(float),
                             JOINT = static_cast<size_t>(KG - 1) * WORDS * RG * 64 * 16;
     static constexpr size_t LDS = TILES + SCALES > JOINT ? TILES + SCALES : JOINT;
-    __host__ __device__ static constexpr int swizzle(int t)
+    // Place of a 16-byte piece of row t, so that 16 rows of one piece (a K read) fall
+    // on all 64 banks, 4 rows of 4 pieces (a V read) do too, and the pieces that
+    // eight lanes write at once on 32 of them: every one of a row of halves, every
+    // other one of unpacked bytes (in the order of the pieces those took 10% of the
+    // cycles at 64 streams of 16 drafts).
+    __host__ __device__ static constexpr int place(int piece, int t)
     {
-        return D == 128 ? 4 * (t & 3) + (t >> 2 & 3) : 4 * (t >> 1 & 1) + (t >> 2 & 3);
+        if (BYTES == 2) return piece ^ (D == 128 ? 4 * (t & 3) + (t >> 2 & 3) : 4 * (t >> 1 & 1) + (t >> 2 & 3));
+        const int evens_first = (piece >> 1) + (piece & 1) * (D / 16);
+        return evens_first ^ (D == 128 ? 2 * (t & 3) + (t >> 2 & 1) + 8 * (t >> 3 & 1) : 2 * (t >> 1 & 1) + (t >> 2 & 1) + 4 * ((t >> 3 ^ t) & 1));
     }
 };
 
@@ -684,13 +691,13 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
     // + 0..3 of a 16-row step) a lane and returns one column's four.
     int kat[KS], vat[DT][2];
 #pragma unroll
-    for (int i = 0; i < KS; ++i) kat[i] = column * D + ((2 * i + hi) ^ C::swizzle(column)) * 8;
+    for (int i = 0; i < KS; ++i) kat[i] = column * D + C::place(2 * i + hi, column) * 8;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int r = 8 * e + 4 * hi + ((lane & 15) >> 2);
-            vat[dt][e] = r * D + ((4 * dt + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ C::swizzle(r)) * 8 + (lane & 1) * 4;
+            vat[dt][e] = r * D + C::place(4 * dt + 2 * (lane >> 4 & 1) + (lane >> 1 & 1), r) * 8 + (lane & 1) * 4;
         }
     floatx16 acc[DT];
 #pragma unroll
@@ -723,7 +730,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
                         x[e] = gone ? 0u : x[e] & ~odd;
                     }
                 }
-                *reinterpret_cast<u32x4*>(to + (at ^ C::swizzle(r)) * 8) = x;
+                *reinterpret_cast<u32x4*>(to + C::place(at, r) * 8) = x;
             };
             if constexpr (KIND == MLVC_KV_F16) {
                 put(piece, c.raw[i]);
