@@ -534,7 +534,12 @@ int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip
  *
  * Window and sinks, in all of them: a token at place p sees a token at place j
  * if p - j < window (and j - p < window, where it sees later ones at all) or
- * j < sinks. Window 0: no window. */
+ * j < sinks. Window 0: no window.
+ *
+ * As above, 16-byte aligned rows of heads of 64 or 128 run the fast attention
+ * kernels; others take plain ones, one wave a draft and head, on long contexts
+ * slower than a matrix product of a library. Nothing here allocates, waits or
+ * reads device memory on the host, so a step can be captured into a graph. */
 
 /* Page tables, slots and positions of a step, from the streams' lengths on the
  * device. Stream n has `past[n]` tokens in the cache and gets fresh[n] more, or

@@ -6,6 +6,15 @@
 // V(i) holds the context's places j with place_i - j < window or j < sinks, and
 // the drafts of i's mask, at places past + depth, by the same rule. depth is the
 // number of other drafts that a draft sees.
+//
+// Bound by the bytes of the cache while a key head has few rows (drafts times the
+// query heads that share it): 64 streams of one token under a window of 4080, 32
+// query heads on 8 of 128, E4M3, 0.51 GB in 111 us or 4.6 TB/s. From 64 rows on
+// by what is computed for a cached row, its unpacking and the softmax: 64 streams
+// of 16 drafts on up to 8160 tokens, INT8, 0.55 GB and 69 GFLOP in 170 us, vector
+// units busy 50% of the time and matrix cores 20%, the rest waits for LDS and for
+// products that follow from each other; 64 of 64 drafts 275 GFLOP in 462 us. One
+// token under a window of 920 is a launch and the latency of four steps, 9.0 us.
 
 #include "attention_cache.hpp"
 
@@ -102,87 +111,6 @@ __device__ __forceinline__ std::int64_t token_row(const DraftArgs& a, int stream
     return page < 0 || page >= a.pages ? -1 : (static_cast<std::int64_t>(page) * a.heads + head) * a.page + j % a.page;
 }
 
-// Any head size: one wave for a draft and a query head, 64 tokens at a time,
-// one token a lane for the scores and one value column a lane for the sum.
-template <int KIND>
-__global__ __launch_bounds__(64) void drafts_any_kernel(DraftArgs a)
-{
-    __shared__ float qs[kMaxHeadDim], ps[64];
-    __shared__ long long at[64];
-    const int lane = threadIdx.x, head = blockIdx.x % a.q_heads, rest = blockIdx.x / a.q_heads;
-    const int draft = rest % a.longest_q, stream = rest / a.longest_q;
-    const View w(a, stream);
-    if (draft >= w.queries) return;
-    Sight sight;
-    {
-        const unsigned long long mine = mask_of(a, w, lane), mask = __shfl(mine, draft);
-        const int depth = depth_of(mine, lane), depth_i = __shfl(depth, draft);
-        sight.past = w.past;
-        sight.from = a.window ? first_seen(w.past + depth_i, a.window) : 0;
-        sight.sinks = w.sinks;
-        sight.drafts = mask & __ballot(!a.window || depth_i - depth < a.window || w.past + depth < a.sinks);
-    }
-    constexpr int kColumns = kMaxHeadDim / 64;
-    auto value = [&](const std::uint8_t* x, long long row, int d) {
-        if constexpr (KIND == MLVC_KV_F16) return h2f(reinterpret_cast<const std::uint16_t*>(x)[row * a.dim + d]);
-        else return from_byte(KIND, x[row * a.dim + d]);
-    };
-    const std::int64_t token = w.start + draft;
-    const std::uint16_t* q = a.q + token * a.q_stride + static_cast<std::int64_t>(head) * a.dim;
-    for (int d = lane; d < a.dim; d += 64) qs[d] = h2f(q[d]) * a.scale2;
-    __syncthreads();
-    float acc[kColumns] = {}, m = -INFINITY, l = 0.0f;
-    for (int step = 0; step < w.steps; step += 2) {
-        const int mine = step + lane / kStep, j = mine < w.steps ? w.token(mine) + lane % kStep : w.length;
-        const long long row = j < w.length && sight(j) ? token_row(a, stream, head / a.group, j) : -1;
-        float s = -INFINITY;
-        if (row >= 0) {
-            s = 0.0f;
-            for (int d = 0; d < a.dim; ++d) s = fmaf(qs[d], value(a.k, row, d), s);
-            if constexpr (KIND != MLVC_KV_F16) s *= a.k_scale[row];
-        }
-        const float top = fmaxf(m, group_max<64>(s)), base = top == -INFINITY ? 0.0f : top;
-        float p = __builtin_amdgcn_exp2f(s - base);
-        const float keep = __builtin_amdgcn_exp2f(m - base);
-        m = top;
-        l = l * keep + group_sum<64>(p);
-        if constexpr (KIND != MLVC_KV_F16) p = row < 0 ? 0.0f : p * a.v_scale[row];
-        ps[lane] = p;
-        at[lane] = row;
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c) {
-            const int d = c * 64 + lane;
-            if (d >= a.dim) break;
-            float sum = acc[c] * keep;
-            for (int i = 0; i < 64; ++i)
-                if (at[i] >= 0) sum = fmaf(ps[i], value(a.v, at[i], d), sum);
-            acc[c] = sum;
-        }
-        __syncthreads();
-    }
-    if constexpr (KIND == MLVC_KV_F16) {
-        for (int c = 0; c < kColumns; ++c) {
-            const int d = c * 64 + lane;
-            if (d >= a.dim || is_finite(acc[c])) continue;
-            OddValues odd;
-            for (int step = 0; step < w.steps; ++step)
-                for (int j = w.token(step), i = 0; i < kStep && j < w.length; ++i, ++j) {
-                    const std::int64_t row = sight(j) ? token_row(a, stream, head / a.group, j) : -1;
-                    if (row >= 0) odd.add(reinterpret_cast<const std::uint16_t*>(a.v)[row * a.dim + d]);
-                }
-            acc[c] = odd.sum(acc[c]);
-        }
-    }
-    const float r = l == 0.0f ? 0.0f : 1.0f / l;
-    std::uint16_t* out = a.out + token * a.out_stride + static_cast<std::int64_t>(head) * a.dim;
-#pragma unroll
-    for (int c = 0; c < kColumns; ++c)
-        if (c * 64 + lane < a.dim) out[c * 64 + lane] = f2h(opaque(acc[c] * r));
-}
-
-// ------------------------------------------------------------ matrix cores
-
 // Calls fn(stream, first, last, whole, place) for each piece of a context, steps
 // [first, last), that workgroup `share` of a key head and block of rows takes;
 // place: the piece's among a row's parts, when it is not the whole context.
@@ -235,6 +163,103 @@ __device__ __forceinline__ void decide_odd(const DraftArgs& a, const View& w, co
     for (int r = 0; r < 4; ++r) sums[r] = odd[r].sum(sums[r]);
 }
 
+// Any head size: one wave for a piece of a context and a draft's query head, 64
+// tokens at a time, one token a lane for the scores and one value column a lane
+// for the sum.
+template <int KIND>
+__global__ __launch_bounds__(64) void drafts_any_kernel(DraftArgs a)
+{
+    __shared__ float qs[kMaxHeadDim], ps[64];
+    __shared__ long long at[64];
+    const int rows = a.longest_q * a.group, row_of_head = blockIdx.x % rows, draft = row_of_head / a.group;
+    const int lane = threadIdx.x, rest = blockIdx.x / rows, kv_head = rest % a.heads, head = kv_head * a.group + row_of_head - draft * a.group;
+    constexpr int kColumns = kMaxHeadDim / 64;
+    constexpr float kBase0 = -3.402823466e38f;
+    auto value = [&](const std::uint8_t* x, long long row, int d) {
+        if constexpr (KIND == MLVC_KV_F16) return h2f(reinterpret_cast<const std::uint16_t*>(x)[row * a.dim + d]);
+        else return from_byte(KIND, x[row * a.dim + d]);
+    };
+    auto piece = [&](int stream, int first, int last, bool whole, int place) {
+        const View w(a, stream);
+        if (draft >= w.queries) return;
+        Sight sight;
+        {
+            const unsigned long long mine = mask_of(a, w, lane), mask = __shfl(mine, draft);
+            const int depth = depth_of(mine, lane), depth_i = __shfl(depth, draft);
+            sight.past = w.past;
+            sight.from = a.window ? first_seen(w.past + depth_i, a.window) : 0;
+            sight.sinks = w.sinks;
+            sight.drafts = mask & __ballot(!a.window || depth_i - depth < a.window || w.past + depth < a.sinks);
+        }
+        const std::int64_t token = w.start + draft;
+        const std::uint16_t* q = a.q + token * a.q_stride + static_cast<std::int64_t>(head) * a.dim;
+        for (int d = lane; d < a.dim; d += 64) qs[d] = h2f(q[d]) * a.scale2;
+        __syncthreads();
+        float acc[kColumns] = {}, m = -INFINITY, l = 0.0f;
+        for (int step = first; step < last; step += 2) {
+            const int mine = step + lane / kStep, j = mine < last ? w.token(mine) + lane % kStep : w.length;
+            const long long row = j < w.length && sight(j) ? token_row(a, stream, kv_head, j) : -1;
+            float s = -INFINITY;
+            if (row >= 0) {
+                s = 0.0f;
+                for (int d = 0; d < a.dim; ++d) s = fmaf(qs[d], value(a.k, row, d), s);
+                if constexpr (KIND != MLVC_KV_F16) s *= a.k_scale[row];
+            }
+            const float top = fmaxf(m, group_max<64>(s)), base = top == -INFINITY ? 0.0f : top;
+            float p = __builtin_amdgcn_exp2f(s - base);
+            const float keep = __builtin_amdgcn_exp2f(m - base);
+            m = top;
+            l = l * keep + group_sum<64>(p);
+            if constexpr (KIND != MLVC_KV_F16) p = row < 0 ? 0.0f : p * a.v_scale[row];
+            ps[lane] = p;
+            at[lane] = row;
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c) {
+                const int d = c * 64 + lane;
+                if (d >= a.dim) break;
+                float sum = acc[c] * keep;
+                for (int i = 0; i < 64; ++i)
+                    if (at[i] >= 0) sum = fmaf(ps[i], value(a.v, at[i], d), sum);
+                acc[c] = sum;
+            }
+            __syncthreads();
+        }
+        if constexpr (KIND == MLVC_KV_F16) {
+            for (int c = 0; c < kColumns; ++c) {
+                const int d = c * 64 + lane;
+                if (d >= a.dim || is_finite(acc[c])) continue;
+                OddValues odd;
+                for (int step = first; step < last; ++step)
+                    for (int j = w.token(step), i = 0; i < kStep && j < w.length; ++i, ++j) {
+                        const std::int64_t row = sight(j) ? token_row(a, stream, kv_head, j) : -1;
+                        if (row >= 0) odd.add(reinterpret_cast<const std::uint16_t*>(a.v)[row * a.dim + d]);
+                    }
+                acc[c] = odd.sum(acc[c]);
+            }
+        }
+        if (whole) {
+            const float r = l == 0.0f ? 0.0f : 1.0f / l;
+            std::uint16_t* out = a.out + token * a.out_stride + static_cast<std::int64_t>(head) * a.dim;
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c)
+                if (c * 64 + lane < a.dim) out[c * 64 + lane] = f2h(opaque(acc[c] * r));
+            return;
+        }
+        const std::int64_t slot = (static_cast<std::int64_t>(kv_head) * rows + row_of_head) * a.places + place;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c)
+            if (c * 64 + lane < a.dim) a.part[slot * a.dim + c * 64 + lane] = acc[c];
+        if (lane == 0) a.state[slot] = make_float2(m == -INFINITY ? kBase0 : m, l);
+        __syncthreads();  // before the next piece's query
+    };
+    const int item = rest / a.heads;
+    if (a.shares) each_piece(a, item, piece);
+    else piece(item, 0, View(a, item).steps, true, 0);
+}
+
+// ------------------------------------------------------------ matrix cores
+
 // Rows of the cache of a stream's tiles of 16 tokens (each in one page), those of
 // 64 tiles at a time, one a lane: the table is read once for 32 steps, and no
 // step waits for it.
@@ -282,6 +307,9 @@ struct Tiles {
 // rounded to FP16, the type the matrix cores take beside V: by 2^-11 of
 // themselves, as the output is, or by 2^-37 of the largest where they are
 // subnormal.
+//
+// An RNE narrowing of a weight that is kept as two halves, as attention of single
+// tokens has it, would double the products of V, which here are many.
 //
 // A step whose tokens all rows see needs no masks. In the others, those of the
 // drafts, of the window's edge and of missing pages, what some of the rows do
@@ -588,7 +616,10 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
 // holds 32 rows as columns of S^T = K Q^T (32x32x16 products, keys as rows), so
 // that a lane's scores all belong to one row, and rounded to halves they are the
 // B operand of O^T += V^T P^T as they stand. 16-byte pieces of a row are permuted
-// in LDS against bank conflicts; V is read transposing.
+// in LDS against bank conflicts; V is read transposing. 8-bit steps are asked for
+// two ahead, FP16 ones, twice as large, one ahead. Three workgroups a CU instead of
+// two, on one buffer and one step ahead, spill with heads of 128 and took 107
+// instead of 111 us at 64 streams of 16 drafts, heads of 64.
 template <int KIND_, int D_, int RG_, int KG_>
 struct TileCfg {
     static constexpr int KIND = KIND_, D = D_, RG = RG_, KG = KG_, WAVES = RG * KG, ROWS = RG * 32, OCC = 2;
@@ -925,15 +956,16 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void drafts_kernel(DraftArgs
 // Puts the parts of a stream's and key head's rows together, ROWS at a time:
 // LANES threads hold a part's row, four values each, and GROUPS of them take every
 // GROUPS-th part, each with a base of its own; they are put together in LDS.
-// `turns` workgroups take a stream's and key head's rows by turns.
-template <int LANES, int ROWS, int GROUPS>
+// `turns` workgroups take a stream's and key head's rows by turns. ANY: heads of
+// any size, rows of any alignment.
+template <int LANES, int ROWS, int GROUPS, bool ANY = false>
 __global__ __launch_bounds__(LANES* ROWS* GROUPS) void drafts_join_kernel(DraftArgs a, int turns)
 {
     __shared__ floatx4 sums[GROUPS][ROWS][LANES];
     __shared__ float2 states[GROUPS][ROWS];
     constexpr float kBase0 = -3.402823466e38f;
     const int lane = threadIdx.x & 63, rest = blockIdx.x / turns, head = rest % a.heads, stream = rest / a.heads;
-    const int at = threadIdx.x % LANES, r = threadIdx.x / LANES % ROWS, group = threadIdx.x / (LANES * ROWS), d = at * 4;
+    const int at = threadIdx.x % LANES, r = threadIdx.x / LANES % ROWS, group = threadIdx.x / (LANES * ROWS);
     const View w(a, stream);
     const int rows = w.queries * a.group;
     int total = 0, start = 0;
@@ -946,58 +978,64 @@ __global__ __launch_bounds__(LANES* ROWS* GROUPS) void drafts_join_kernel(DraftA
     const Shares shares(a.shares, total, a.spare);
     const int first = w.steps ? shares.holder(start) : 0, parts = w.steps ? shares.holder(start + w.steps - 1) - first + 1 : 0;
     if (parts == 1) return;  // written by the share that holds it
-    for (int row0 = blockIdx.x % turns * ROWS; row0 < rows; row0 += turns * ROWS) {
-        const int row = min(row0 + r, rows - 1);
-        const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + row) * a.places + first + stream;
-        float base = kBase0, l = 0.0f;
-        floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int row0 = blockIdx.x % turns * ROWS; row0 < rows; row0 += turns * ROWS)
+        for (int d = at * 4; d < (ANY ? a.dim : LANES * 4); d += LANES * 4) {
+            const int row = min(row0 + r, rows - 1);
+            const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + row) * a.places + first + stream;
+            float base = kBase0, l = 0.0f;
+            floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-        for (int i = group; i < parts; i += GROUPS) {
-            const floatx4 v = *reinterpret_cast<const floatx4*>(a.part + (slot + i) * a.dim + d);
-            const float2 st = a.state[slot + i];
-            const float now = fmaxf(base, st.x), old = __builtin_amdgcn_exp2f(base - now), f = __builtin_amdgcn_exp2f(st.x - now);
-            base = now;
-            l = l * old + st.y * f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) sum[c] = sum[c] * old + v[c] * f;
-        }
-        if constexpr (GROUPS > 1) {
-            __syncthreads();  // the last rows' sums are read
-            sums[group][r][at] = sum;
-            if (at == 0) states[group][r] = make_float2(base, l);
-            __syncthreads();
-            if (group != 0) continue;
-            float top = kBase0;
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, states[i][r].x);
-            l = 0.0f;
-            sum = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                const float2 st = states[i][r];
-                const float f = __builtin_amdgcn_exp2f(st.x - top);
-                l += st.y * f;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) sum[c] = fmaf(sums[i][r][at][c], f, sum[c]);
-            }
-        }
-        // A part that is infinite, with however small a weight.
-        if (!is_finite(sum[0]) || !is_finite(sum[1]) || !is_finite(sum[2]) || !is_finite(sum[3])) {
-            floatx4 odd = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int i = 0; i < parts; ++i) {
+            for (int i = group; i < parts; i += GROUPS) {
                 const floatx4 v = *reinterpret_cast<const floatx4*>(a.part + (slot + i) * a.dim + d);
+                const float2 st = a.state[slot + i];
+                const float now = fmaxf(base, st.x), old = __builtin_amdgcn_exp2f(base - now), f = __builtin_amdgcn_exp2f(st.x - now);
+                base = now;
+                l = l * old + st.y * f;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) odd[c] += is_finite(v[c]) ? 0.0f : v[c];
+                for (int c = 0; c < 4; ++c) sum[c] = sum[c] * old + v[c] * f;
             }
+            if constexpr (GROUPS > 1) {
+                __syncthreads();  // the last rows' sums are read
+                sums[group][r][at] = sum;
+                if (at == 0) states[group][r] = make_float2(base, l);
+                __syncthreads();
+                if (group != 0) continue;
+                float top = kBase0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) sum[c] = is_finite(sum[c]) ? sum[c] : odd[c];
+                for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, states[i][r].x);
+                l = 0.0f;
+                sum = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < GROUPS; ++i) {
+                    const float2 st = states[i][r];
+                    const float f = __builtin_amdgcn_exp2f(st.x - top);
+                    l += st.y * f;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) sum[c] = fmaf(sums[i][r][at][c], f, sum[c]);
+                }
+            }
+            // A part that is infinite, with however small a weight.
+            if (!is_finite(sum[0]) || !is_finite(sum[1]) || !is_finite(sum[2]) || !is_finite(sum[3])) {
+                floatx4 odd = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int i = 0; i < parts; ++i) {
+                    const floatx4 v = *reinterpret_cast<const floatx4*>(a.part + (slot + i) * a.dim + d);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) odd[c] += is_finite(v[c]) ? 0.0f : v[c];
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sum[c] = is_finite(sum[c]) ? sum[c] : odd[c];
+            }
+            if (row0 + r >= rows) continue;
+            const float f = l == 0.0f ? 0.0f : 1.0f / l;
+            const int of = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(a.group));
+            std::uint16_t* const out = a.out + (w.start + of) * a.out_stride + static_cast<std::int64_t>(head * a.group + row - of * a.group) * a.dim + d;
+            if constexpr (ANY) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) out[c] = f2h(opaque(sum[c] * f));
+            } else {
+                *reinterpret_cast<uint2*>(out) = make_uint2(pack_rounded(sum[0] * f, sum[1] * f), pack_rounded(sum[2] * f, sum[3] * f));
+            }
         }
-        if (row0 + r >= rows) continue;
-        const float f = l == 0.0f ? 0.0f : 1.0f / l;
-        const int of = static_cast<int>(static_cast<unsigned>(row) / static_cast<unsigned>(a.group));
-        *reinterpret_cast<uint2*>(a.out + (w.start + of) * a.out_stride + static_cast<std::int64_t>(head * a.group + row - of * a.group) * a.dim + d) =
-            make_uint2(pack_rounded(sum[0] * f, sum[1] * f), pack_rounded(sum[2] * f, sum[3] * f));
-    }
 }
 
 void check_desc(const mlvc_hip_attention_drafts_desc* d, const char* op)
@@ -1013,15 +1051,15 @@ void check_desc(const mlvc_hip_attention_drafts_desc* d, const char* op)
 }
 
 // Workgroups: rows of one, and how many fit a CU.
-enum Shape { kOne8, kOne4, kTwo4, kTile21, kTile22, kTile41, kTile42 };
-constexpr int kRows[] = {16, 16, 32, 64, 64, 128, 128}, kPerCu[] = {1, 3, 2, 4, 2, 2, 1};
+enum Shape { kOne8, kOne4, kTwo4, kTile21, kTile22, kTile41, kTile42, kAny };
+constexpr int kRows[] = {16, 16, 32, 64, 64, 128, 128, 1}, kPerCu[] = {1, 3, 2, 4, 2, 2, 1, 16};
 
 // Parts of a call for each CU, at most: those of its workgroups' rows, twice where
 // there are small shares behind the large ones.
 constexpr int kParts = 256;
 constexpr bool enough_parts()
 {
-    for (int i = kOne8; i <= kTile42; ++i)
+    for (int i = kOne8; i <= kAny; ++i)
         if (kRows[i] * kPerCu[i] * (i == kOne4 ? 2 : 1) > kParts) return false;
     return true;
 }
@@ -1031,7 +1069,6 @@ static_assert(enough_parts());
 struct Plan {
     Shape shape;
     int blocks, shares;
-    bool fast;
     std::int64_t row_count;  // rows of all key heads
     size_t part_bytes, bytes;
 };
@@ -1064,20 +1101,21 @@ struct Plan {
 //     8 x 32, 4000 to 8160, FP16     151   90.1  75.0   70.9   73.9   67.2*
 //     1 x 64, 65280                  223   128   130    132    123*   129
 //     64 x 64, 64 to 8160            906   599   524    563    476*   537
-Plan plan(const mlvc_hip_attention_drafts_desc* d)
+// `vectors`: rows of q and out on 16 bytes. Other rows and heads take a wave each.
+Plan plan(const mlvc_hip_attention_drafts_desc* d, bool vectors)
 {
     Plan p{};
     const mlvc_hip_kv_cache* c = d->cache;
     const std::int64_t rows = static_cast<std::int64_t>(d->longest_q) * (d->q_heads / c->heads), cus = conv::cu_count();
     p.row_count = rows * c->heads;
-    p.fast = c->head_dim == 64 || c->head_dim == 128;
-    if (!p.fast) return p;
+    const bool fast = vectors && (c->head_dim == 64 || c->head_dim == 128);
     // Tokens that a stream's drafts see at most, and those beside them in their steps.
     std::int64_t longest = d->longest;
     if (d->window) longest = std::min(longest, static_cast<std::int64_t>(d->window) + d->longest_q + std::min(d->sinks, d->longest) + 2 * kStep);
     auto workgroups = [&](Shape shape) { return (rows + kRows[shape] - 1) / kRows[shape] * c->heads * d->streams; };
     auto take = [&](Shape shape) { p.shape = shape, p.blocks = static_cast<int>((rows + kRows[shape] - 1) / kRows[shape]); };
-    take(workgroups(kOne4) <= cus                                     ? kOne8
+    take(!fast                                                        ? kAny
+         : workgroups(kOne4) <= cus                                   ? kOne8
          : rows <= 16                                                 ? kOne4
          : rows <= 32 || workgroups(kTwo4) <= 2 * cus                 ? kTwo4
          : rows <= 64 || workgroups(kTile22) <= 4 * cus               ? kTile22
@@ -1090,9 +1128,10 @@ Plan plan(const mlvc_hip_attention_drafts_desc* d)
     p.part_bytes = slots * c->head_dim * sizeof(float);
     p.bytes = p.part_bytes + slots * sizeof(float2);
     const std::int64_t whole = workgroups(p.shape);
-    if ((longest <= 2048 && 2 * whole >= cus) || (longest <= 4096 && whole >= 3 * cus)) return p;
+    if (fast ? (longest <= 2048 && 2 * whole >= cus) || (longest <= 4096 && whole >= 3 * cus) : whole >= kPerCu[kAny] * cus) return p;
     const bool bytes = c->kind != MLVC_KV_F16, many = static_cast<std::int64_t>(c->heads) * d->streams >= cus;
-    take(rows <= 16 || workgroups(kOne4) * (longest / kStep) <= 48 * cus ? kOne4
+    take(!fast                                                           ? kAny
+         : rows <= 16 || workgroups(kOne4) * (longest / kStep) <= 48 * cus ? kOne4
          : rows <= 32                                                    ? kTwo4
          : rows <= 64                                                    ? (bytes && many ? kTile21 : kTile22)
                                                                          : (bytes ? kTile41 : kTile42));
@@ -1118,27 +1157,30 @@ void launch_drafts(const DraftArgs& a, Shape shape, unsigned grid, hipStream_t s
     case kTile22: return launch_drafts<TileCfg<KIND, D, 2, 2>>(a, grid, s);
     case kTile41: return launch_drafts<TileCfg<KIND, D, 4, 1>>(a, grid, s);
     case kTile42: return launch_drafts<TileCfg<KIND, D, 4, 2>>(a, grid, s);
+    case kAny: break;
     }
 }
 
 template <int KIND>
-void launch_drafts(const DraftArgs& a, const Plan& p, bool fast, unsigned grid, hipStream_t s)
+void launch_drafts(const DraftArgs& a, const Plan& p, unsigned grid, hipStream_t s)
 {
-    if (!fast) drafts_any_kernel<KIND><<<grid, 64, 0, s>>>(a);
+    if (p.shape == kAny) drafts_any_kernel<KIND><<<grid, 64, 0, s>>>(a);
     else if (a.dim == 64) launch_drafts<KIND, 64>(a, p.shape, grid, s);
     else launch_drafts<KIND, 128>(a, p.shape, grid, s);
 }
 
 template <int LANES>
-void launch_join(const DraftArgs& a, hipStream_t s)
+void launch_join(const DraftArgs& a, bool any, hipStream_t s)
 {
     // A row for 256 threads where there are few; else eight at a time, by no more
     // workgroups than find where the parts lie in one turn of the GPU.
     const int rows = a.longest_q * a.group;
     const std::int64_t of_head = static_cast<std::int64_t>(a.heads) * a.streams;
-    if (rows * of_head > 4096) {
+    if (any || rows * of_head > 4096) {
         const int turns = static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>((rows + 7) / 8, 8 * conv::cu_count() / of_head)));
-        drafts_join_kernel<LANES, 8, 1><<<static_cast<unsigned>(turns * of_head), LANES * 8, 0, s>>>(a, turns);
+        const unsigned grid = static_cast<unsigned>(turns * of_head);
+        if (any) drafts_join_kernel<LANES, 8, 1, true><<<grid, LANES * 8, 0, s>>>(a, turns);
+        else drafts_join_kernel<LANES, 8, 1><<<grid, LANES * 8, 0, s>>>(a, turns);
     } else {
         drafts_join_kernel<LANES, 1, 256 / LANES><<<static_cast<unsigned>(rows * of_head), 256, 0, s>>>(a, rows);
     }
@@ -1156,16 +1198,11 @@ void attention_drafts(const mlvc_hip_attention_drafts_desc* d, hipStream_t s)
     require(aligned2(d->q) && aligned2(d->out), op, "a tensor is not aligned to its FP16 values");
     require(aligned_to<8>(d->seen) && aligned_to<4>(d->starts) && aligned_to<4>(d->lengths) && aligned_to<4>(d->table), op,
             "seen, starts, lengths or table is not aligned to its values");
-    Plan p = plan(d);
-    const bool fast = p.fast && vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride);
-    if (!fast) p.shares = 0;
+    const Plan p = plan(d, vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride));
     const std::int64_t all_rows = static_cast<std::int64_t>(d->streams) * p.row_count;
-    std::int64_t grid = all_rows;
-    if (fast) {
-        const std::int64_t items = static_cast<std::int64_t>(d->cache->heads) * (p.shares ? (p.shape == kOne4 ? 2 : 1) * p.shares : d->streams);
-        grid = p.blocks == 1 ? items : (items + kXcds - 1) / kXcds * kXcds * p.blocks;
-    }
-    require(launchable(grid, fast ? 512 : 64) && launchable(all_rows, 256) &&
+    const std::int64_t items = static_cast<std::int64_t>(d->cache->heads) * (p.shares ? (p.shape == kOne4 ? 2 : 1) * p.shares : d->streams);
+    const std::int64_t grid = p.blocks == 1 || p.shape == kAny ? items * p.blocks : (items + kXcds - 1) / kXcds * kXcds * p.blocks;
+    require(launchable(grid, 512) && launchable(all_rows, 256) &&
                 static_cast<std::int64_t>(d->streams) * (d->longest / kStep + 2) <= INT_MAX, op,
             "too many streams, heads and drafts in one call");
     require(p.bytes == 0 || (d->workspace && d->workspace_bytes >= p.bytes && aligned16(d->workspace)), op,
@@ -1188,13 +1225,13 @@ void attention_drafts(const mlvc_hip_attention_drafts_desc* d, hipStream_t s)
     a.shares = p.shares, a.blocks = p.blocks, a.spare = p.shape == kOne4;
     a.places = (a.spare ? 2 : 1) * a.shares + a.streams;
     const unsigned n = static_cast<unsigned>(grid);
-    if (c->kind == MLVC_KV_F16) launch_drafts<MLVC_KV_F16>(a, p, fast, n, s);
-    else if (c->kind == MLVC_KV_E4M3) launch_drafts<MLVC_KV_E4M3>(a, p, fast, n, s);
-    else launch_drafts<MLVC_KV_INT8>(a, p, fast, n, s);
+    if (c->kind == MLVC_KV_F16) launch_drafts<MLVC_KV_F16>(a, p, n, s);
+    else if (c->kind == MLVC_KV_E4M3) launch_drafts<MLVC_KV_E4M3>(a, p, n, s);
+    else launch_drafts<MLVC_KV_INT8>(a, p, n, s);
     check(hipGetLastError(), "attention_drafts launch");
     if (!p.shares) return;
-    if (a.dim == 64) launch_join<16>(a, s);
-    else launch_join<32>(a, s);
+    if (a.dim == 64) launch_join<16>(a, p.shape == kAny, s);
+    else launch_join<32>(a, p.shape == kAny, s);
 }
 
 }  // namespace
@@ -1209,7 +1246,7 @@ size_t mlvc_hip_attention_drafts_workspace_bytes(const mlvc_hip_attention_drafts
     size_t bytes = 0;
     guard([&] {
         check_desc(desc, "attention_drafts");
-        bytes = plan(desc).bytes;
+        bytes = plan(desc, true).bytes;  // the same for any rows
     });
     return bytes;
 }

@@ -9,9 +9,12 @@
 // searched: what goes back and what is taken are ranges of entries, and prefix
 // sums over the streams give each of them its place in the stack of free pages.
 //
-// Bound by latency: one workgroup does the table (lengths, three scans, the few
-// entries that change), and the tokens too where they are few; more of them are
-// a second launch over all CUs, bound by 8 bytes written a token.
+// Bound by latency: one workgroup does the table (lengths, scans, the few entries
+// that change, dealt to all threads), and the tokens too where they are few; more
+// of them are a second launch over all CUs. 64 streams of one token: 4.3 us in the
+// kernel, of them 3 for an empty launch; 64 ragged prompts of up to 2040 tokens
+// behind a window, 61 thousand slots and 4 thousand pages handed out, 10.7 + 3.4
+// (37 + 5 with a stream's pages by one thread).
 
 #include "attention.hpp"
 

@@ -351,6 +351,14 @@ def test_drafts_shapes(dev, rng, kind, dim, q_heads, heads, counts, lengths, win
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("q_heads,heads,dim,extra,shift", [(4, 2, 96, 0, 0), (3, 1, 24, 0, 0), (2, 1, 200, 0, 0), (4, 2, 64, 1, 0), (2, 1, 128, 0, 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1500, 40)])
+def test_drafts_cut_other_heads(dev, rng, kind, q_heads, heads, dim, extra, shift, window, sinks):
+    """Contexts that are cut, heads and rows of the plain kernel."""
+    _drafts(dev, rng, kind, q_heads, heads, dim, 16, [5, 1, 9, 0], [2100, 40, 1700, 3], window, sinks, extra, shift)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("q_heads,drafts,n", [(2, 3, 700), (4, 16, 700), (6, 40, 300), (2, 5, 1500), (4, 60, 6000), (2, 20, 9000)])
 def test_drafts_of_zero_values_and_far_scores(dev, rng, kind, dim, q_heads, drafts, n):
@@ -394,7 +402,7 @@ def test_drafts_of_large_scores(dev, rng, kind, q_heads, drafts, dim):
             within(got[i, h], want, tol, f"draft {i}")
 
 
-@pytest.mark.parametrize("q_heads,drafts,dim,n", [(2, 3, 64, 200), (4, 8, 128, 900), (6, 40, 128, 300), (4, 64, 64, 3000), (4, 30, 128, 5000), (2, 9, 96, 100)])
+@pytest.mark.parametrize("q_heads,drafts,dim,n", [(2, 3, 64, 200), (4, 8, 128, 900), (6, 40, 128, 300), (4, 64, 64, 3000), (4, 30, 128, 5000), (2, 9, 96, 100), (2, 9, 96, 2000)])
 def test_drafts_of_infinite_values(dev, rng, q_heads, drafts, dim, n):
     """Infinities and NaN among the values of an FP16 cache reach the drafts that see them, and no others."""
     ctx = Contexts(dev, rng, Cache, KV_F16, 1, dim, 16, [n, n])
