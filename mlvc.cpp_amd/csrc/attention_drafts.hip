@@ -11,7 +11,7 @@
 // query heads that share it): 64 streams of one token under a window of 4080, 32
 // query heads on 8 of 128, E4M3, 0.51 GB in 111 us or 4.6 TB/s. From 64 rows on
 // by what is computed for a cached row, its unpacking and the softmax: 64 streams
-// of 16 drafts on up to 8160 tokens, INT8, 0.55 GB and 69 GFLOP in 170 us, vector
+// of 16 drafts on up to 8160 tokens, INT8, 0.57 GB and 69 GFLOP in 170 us, vector
 // units busy 50% of the time and matrix cores 20%, the rest waits for LDS and for
 // products that follow from each other; 64 of 64 drafts 275 GFLOP in 462 us. One
 // token under a window of 920 is a launch and the latency of four steps, 9.0 us.

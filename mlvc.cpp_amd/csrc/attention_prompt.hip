@@ -806,7 +806,8 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 // Under a window a workgroup's keys are few and as many in each, so that 256
 // queries gain nothing, and key groups less: two beside 64 queries while those
 // workgroups fit the GPU at once, four beside 32 or 64 while they fit the CUs.
-// us, a window of w (16 query heads, 4 sinks, causal):
+// us, a window of w (16 query heads, 4 sinks, causal; each is 3 to 6% less since
+// masks come from a word of bits):
 //   heads of 128              (1,4,32) (2,4,32) (2,2,32) (4,2,64) (4,1,64) (8,1,64)
 //     10 on 1500, w 700         12.1     13.3     14.9     17.6     21.6     24.8
 //     240, w 80                  9.2     10.7     10.0     12.6     13.3     16.0
