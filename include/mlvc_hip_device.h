@@ -533,7 +533,7 @@ int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip
  * window and of the first `sinks` tokens only.
  *
  * Window and sinks, in all of them: a token at place p sees a token at place j
- * if p - j < window (and j - p < window, where it sees later ones at all) or
+ * if p - j < window (and j - p < window in attention_window both ways) or
  * j < sinks. Window 0: no window.
  *
  * As above, 16-byte aligned rows of heads of 64 or 128 run the fast attention
@@ -551,7 +551,7 @@ int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip
  *      stream by stream, from the top of the stack free_pages; the first one
  *      that the pool does not suffice for and those behind it that need a page
  *      get none (lacking counts them), nor does a stream whose tokens go beyond
- *      its table row;
+ *      its table row or 2^31 - 1;
  *   3. lengths[n] = past[n] + fresh[n] (past[n] for a stream that got no pages),
  *      starts = 0, then the sums of fresh; token t, the i-th new one of stream
  *      n, has slots[t], the slot of place past[n] + i, and positions[t] = past[n]

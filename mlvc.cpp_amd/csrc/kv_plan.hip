@@ -66,7 +66,7 @@ struct Row {
         back = min(end, kept);
         front = a.window ? max(window, min(begin, kept)) : 0;
         const std::int64_t all = static_cast<std::int64_t>(past) + fresh;
-        fits = all <= static_cast<std::int64_t>(a.table_stride) * a.page;
+        fits = all <= min(static_cast<std::int64_t>(a.table_stride) * a.page, static_cast<std::int64_t>(INT_MAX));  // lengths have 32 bits
         need = fits ? max(pages_of(a, all) - back, 0) : 0;
     }
     __device__ int returned() const { return count[0] + count[1] + count[2]; }

@@ -91,6 +91,24 @@ def test_plan_of_a_long_prompt(dev, rng):
     plan.step([8160, 1, 5000, 0, 3001], [1, 2000, 8, 600, -1])
 
 
+def test_plan_of_lengths_at_31_bits(dev):
+    page, last = 1 << 28, (1 << 31) - 1
+    plan = Plan(dev, 1, 7, page, 9, window=16)
+    get = lambda at, n: dev.get(at, (n,), np.int32).tolist()  # noqa: E731
+
+    def step(past, fresh, tokens=8):
+        mlvc_hip.kv_plan(plan.desc([past], [fresh], tokens))
+        return get(plan.d_lengths, 1)[0], get(plan.d_lacking, 1)[0], get(plan.slots, tokens)
+
+    assert step(0, 1 << 30)[:2] == (1 << 30, 0)
+    assert step(1 << 30, (1 << 30) - 5)[:2] == (last - 4, 0)
+    page_of = get(plan.d_table, 9)[7] * page
+    assert get(plan.d_table, 9)[8] == -1 and page_of >= 0
+    # One more than a length can count: the row has an entry for it, and it goes without.
+    assert step(last - 4, 5) == (last - 4, 1, [-1] * 8)
+    assert step(last - 4, 4) == (last, 0, [page_of + page - 5 + i for i in range(4)] + [-1] * 4)
+
+
 # ------------------------------------------------------------ kept drafts
 
 @pytest.mark.parametrize("kind", KINDS)
