@@ -537,8 +537,10 @@ int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip
  * j < sinks. Window 0: no window.
  *
  * As above, 16-byte aligned rows of heads of 64 or 128 run the fast attention
- * kernels; others take plain ones, one wave a draft and head, on long contexts
- * slower than a matrix product of a library. Nothing here allocates, waits or
+ * kernels. attention_drafts pads other rows and heads of up to 256 whose cached
+ * rows are multiples of 16 bytes; what is left takes plain kernels, one wave a
+ * query and head, on long contexts slower than a matrix product of a library.
+ * Nothing here allocates, waits or
  * reads device memory on the host, so a step can be captured into a graph. */
 
 /* Page tables, slots and positions of a step, from the streams' lengths on the

@@ -163,7 +163,8 @@ __device__ __forceinline__ void decide_odd(const DraftArgs& a, const View& w, co
     for (int r = 0; r < 4; ++r) sums[r] = odd[r].sum(sums[r]);
 }
 
-// Any head size: one wave for a piece of a context and a draft's query head, 64
+// Heads of more than 256 values and cached rows that are no whole 16-byte pieces
+// (8-bit heads of 8, 24, 40, ...): one wave for a piece of a context and a draft's query head, 64
 // tokens at a time, one token a lane for the scores and one value column a lane
 // for the sum.
 template <int KIND>
@@ -620,14 +621,26 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
 // two ahead, FP16 ones, twice as large, one ahead. Three workgroups a CU instead of
 // two, on one buffer and one step ahead, spill with heads of 128 and took 107
 // instead of 111 us at 64 streams of 16 drafts, heads of 64.
-template <int KIND_, int D_, int RG_, int KG_>
+//
+// PAD: heads of up to D values, with zeros behind them in LDS, and rows of q and
+// out of any alignment; the cache's rows are whole 16-byte pieces. us of a call,
+// and of one wave for each row, value by value, as other rows are taken:
+//   1 x 16 on 65280, E4M3, 32 / 8 heads of 96     67.8   8720
+//                                    of 256        149  31900
+//   64 x 16 on 16 to 8160, INT8, heads of 96       181  17400
+//   16 x 64 on 920 to 3001, FP16, 16 heads of 96  62.8   4050
+//   1 x 1, a window of 920, INT8, heads of 96     24.9    272
+// Heads of more than 128 leave one wave a SIMD, of up to 512 registers, with steps
+// one ahead (two ahead spill twice as many registers).
+template <int KIND_, int D_, int RG_, int KG_, bool PAD_ = false>
 struct TileCfg {
-    static constexpr int KIND = KIND_, D = D_, RG = RG_, KG = KG_, WAVES = RG * KG, ROWS = RG * 32, OCC = 2;
+    static constexpr int KIND = KIND_, D = D_, RG = RG_, KG = KG_, WAVES = RG * KG, ROWS = RG * 32, OCC = D > 128 ? 1 : 2;
+    static constexpr bool PAD = PAD_;
     static constexpr int BYTES = KIND == MLVC_KV_F16 ? 2 : 1;
     static constexpr int TILE = kStep * D;                     // halves of K or V of a step
     static constexpr int LOADS = 2 * kStep * D * BYTES / 1024; // of a wave, for K and V of a step
     static constexpr int MINE = (LOADS + RG - 1) / RG;         // of each wave of a group
-    static constexpr int DEPTH = KIND == MLVC_KV_F16 ? 1 : 2;     // steps on their way
+    static constexpr int DEPTH = KIND == MLVC_KV_F16 || D > 128 ? 1 : 2;  // steps on their way
     static constexpr int WORDS = D / 8 + 1;                    // 16-byte words of a lane's state
     static constexpr size_t TILES = KG * 2 * 2 * TILE * 2, SCALES = KG * 2 * 2 * kStep * sizeof(float),
                             JOINT = static_cast<size_t>(KG - 1) * WORDS * RG * 64 * 16;
@@ -639,9 +652,9 @@ struct TileCfg {
     // cycles at 64 streams of 16 drafts).
     __host__ __device__ static constexpr int place(int piece, int t)
     {
-        if (BYTES == 2) return piece ^ (D == 128 ? 4 * (t & 3) + (t >> 2 & 3) : 4 * (t >> 1 & 1) + (t >> 2 & 3));
+        if (BYTES == 2) return piece ^ (D >= 128 ? 4 * (t & 3) + (t >> 2 & 3) : 4 * (t >> 1 & 1) + (t >> 2 & 3));
         const int evens_first = (piece >> 1) + (piece & 1) * (D / 16);
-        return evens_first ^ (D == 128 ? 2 * (t & 3) + (t >> 2 & 1) + 8 * (t >> 3 & 1) : 2 * (t >> 1 & 1) + (t >> 2 & 1) + 4 * ((t >> 3 ^ t) & 1));
+        return evens_first ^ (D >= 128 ? 2 * (t & 3) + (t >> 2 & 1) + 8 * (t >> 3 & 1) : 2 * (t >> 1 & 1) + (t >> 2 & 1) + 4 * ((t >> 3 ^ t) & 1));
     }
 };
 
@@ -650,6 +663,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
                                            int first, int last, bool whole, int place)
 {
     constexpr int D = C::D, KIND = C::KIND, RG = C::RG, KG = C::KG, KS = D / 16, DT = D / 32, RB = D * C::BYTES;
+    const int dim = C::PAD ? a.dim : D;
     constexpr float kBase0 = -3.402823466e38f;
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
@@ -680,7 +694,12 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
             if (C::LOADS % RG != 0 && n >= C::LOADS) continue;
             const bool is_v = n >= C::LOADS / 2;
             const int byte = (n - (is_v ? C::LOADS / 2 : 0)) * 1024, t = byte / RB / 16;
-            c.raw[i] = *reinterpret_cast<const u32x4*>((is_v ? a.v : a.k) + (t ? row[1] : row[0]) * RB + (byte - t * 16 * RB) + lane * 16);
+            if constexpr (C::PAD) {  // the first piece again where there is none
+                const int at = byte - t * 16 * RB + lane * 16, r = at / RB, inside = at - r * RB, rb = dim * C::BYTES;
+                c.raw[i] = *reinterpret_cast<const u32x4*>((is_v ? a.v : a.k) + (t ? row[1] : row[0]) * rb + r * rb + (inside < rb ? inside : 0));
+            } else {
+                c.raw[i] = *reinterpret_cast<const u32x4*>((is_v ? a.v : a.k) + (t ? row[1] : row[0]) * RB + (byte - t * 16 * RB) + lane * 16);
+            }
         }
         if constexpr (KIND != MLVC_KV_F16) c.scale = (hi ? a.v_scale : a.k_scale)[(lane & 16 ? row[1] : row[0]) + (lane & 15)];
     };
@@ -708,12 +727,21 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
     // This lane's row: of a draft and a query head.
     const int at_row = row0 + min(rg * 32 + column, mine - 1), draft = static_cast<int>(static_cast<unsigned>(at_row) / static_cast<unsigned>(a.group));
     const bool has_rows = rg * 32 < mine, my_row = rg * 32 + column < mine;
-    const std::int64_t token = w.start + draft, at_head = static_cast<std::int64_t>(head * a.group + at_row - draft * a.group) * D;
+    const std::int64_t token = w.start + draft, at_head = static_cast<std::int64_t>(head * a.group + at_row - draft * a.group) * dim;
     half8 q[KS];
     {
         const std::uint16_t* x = a.q + token * a.q_stride + at_head + hi * 8;
 #pragma unroll
-        for (int i = 0; i < KS; ++i) q[i] = __builtin_bit_cast(half8, *reinterpret_cast<const u32x4*>(x + i * 16));
+        for (int i = 0; i < KS; ++i) {
+            if constexpr (C::PAD) {
+                q[i] = half8{};
+                if (i * 16 + hi * 8 >= dim) continue;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q[i][e] = __builtin_bit_cast(_Float16, x[i * 16 + e]);
+            } else {
+                q[i] = __builtin_bit_cast(half8, *reinterpret_cast<const u32x4*>(x + i * 16));
+            }
+        }
     }
     const int clear_from = a.window ? max(w.past + min(w.drafts, kMostDrafts) - a.window, 0) : 0;
 
@@ -753,6 +781,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
             std::uint16_t* const to = tile + (is_v ? C::TILE : 0) + r * D;
             const bool gone = masked && is_v && (!(r & 16 ? c.there[1] : c.there[0]) || c.j + r >= w.length);
             auto put = [&](int at, u32x4 x) {
+                if (C::PAD && at * 8 >= dim) x = u32x4{0, 0, 0, 0};
                 if (masked && is_v) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -899,6 +928,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 floatx4 v = {acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+                if (C::PAD && dt * 32 + 8 * g >= dim) continue;
                 if (*odd_met || !is_finite(v[0]) || !is_finite(v[1]) || !is_finite(v[2]) || !is_finite(v[3])) {
                     decide_odd(a, w, sight, stream, head, first, last, dt * 32 + 8 * g + 4 * hi, v);
 #pragma unroll
@@ -913,16 +943,22 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<uint2*>(out + dt * 32 + 8 * g) = make_uint2(pack_rounded(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f),
-                                                                              pack_rounded(acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f));
+                if constexpr (C::PAD) {
+                    if (dt * 32 + 8 * g >= dim) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[dt * 32 + 8 * g + e] = f2h(opaque(acc[dt][4 * g + e] * f));
+                } else {
+                    *reinterpret_cast<uint2*>(out + dt * 32 + 8 * g) = make_uint2(pack_rounded(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f),
+                                                                                  pack_rounded(acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f));
+                }
     } else {
         const std::int64_t slot = (static_cast<std::int64_t>(head) * a.longest_q * a.group + at_row) * a.places + place;
-        float* const part = a.part + slot * D + 4 * hi;
+        float* const part = a.part + slot * dim + 4 * hi;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<floatx4*>(part + dt * 32 + 8 * g) = floatx4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
+                if (!C::PAD || dt * 32 + 8 * g < dim) *reinterpret_cast<floatx4*>(part + dt * 32 + 8 * g) = floatx4{acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]};
         if (hi == 0) a.state[slot] = make_float2(base, l);
     }
 }
@@ -1051,8 +1087,8 @@ void check_desc(const mlvc_hip_attention_drafts_desc* d, const char* op)
 }
 
 // Workgroups: rows of one, and how many fit a CU.
-enum Shape { kOne8, kOne4, kTwo4, kTile21, kTile22, kTile41, kTile42, kAny };
-constexpr int kRows[] = {16, 16, 32, 64, 64, 128, 128, 1}, kPerCu[] = {1, 3, 2, 4, 2, 2, 1, 16};
+enum Shape { kOne8, kOne4, kTwo4, kTile21, kTile22, kTile41, kTile42, kPad, kAny };
+constexpr int kRows[] = {16, 16, 32, 64, 64, 128, 128, 64, 1}, kPerCu[] = {1, 3, 2, 4, 2, 2, 1, 2, 16};
 
 // Parts of a call for each CU, at most: those of its workgroups' rows, twice where
 // there are small shares behind the large ones.
@@ -1101,7 +1137,8 @@ struct Plan {
 //     8 x 32, 4000 to 8160, FP16     151   90.1  75.0   70.9   73.9   67.2*
 //     1 x 64, 65280                  223   128   130    132    123*   129
 //     64 x 64, 64 to 8160            906   599   524    563    476*   537
-// `vectors`: rows of q and out on 16 bytes. Other rows and heads take a wave each.
+// `vectors`: rows of q and out on 16 bytes. Other rows and heads are padded, or
+// take a wave a row.
 Plan plan(const mlvc_hip_attention_drafts_desc* d, bool vectors)
 {
     Plan p{};
@@ -1109,12 +1146,14 @@ Plan plan(const mlvc_hip_attention_drafts_desc* d, bool vectors)
     const std::int64_t rows = static_cast<std::int64_t>(d->longest_q) * (d->q_heads / c->heads), cus = conv::cu_count();
     p.row_count = rows * c->heads;
     const bool fast = vectors && (c->head_dim == 64 || c->head_dim == 128);
+    const bool any = c->head_dim > 256 || c->head_dim * (c->kind == MLVC_KV_F16 ? 2 : 1) % 16 != 0;  // cached rows off 16 bytes
     // Tokens that a stream's drafts see at most, and those beside them in their steps.
     std::int64_t longest = d->longest;
     if (d->window) longest = std::min(longest, static_cast<std::int64_t>(d->window) + d->longest_q + std::min(d->sinks, d->longest) + 2 * kStep);
     auto workgroups = [&](Shape shape) { return (rows + kRows[shape] - 1) / kRows[shape] * c->heads * d->streams; };
     auto take = [&](Shape shape) { p.shape = shape, p.blocks = static_cast<int>((rows + kRows[shape] - 1) / kRows[shape]); };
-    take(!fast                                                        ? kAny
+    take(any                                                          ? kAny
+         : !fast                                                      ? kPad
          : workgroups(kOne4) <= cus                                   ? kOne8
          : rows <= 16                                                 ? kOne4
          : rows <= 32 || workgroups(kTwo4) <= 2 * cus                 ? kTwo4
@@ -1128,9 +1167,10 @@ Plan plan(const mlvc_hip_attention_drafts_desc* d, bool vectors)
     p.part_bytes = slots * c->head_dim * sizeof(float);
     p.bytes = p.part_bytes + slots * sizeof(float2);
     const std::int64_t whole = workgroups(p.shape);
-    if (fast ? (longest <= 2048 && 2 * whole >= cus) || (longest <= 4096 && whole >= 3 * cus) : whole >= kPerCu[kAny] * cus) return p;
+    if (!any ? (longest <= 2048 && 2 * whole >= cus) || (longest <= 4096 && whole >= 3 * cus) : whole >= kPerCu[kAny] * cus) return p;
     const bool bytes = c->kind != MLVC_KV_F16, many = static_cast<std::int64_t>(c->heads) * d->streams >= cus;
-    take(!fast                                                           ? kAny
+    take(any                                                             ? kAny
+         : !fast                                                         ? kPad
          : rows <= 16 || workgroups(kOne4) * (longest / kStep) <= 48 * cus ? kOne4
          : rows <= 32                                                    ? kTwo4
          : rows <= 64                                                    ? (bytes && many ? kTile21 : kTile22)
@@ -1157,6 +1197,7 @@ void launch_drafts(const DraftArgs& a, Shape shape, unsigned grid, hipStream_t s
     case kTile22: return launch_drafts<TileCfg<KIND, D, 2, 2>>(a, grid, s);
     case kTile41: return launch_drafts<TileCfg<KIND, D, 4, 1>>(a, grid, s);
     case kTile42: return launch_drafts<TileCfg<KIND, D, 4, 2>>(a, grid, s);
+    case kPad:
     case kAny: break;
     }
 }
@@ -1165,6 +1206,7 @@ template <int KIND>
 void launch_drafts(const DraftArgs& a, const Plan& p, unsigned grid, hipStream_t s)
 {
     if (p.shape == kAny) drafts_any_kernel<KIND><<<grid, 64, 0, s>>>(a);
+    else if (p.shape == kPad) a.dim <= 128 ? launch_drafts<TileCfg<KIND, 128, 2, 2, true>>(a, grid, s) : launch_drafts<TileCfg<KIND, 256, 2, 1, true>>(a, grid, s);
     else if (a.dim == 64) launch_drafts<KIND, 64>(a, p.shape, grid, s);
     else launch_drafts<KIND, 128>(a, p.shape, grid, s);
 }
@@ -1230,8 +1272,8 @@ void attention_drafts(const mlvc_hip_attention_drafts_desc* d, hipStream_t s)
     else launch_drafts<MLVC_KV_INT8>(a, p, n, s);
     check(hipGetLastError(), "attention_drafts launch");
     if (!p.shares) return;
-    if (a.dim == 64) launch_join<16>(a, p.shape == kAny, s);
-    else launch_join<32>(a, p.shape == kAny, s);
+    if (a.dim == 64) launch_join<16>(a, p.shape >= kPad, s);
+    else launch_join<32>(a, p.shape >= kPad, s);
 }
 
 }  // namespace

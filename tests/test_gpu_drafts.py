@@ -369,11 +369,23 @@ def test_drafts_shapes(dev, rng, kind, dim, q_heads, heads, counts, lengths, win
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("q_heads,heads,dim,extra,shift", [(4, 2, 96, 0, 0), (3, 1, 24, 0, 0), (2, 1, 200, 0, 0), (4, 2, 64, 1, 0), (2, 1, 128, 0, 3)])
+@pytest.mark.parametrize("q_heads,heads,dim,extra,shift", [(4, 2, 96, 0, 0), (3, 1, 24, 0, 0), (2, 1, 200, 0, 0), (2, 1, 264, 0, 0), (4, 2, 64, 1, 0), (2, 1, 128, 0, 3)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (1500, 40)])
 def test_drafts_cut_other_heads(dev, rng, kind, q_heads, heads, dim, extra, shift, window, sinks):
-    """Contexts that are cut, heads and rows of the plain kernel."""
+    """Contexts that are cut, heads and rows of the plain kernel and of the padded ones."""
     _drafts(dev, rng, kind, q_heads, heads, dim, 16, [5, 1, 9, 0], [2100, 40, 1700, 3], window, sinks, extra, shift)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [16, 96, 144, 256])
+@pytest.mark.parametrize("q_heads,heads,counts,lengths,window,sinks", [
+    (4, 2, [1, 3, 2, 0, 9], [5, 300, 77, 30, 8], 0, 0),                # whole contexts, few rows
+    (16, 8, [64, 40, 33, 50, 1] * 5, [70, 130, 64, 96, 33] * 5, 50, 3),  # rows of two workgroups
+    (6, 2, [20, 16] * 20, [2600, 31] + [77, 40] * 19, 0, 0),           # cut
+    (4, 2, [64, 3, 33], [5000, 40, 4700], 4400, 100),
+])
+def test_drafts_padded_heads(dev, rng, kind, dim, q_heads, heads, counts, lengths, window, sinks):
+    _drafts(dev, rng, kind, q_heads, heads, dim, 16, counts, lengths, window, sinks)
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -397,7 +409,7 @@ def test_drafts_of_zero_values_and_far_scores(dev, rng, kind, dim, q_heads, draf
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("q_heads,drafts,dim", [(2, 3, 64), (4, 8, 128), (6, 40, 128), (4, 64, 64)])
+@pytest.mark.parametrize("q_heads,drafts,dim", [(2, 3, 64), (4, 8, 128), (6, 40, 128), (4, 64, 64), (3, 9, 96), (2, 9, 512)])
 def test_drafts_of_large_scores(dev, rng, kind, q_heads, drafts, dim):
     """Scores of 2^22 and more, whose last place is more than the weights' own: the largest decides."""
     n = 260
@@ -420,7 +432,7 @@ def test_drafts_of_large_scores(dev, rng, kind, q_heads, drafts, dim):
             within(got[i, h], want, tol, f"draft {i}")
 
 
-@pytest.mark.parametrize("q_heads,drafts,dim,n", [(2, 3, 64, 200), (4, 8, 128, 900), (6, 40, 128, 300), (4, 64, 64, 3000), (4, 30, 128, 5000), (2, 9, 96, 100), (2, 9, 96, 2000)])
+@pytest.mark.parametrize("q_heads,drafts,dim,n", [(2, 3, 64, 200), (4, 8, 128, 900), (6, 40, 128, 300), (4, 64, 64, 3000), (4, 30, 128, 5000), (2, 9, 96, 100), (2, 9, 96, 2000), (2, 40, 256, 3000), (2, 9, 264, 2000)])
 def test_drafts_of_infinite_values(dev, rng, q_heads, drafts, dim, n):
     """Infinities and NaN among the values of an FP16 cache reach the drafts that see them, and no others."""
     ctx = Contexts(dev, rng, Cache, KV_F16, 1, dim, 16, [n, n])
@@ -457,7 +469,7 @@ def test_one_draft_is_the_token_step(dev, rng, kind, dim):
     assert np.abs(a - b).max() <= top * (2.0 ** -10 + 2.0 ** -10)
 
 
-@pytest.mark.parametrize("dim", [64, 96])
+@pytest.mark.parametrize("dim", [64, 96, 264])
 def test_drafts_of_any_masks(dev, rng, dim):
     """Masks that are no tree: later drafts, none at all, bits past the last draft."""
     lengths = [6, 200]
@@ -475,7 +487,7 @@ def test_drafts_of_any_masks(dev, rng, dim):
     assert not got[0].any() and not got[5].any()  # nothing seen
 
 
-@pytest.mark.parametrize("dim", [64, 128, 40])
+@pytest.mark.parametrize("dim", [64, 128, 40, 96])
 def test_drafts_rows_that_are_not_computed(dev, rng, dim):
     """More drafts than longest_q, than 64, than rows of q; more drafts than tokens; rows past the last stream."""
     counts, lengths = [70, 4, 9, 6], [100, 300, 5, 40]
@@ -504,7 +516,7 @@ def test_drafts_rows_that_are_not_computed(dev, rng, dim):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("dim", [64, 128, 72])
+@pytest.mark.parametrize("dim", [64, 128, 72, 160])
 @pytest.mark.parametrize("window", [0, 40])
 def test_drafts_unseen_places_do_not_reach(dev, rng, kind, dim, window):
     """NaN and infinities in drafts of other branches, behind the window, past the end and on pages outside."""
@@ -539,7 +551,7 @@ def test_drafts_unseen_places_do_not_reach(dev, rng, kind, dim, window):
         at += count
 
 
-@pytest.mark.parametrize("dim", [64, 128, 40])
+@pytest.mark.parametrize("dim", [64, 128, 40, 96])
 def test_drafts_of_the_widest_window(dev, rng, dim):
     """A window and sinks of 2^31 - 1, more drafts than tokens among the streams: nothing is cut."""
     counts, lengths = [5, 9, 20], [300, 4, 40]
