@@ -537,9 +537,10 @@ int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip
  * j < sinks. Window 0: no window.
  *
  * As above, 16-byte aligned rows of heads of 64 or 128 run the fast attention
- * kernels. attention_drafts pads other rows and heads of up to 256 whose cached
- * rows are multiples of 16 bytes; what is left takes plain kernels, one wave a
- * query and head, on long contexts slower than a matrix product of a library.
+ * kernels. Heads of other sizes up to 256 are padded: under a window multiples of
+ * 8 on 16-byte aligned rows, for drafts those whose cached rows are multiples of
+ * 16 bytes, on rows of any alignment. What is left takes plain kernels, one wave
+ * a query and head, on long contexts slower than a matrix product of a library.
  * Nothing here allocates, waits or
  * reads device memory on the host, so a step can be captured into a graph. */
 

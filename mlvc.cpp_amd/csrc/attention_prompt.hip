@@ -164,8 +164,12 @@ __device__ __forceinline__ std::uint32_t lds_address(const void* p)
 // the accumulators are seldom rescaled. Weights are rounded to FP16, the type
 // the matrix cores take beside V: by 2^-11 of themselves, as the output is, or
 // by 2^-37 of the largest where they are subnormal. Their sum is of FP32 values.
-template <int D_, int RG_, int KG_, int KEYS_, int OCC_>
+//
+// PAD: heads of up to D values; pieces behind them are out of the buffer's range
+// too. Heads of more than 128 leave one wave a SIMD, of up to 512 registers.
+template <int D_, int RG_, int KG_, int KEYS_, int OCC_, bool PAD_ = false>
 struct PromptCfg {
+    static constexpr bool PAD = PAD_;
     static constexpr int D = D_, RG = RG_, KG = KG_, KEYS = KEYS_, OCC = OCC_;
     static constexpr int WAVES = RG * KG;
     // Several workgroups on a CU: long ones are put beside short ones.
@@ -181,7 +185,7 @@ struct PromptCfg {
     // (a K read) fall on all 64 banks, and so do 4 rows of 4 pieces (a V read).
     __host__ __device__ static constexpr int swizzle(int t)
     {
-        return D == 128 ? 4 * (t & 3) + (t >> 2 & 3) : 4 * (t >> 1 & 1) + (t >> 2 & 3);
+        return D >= 128 ? 4 * (t & 3) + (t >> 2 & 3) : 4 * (t >> 1 & 1) + (t >> 2 & 3);
     }
 };
 
@@ -297,6 +301,7 @@ template <class C, bool WINDOW>
 __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArgs a, int tiles, bool by_turns)
 {
     constexpr int D = C::D, KS = D / 16, DT = D / 32, kKeys = C::KEYS, TT = kKeys / 32;
+    const int dim = C::PAD ? a.dim : D;
     extern __shared__ __attribute__((aligned(16))) std::uint16_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row_group = wave % C::RG, key_group = wave / C::RG, column = lane & 31, hi = lane >> 5;
@@ -352,10 +357,11 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
     const int w0 = q0 + row_group * 32, i_query = w0 + column, at_query = min(i_query, nq - 1);
     half8 q[KS];
     {
-        const std::uint16_t* row = a.q + (sq.first + at_query) * a.q_stride + static_cast<std::int64_t>(head) * D + hi * 8;
+        const std::uint16_t* row = a.q + (sq.first + at_query) * a.q_stride + static_cast<std::int64_t>(head) * dim + hi * 8;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            u32x4 v = *reinterpret_cast<const u32x4*>(row + ks * 16);
+            u32x4 v = {0, 0, 0, 0};
+            if (!C::PAD || ks * 16 + hi * 8 < dim) v = *reinterpret_cast<const u32x4*>(row + ks * 16);
             if (a.negate)
                 for (int e = 0; e < 4; ++e) v[e] ^= 0x80008000u;
             q[ks] = __builtin_bit_cast(half8, v);
@@ -373,7 +379,7 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
         return (below(of_lane.to) & ~below(of_lane.from)) | below(of_lane.sinks);
     };
 
-    const std::int64_t kv = static_cast<std::int64_t>(head / a.group) * D;
+    const std::int64_t kv = static_cast<std::int64_t>(head / a.group) * dim;
     const std::uint16_t* const k0 = a.k + sk.first * a.k_stride + kv;
     const std::uint16_t* const v0 = a.v + sk.first * a.v_stride + kv;
     // A tile's DMA instructions are dealt to the waves of its group.
@@ -384,12 +390,13 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
         const std::uint64_t p = reinterpret_cast<std::uint64_t>(x + static_cast<std::int64_t>(step) * kKeys * stride);
         const int rows = min(kKeys, sk.count - step * kKeys);
         const u32x4 r = {uniform(static_cast<std::uint32_t>(p)), uniform(static_cast<std::uint32_t>(p >> 32)) & 0xffffu,
-                         uniform((rows - 1) * stride2 + 2u * D), kRawBufferFlags};
+                         uniform((rows - 1) * stride2 + 2u * dim), kRawBufferFlags};
 #pragma unroll
         for (int i = 0; i < (C::DMA + C::RG - 1) / C::RG; ++i) {
             if (C::DMA % C::RG != 0 && row_group + i * C::RG >= C::DMA) continue;
             const int t = first_row + i * C::RG * C::DMA_ROWS;
-            lds_dma16(r, to + (row_group + i * C::RG) * 1024, t * stride2 + ((lane % C::PIECES) ^ C::swizzle(t)) * 16u);
+            const unsigned piece = (lane % C::PIECES) ^ C::swizzle(t);
+            lds_dma16(r, to + (row_group + i * C::RG) * 1024, C::PAD && piece * 8 >= static_cast<unsigned>(dim) ? 1u << 31 : t * stride2 + piece * 16u);
         }
     };
     // Places of this lane's pieces: of K, pieces 2 ks + hi of row lane & 31; of
@@ -654,12 +661,16 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
 #pragma unroll 4
                 for (int j = part ? of_wave.from : 0; j < (part ? of_wave.to : of_wave.sinks); ++j) {
                     const std::uint16_t* const row = v0 + j * a.v_stride + lane * PER;
-                    std::uint32_t v;
-                    if constexpr (PER == 2) v = *reinterpret_cast<const std::uint32_t*>(row);
-                    else v = *row;
+                    std::uint32_t v[(PER + 1) / 2] = {};
+                    if (!C::PAD || lane * PER < dim) {
+#pragma unroll
+                        for (int c = 0; c < (PER + 1) / 2; ++c)
+                            if constexpr (PER >= 2) v[c] = reinterpret_cast<const std::uint32_t*>(row)[c];
+                            else v[c] = *row;
+                    }
 #pragma unroll
                     for (int c = 0; c < PER; ++c) {
-                        const unsigned kind = OddValues::of(static_cast<std::uint16_t>(v >> 16 * c));
+                        const unsigned kind = OddValues::of(static_cast<std::uint16_t>(v[c / 2] >> 16 * (c & 1)));
 #pragma unroll
                         for (int k = 0; k < 3; ++k) {
                             if (kind != 1u << k) continue;
@@ -719,12 +730,12 @@ __global__ __launch_bounds__(C::WAVES * 64, C::OCC) void prompt_kernel(PromptArg
 
     const float sum = both_sum(l), r = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (i_query >= nq) return;
-    std::uint16_t* out = a.out + (sq.first + i_query) * a.out_stride + static_cast<std::int64_t>(head) * D + 4 * hi;
+    std::uint16_t* out = a.out + (sq.first + i_query) * a.out_stride + static_cast<std::int64_t>(head) * dim + 4 * hi;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<uint2*>(out + dt * 32 + 8 * g) =
+            if (!C::PAD || dt * 32 + 8 * g < dim) *reinterpret_cast<uint2*>(out + dt * 32 + 8 * g) =
                 make_uint2(pack_rounded(acc[dt][4 * g] * r, acc[dt][4 * g + 1] * r),
                            pack_rounded(acc[dt][4 * g + 2] * r, acc[dt][4 * g + 3] * r));
 }
@@ -840,6 +851,24 @@ void launch_window(const PromptArgs& a, hipStream_t s)
     else launch_prompt<PromptCfg<D, 4, 1, 64, D == 64 ? 3 : 2>, true>(a, s);
 }
 
+// Heads of other sizes, padded to 128 or 256. us of a call, and of one wave for
+// each query, value by value, as rows off 16 bytes are taken:
+//   32640, w 1024, 16 / 4 heads of 96              345  202000
+//                                  of 256         1120
+//   240, w 80, 16 / 4 heads of 96                  9.3      67
+//                           of 256 (2,2,32)       17.4, (4,1,32) 26.0
+//   1..2040 packed, w 240 both ways, heads of 96  48.7
+template <int D>
+void launch_padded_window(const PromptArgs& a, hipStream_t s)
+{
+    const std::int64_t cus = conv::cu_count();
+    if constexpr (D > 128) {
+        if (workgroups_of(a, 64) <= cus) launch_prompt<PromptCfg<D, 2, 2, 32, 1, true>, true>(a, s);
+        else launch_prompt<PromptCfg<D, 4, 1, 32, 1, true>, true>(a, s);
+    } else if (workgroups_of(a, 64) <= 2 * cus) launch_prompt<PromptCfg<D, 2, 2, 32, 2, true>, true>(a, s);
+    else launch_prompt<PromptCfg<D, 4, 1, 64, 2, true>, true>(a, s);
+}
+
 void attention_prompt(const mlvc_hip_attention_prompt_desc* d, int window, int sinks, const char* op, hipStream_t s)
 {
     require(d != nullptr, op, "no descriptor");
@@ -877,9 +906,15 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, int window, int s
     const bool rows = vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride) && vector_rows(d->k, d->k_stride) &&
                       vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f;
     // The kernel under a window counts places in 32 bits.
-    const bool fast = rows && (!a.window || static_cast<std::int64_t>(d->q_tokens) + d->k_tokens < (std::int64_t{1} << 30));
+    const std::int64_t tokens = static_cast<std::int64_t>(d->q_tokens) + d->k_tokens;
+    const bool fast = rows && (!a.window || tokens < (std::int64_t{1} << 30));
+    const bool padded = rows && window && tokens < (std::int64_t{1} << 30) && d->head_dim % 8 == 0 && d->head_dim <= 256;
     if (fast && d->head_dim == 128) a.window ? launch_window<128>(a, s) : launch_prompt<128>(a, s);
     else if (fast && d->head_dim == 64) a.window ? launch_window<64>(a, s) : launch_prompt<64>(a, s);
+    else if (padded) {
+        a.window = static_cast<int>(std::min<std::int64_t>(window, tokens));
+        d->head_dim < 128 ? launch_padded_window<128>(a, s) : launch_padded_window<256>(a, s);
+    }
     else {
         require(launchable(d->q_tokens, 64), op, "too many sequences, heads and queries in one call");
         prompt_any_kernel<<<dim3(static_cast<unsigned>(d->q_tokens), static_cast<unsigned>(d->q_heads)), 64, 0, s>>>(a);

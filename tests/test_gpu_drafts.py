@@ -217,6 +217,8 @@ def test_window_lengths(dev, rng, queries, keys, window, sinks, dim, causal):
     (64, 4, 4, 0, 0), (128, 8, 1, 0, 0), (64, 6, 2, 64, 0), (128, 16, 1, 8, 16),
     (64, 3, 1, 1, 0), (128, 2, 2, 0, 1),                       # off 16 bytes
     (96, 3, 1, 0, 0), (33, 2, 1, 0, 0), (512, 1, 1, 0, 0),     # other heads
+    (8, 4, 2, 0, 0), (40, 6, 3, 8, 8), (120, 4, 2, 0, 0), (136, 4, 4, 0, 0), (200, 4, 2, 64, 0), (256, 2, 2, 0, 8), (264, 2, 1, 0, 0),
+    (96, 2, 2, 1, 0), (256, 2, 2, 0, 1),
 ])
 def test_window_heads_and_strides(dev, rng, dim, q_heads, kv_heads, extra, shift, causal):
     _window(dev, rng, [70, 9], [200, 9], q_heads, kv_heads, dim, causal, 40, 6, extra, shift)
@@ -235,9 +237,21 @@ def test_window_tiles(dev, rng, queries, keys, q_heads, dim, causal, window, sin
 
 
 @pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [24, 96, 160, 256])
+@pytest.mark.parametrize("queries,keys,q_heads,window,sinks", [
+    ([1, 240, 0, 65, 3], [1, 240, 7, 65, 3], 4, 33, 4), ([1, 17, 130], [300, 64, 260], 4, 100, 130), ([40, 200, 5], [7, 64, 0], 4, 1, 0),
+    ([1500], [1500], 16, 333, 70), ([1100, 40], [1100, 2000], 16, 65, 65), ([30] * 70, [100] * 70, 6, 33, 2),
+    ([300, 20], [300, 50], 4, 5000, 9),                        # wider than all there is
+])
+def test_window_padded_heads(dev, rng, queries, keys, q_heads, dim, causal, window, sinks):
+    _window(dev, rng, queries, keys, q_heads, 2, dim, causal, window, sinks)
+
+
+@pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("queries,keys,q_heads,dim,window,sinks", [
     ([70], [70], 2, 64, 20, 3), ([200, 33], [300, 33], 2, 128, 40, 70), ([900], [900], 16, 64, 31, 5), ([520], [700], 16, 128, 300, 0),
-    ([300], [300], 2, 96, 33, 2), ([1200], [1200], 16, 128, 1, 66),
+    ([300], [300], 2, 96, 33, 2), ([1200], [1200], 16, 128, 1, 66), ([400], [500], 3, 264, 33, 2),
+    ([1200], [1200], 16, 72, 40, 66), ([500, 90], [500, 300], 3, 184, 33, 5), ([700], [700], 2, 256, 100, 3),
 ])
 def test_window_of_infinite_values(dev, rng, queries, keys, q_heads, dim, window, sinks, causal):
     """Infinities and NaN among the values reach the queries that see them, and no others."""
@@ -257,7 +271,7 @@ def test_window_of_infinite_values(dev, rng, queries, keys, q_heads, dim, window
         i, j = i + nq, j + nk
 
 
-@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dim", [64, 128, 80, 232])
 def test_window_peaked_and_small_weights(dev, rng, dim):
     """Scores far apart, and many small weights beside a large one among the sinks."""
     for spread in (20.0, 0.01):
