@@ -75,6 +75,9 @@ struct View {
     }
     // First token of a step.
     __device__ int token(int step) const { return (step < sink_steps ? step : step + skipped) * kStep; }
+    // Whether no draft sees a part only of the step at token j, whose tiles are there: it ends before the drafts,
+    // before the context is cut, and not across the window's edge, behind which all drafts see from clear_from on.
+    __device__ bool whole(int j, int clear_from) const { return j + kStep <= min(past, length) && (j >= clear_from || j + kStep <= sinks); }
 };
 
 // What a draft sees.
@@ -473,7 +476,7 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
             factor[e] = KIND == MLVC_KV_F16 ? a.scale2 : ks[e >> 2][e & 3] * a.scale2;
             scale[e] = KIND == MLVC_KV_F16 ? 1.0f : __builtin_elementwise_maximum(vs[e >> 2][e & 3], 0x1p-40f);
         }
-        const bool masked = j + kStep > w.past || !there[0] || !there[1] || (j < clear_from && j + kStep > w.sinks);
+        const bool masked = !there[0] || !there[1] || !w.whole(j, clear_from);
         const bool here[2] = {there[0], there[1]};
         // The last step asks for itself again: so that there are always as many loads,
         // and the wait for K leaves V on its way.
@@ -875,7 +878,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
     auto take_turn = [&](int turn, Coming& c) {
         const int step = first + turn * KG + kg, buffer = turn & 1, j = c.j;
         const bool here0 = c.there[0], here1 = c.there[1];
-        const bool masked = j + kStep > w.past || !here0 || !here1 || (j < clear_from && j + kStep > w.sinks);
+        const bool masked = !here0 || !here1 || !w.whole(j, clear_from);
         unpack(c, buffer, masked);
         fetch(min(step + C::DEPTH * KG, last - 1), c);
         __syncthreads();
