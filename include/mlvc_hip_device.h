@@ -530,7 +530,11 @@ int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip
  * fills them, attention_drafts looks at the cache, mlvc_hip_kv_keep moves the
  * drafts that are kept behind the context and gives the lengths that the next
  * plan starts from. With a window, contexts of any age hold the pages of the
- * window and of the first `sinks` tokens only.
+ * window and of the first `sinks` tokens only. Where the pool or a table row may
+ * be too small, `placed` goes from the plan to attention_drafts and kv_keep: a
+ * stream that got no pages has no drafts there, and its context and length stay
+ * as they are until a later plan serves it. Without it they would take its last
+ * tokens for the drafts.
  *
  * Window and sinks, in all of them: a token at place p sees a token at place j
  * if p - j < window (and j - p < window in attention_window both ways) or
@@ -554,7 +558,8 @@ int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip
  *      stream by stream, from the top of the stack free_pages; the first one
  *      that the pool does not suffice for and those behind it that need a page
  *      get none (lacking counts them), nor does a stream whose tokens go beyond
- *      its table row or 2^31 - 1;
+ *      its table row or 2^31 - 1; placed[n] is the number of a stream's new
+ *      tokens that have slots, fresh[n] or for one that got no pages 0;
  *   3. lengths[n] = past[n] + fresh[n] (past[n] for a stream that got no pages),
  *      starts = 0, then the sums of fresh; token t, the i-th new one of stream
  *      n, has slots[t], the slot of place past[n] + i, and positions[t] = past[n]
@@ -584,6 +589,7 @@ typedef struct mlvc_hip_kv_plan_desc {
     int32_t* slots;                /* [tokens] */
     int32_t* positions;            /* [tokens], or NULL */
     int32_t* lacking;              /* [1] */
+    int32_t* placed;               /* [streams], or NULL; not `past`, `fresh` or `lengths` */
 } mlvc_hip_kv_plan_desc;
 int mlvc_hip_kv_plan(const mlvc_hip_kv_plan_desc* desc, mlvc_hip_stream s);
 
@@ -606,7 +612,8 @@ int mlvc_hip_attention_window(const mlvc_hip_attention_window_desc* desc, mlvc_h
  * length plus the number of other drafts that it sees. One draft a stream is the
  * ordinary step under a window. Drafts past `longest_q` or the 64th are not
  * computed, and seen by none; their rows of out stay as they are, as do those
- * past the last stream's. A draft that sees nothing gives zeros. Pages, lengths,
+ * past the last stream's. With `placed` only the first placed[n] of a stream's
+ * drafts are in the cache, and the others' rows of out stay as they are. A draft that sees nothing gives zeros. Pages, lengths,
  * infinities, the workspace and the order of sums are as in
  * mlvc_hip_attention_token; a weight of the softmax is off by at most 2^-11 of
  * itself or 2^-37 of the largest. */
@@ -628,6 +635,7 @@ typedef struct mlvc_hip_attention_drafts_desc {
     float scale;
     void* workspace;               /* 16-byte aligned; mlvc_hip_attention_drafts_workspace_bytes */
     size_t workspace_bytes;
+    const int32_t* placed;         /* [streams], device memory, or NULL: all drafts are in the cache */
 } mlvc_hip_attention_drafts_desc;
 /* Depends on streams, q_heads, longest_q, longest, window, sinks and the cache's
  * layout only (0: none needed), and grows with streams, longest_q and longest. */
@@ -637,7 +645,8 @@ int mlvc_hip_attention_drafts(const mlvc_hip_attention_drafts_desc* desc, mlvc_h
 /* Keeps a path of each stream's drafts: draft kept[n][i] moves to the i-th place
  * behind the context, its stored values and scales as they are, and
  * lengths_out[n] becomes the context's length with the kept drafts. A number
- * that is no draft of the stream (-1) ends its list. The same draft may stand
+ * that is no draft of the stream (-1) ends its list; with `placed` only the first
+ * placed[n] of its drafts are there, as the last of its tokens. The same draft may stand
  * twice. Rows whose page is not in the cache are not moved. */
 typedef struct mlvc_hip_kv_keep_desc {
     const mlvc_hip_kv_cache* cache;
@@ -648,7 +657,8 @@ typedef struct mlvc_hip_kv_keep_desc {
     const int32_t* lengths;     /* [streams], with the drafts */
     const int32_t* kept;        /* [streams][kept_stride] */
     int kept_stride;            /* 0..64 */
-    int32_t* lengths_out;       /* [streams]; not `lengths` */
+    int32_t* lengths_out;       /* [streams]; not `lengths` or `placed` */
+    const int32_t* placed;      /* [streams], device memory, or NULL: all drafts are in the cache */
 } mlvc_hip_kv_keep_desc;
 int mlvc_hip_kv_keep(const mlvc_hip_kv_keep_desc* desc, mlvc_hip_stream s);
 

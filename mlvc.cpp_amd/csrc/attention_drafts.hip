@@ -37,6 +37,7 @@ struct DraftArgs {
     const unsigned long long* seen;
     const std::int32_t* table;
     const std::int32_t* lengths;
+    const std::int32_t* placed;
     int table_stride, pages, page, heads, q_heads, group, dim, longest, longest_q, q_tokens, streams, window, sinks;
     float scale2;
     float* part;    // [heads][rows][places][dim], a row for each draft and query head of a group
@@ -56,12 +57,14 @@ struct View {
     int start, drafts, queries;  // first row of q; drafts in the cache; rows that are computed
     int past, length;            // place of the first draft; tokens in the cache
     int sinks, sink_steps, skipped, steps;
-    __device__ View(const DraftArgs& a, int stream) : View(a, a.starts[stream], a.starts[stream + 1], a.lengths[stream]) {}
-    __device__ View(const DraftArgs& a, int begin, int end, int tokens)
+    __device__ View(const DraftArgs& a, int stream)
     {
+        const int begin = a.starts[stream], end = a.starts[stream + 1];
+        int tokens = a.lengths[stream];
         const std::int64_t held = static_cast<std::int64_t>(a.table_stride) * a.page;
         start = min(max(begin, 0), a.q_tokens);
         drafts = max(end - begin, 0);
+        if (a.placed) drafts = min(drafts, max(a.placed[stream], 0));
         queries = min(min(drafts, a.longest_q), a.q_tokens - start);
         tokens = max(tokens, 0);
         past = tokens - drafts;
@@ -1241,8 +1244,8 @@ void attention_drafts(const mlvc_hip_attention_drafts_desc* d, hipStream_t s)
     if (d->streams == 0 || d->q_tokens == 0) return;
     require(d->q && d->out && d->starts && d->lengths && (d->table || d->table_stride == 0), op, "null tensor");
     require(aligned2(d->q) && aligned2(d->out), op, "a tensor is not aligned to its FP16 values");
-    require(aligned_to<8>(d->seen) && aligned_to<4>(d->starts) && aligned_to<4>(d->lengths) && aligned_to<4>(d->table), op,
-            "seen, starts, lengths or table is not aligned to its values");
+    require(aligned_to<8>(d->seen) && aligned_to<4>(d->starts) && aligned_to<4>(d->lengths) && aligned_to<4>(d->table) && aligned_to<4>(d->placed), op,
+            "seen, starts, lengths, table or placed is not aligned to its values");
     const Plan p = plan(d, vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride));
     const std::int64_t all_rows = static_cast<std::int64_t>(d->streams) * p.row_count;
     const std::int64_t items = static_cast<std::int64_t>(d->cache->heads) * (p.shares ? (p.shape == kOne4 ? 2 : 1) * p.shares : d->streams);
@@ -1259,7 +1262,7 @@ void attention_drafts(const mlvc_hip_attention_drafts_desc* d, hipStream_t s)
     a.k_scale = c->k_scale, a.v_scale = c->v_scale;
     a.q = static_cast<const std::uint16_t*>(d->q), a.out = static_cast<std::uint16_t*>(d->out);
     a.q_stride = d->q_stride, a.out_stride = d->out_stride;
-    a.starts = d->starts, a.seen = reinterpret_cast<const unsigned long long*>(d->seen), a.table = d->table, a.lengths = d->lengths;
+    a.starts = d->starts, a.seen = reinterpret_cast<const unsigned long long*>(d->seen), a.table = d->table, a.lengths = d->lengths, a.placed = d->placed;
     a.table_stride = d->table_stride, a.pages = c->pages, a.page = c->page_size, a.heads = c->heads;
     a.q_heads = d->q_heads, a.group = d->q_heads / c->heads, a.dim = c->head_dim;
     a.longest = c->pages ? d->longest : 0, a.longest_q = d->longest_q, a.q_tokens = d->q_tokens, a.streams = d->streams;

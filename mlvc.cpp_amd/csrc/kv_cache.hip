@@ -259,6 +259,7 @@ struct KeepArgs {
     const std::int32_t* starts;
     const std::int32_t* lengths;
     const std::int32_t* kept;
+    const std::int32_t* placed;
     std::int32_t* lengths_out;
     int streams, heads, row_bytes, page, pages, table_stride, kept_stride, quantised;
 };
@@ -278,7 +279,9 @@ __global__ __launch_bounds__(kBlock) void kv_keep_kernel(KeepArgs a)
     __shared__ int kept_count;
     const int head = blockIdx.x % a.heads, stream = blockIdx.x / a.heads, tid = threadIdx.x;
     if (tid < 64) {
-        const int drafts = max(a.starts[stream + 1] - a.starts[stream], 0), past = max(a.lengths[stream], 0) - drafts;
+        int drafts = max(a.starts[stream + 1] - a.starts[stream], 0);
+        if (a.placed) drafts = min(drafts, max(a.placed[stream], 0));
+        const int past = max(a.lengths[stream], 0) - drafts;
         const int draft = tid < a.kept_stride ? a.kept[static_cast<std::int64_t>(stream) * a.kept_stride + tid] : -1;
         const unsigned long long ends = ~__ballot(draft >= 0 && draft < drafts);
         const int count = ends ? __builtin_ctzll(ends) : 64;
@@ -335,8 +338,9 @@ void kv_keep(const mlvc_hip_kv_keep_desc* d, hipStream_t s)
     require(d->kept_stride >= 0 && d->kept_stride <= kMostKept, op, "kept_stride must be 0..64");
     if (d->streams == 0) return;
     require(d->starts && d->lengths && d->lengths_out && (d->kept || d->kept_stride == 0) && (d->table || d->table_stride == 0), op, "null tensor");
-    require(d->lengths_out != d->lengths && d->lengths_out != d->starts, op, "lengths_out must not be lengths or starts");
-    for (const std::int32_t* p : {d->table, d->starts, d->lengths, d->kept, static_cast<const std::int32_t*>(d->lengths_out)})
+    require(d->lengths_out != d->lengths && d->lengths_out != d->starts && d->lengths_out != d->placed, op,
+            "lengths_out must not be lengths, starts or placed");
+    for (const std::int32_t* p : {d->table, d->starts, d->lengths, d->kept, d->placed, static_cast<const std::int32_t*>(d->lengths_out)})
         require(aligned_to<4>(p), op, "a tensor is not aligned to its values");
     const mlvc_hip_kv_cache* c = d->cache;
     const std::int64_t grid = static_cast<std::int64_t>(d->streams) * c->heads;
@@ -344,7 +348,7 @@ void kv_keep(const mlvc_hip_kv_keep_desc* d, hipStream_t s)
     KeepArgs a{};
     a.cache[0] = static_cast<std::uint8_t*>(c->k), a.cache[1] = static_cast<std::uint8_t*>(c->v);
     a.scale[0] = c->k_scale, a.scale[1] = c->v_scale;
-    a.table = d->table, a.starts = d->starts, a.lengths = d->lengths, a.kept = d->kept, a.lengths_out = d->lengths_out;
+    a.table = d->table, a.starts = d->starts, a.lengths = d->lengths, a.kept = d->kept, a.placed = d->placed, a.lengths_out = d->lengths_out;
     a.streams = d->streams, a.heads = c->heads, a.page = c->page_size, a.pages = c->pages, a.table_stride = d->table_stride;
     a.kept_stride = d->kept_stride, a.quantised = c->kind != MLVC_KV_F16;
     a.row_bytes = c->head_dim * (a.quantised ? 1 : 2);

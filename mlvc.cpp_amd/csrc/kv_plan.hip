@@ -37,6 +37,7 @@ struct PlanArgs {
     std::int32_t* slots;
     std::int32_t* positions;
     std::int32_t* lacking;
+    std::int32_t* placed;
 };
 
 __device__ __forceinline__ int pages_of(const PlanArgs& a, std::int64_t tokens)
@@ -232,6 +233,7 @@ __global__ __launch_bounds__(kMostThreads) void plan_kernel(PlanArgs a)
         if ((tid & 63) == 0 && short_of) atomicAdd(&lacking_here, __popcll(short_of));
         if (n < a.streams) {
             a.lengths[n] = r.past + (served ? r.fresh : 0);
+            if (a.placed) a.placed[n] = served ? r.fresh : 0;
             a.starts[n + 1] = capped(tokens + sums.c);
             a.held[n] = make_int2(r.front, r.back + got);
         }
@@ -296,10 +298,11 @@ void kv_plan(const mlvc_hip_kv_plan_desc* d, hipStream_t s)
     require(d->held && d->free_count && d->past && d->fresh && d->lengths && d->starts && d->lacking && (d->slots || d->tokens == 0) &&
                 (d->table || d->streams == 0 || d->table_stride == 0) && (d->free_pages || d->pages == 0), op, "null tensor");
     require(d->lengths != d->past && d->lengths != d->fresh, op, "lengths must not be past or fresh");
+    require(!d->placed || (d->placed != d->past && d->placed != d->fresh && d->placed != d->lengths), op, "placed must not be past, fresh or lengths");
     for (const void* p : {static_cast<const void*>(d->table), static_cast<const void*>(d->free_pages), static_cast<const void*>(d->free_count),
                           static_cast<const void*>(d->past), static_cast<const void*>(d->fresh), static_cast<const void*>(d->lengths),
                           static_cast<const void*>(d->starts), static_cast<const void*>(d->slots), static_cast<const void*>(d->positions),
-                          static_cast<const void*>(d->lacking)})
+                          static_cast<const void*>(d->lacking), static_cast<const void*>(d->placed)})
         require(aligned_to<4>(p), op, "a tensor is not aligned to its values");
     require(aligned_to<8>(d->held) && aligned_to<8>(d->seen), op, "held and seen must be 8-byte aligned");
     PlanArgs a{};
@@ -308,7 +311,7 @@ void kv_plan(const mlvc_hip_kv_plan_desc* d, hipStream_t s)
     a.table = d->table, a.table_stride = d->table_stride, a.held = reinterpret_cast<int2*>(d->held);
     a.free_pages = d->free_pages, a.free_count = d->free_count, a.past = d->past, a.fresh = d->fresh;
     a.seen = reinterpret_cast<const unsigned long long*>(d->seen);
-    a.lengths = d->lengths, a.starts = d->starts, a.slots = d->slots, a.positions = d->positions, a.lacking = d->lacking;
+    a.lengths = d->lengths, a.starts = d->starts, a.slots = d->slots, a.positions = d->positions, a.lacking = d->lacking, a.placed = d->placed;
     // A stream a thread, and enough of them for the pages and the tokens.
     const std::int64_t work = std::max<std::int64_t>(d->streams, d->tokens / 4);
     const int threads = static_cast<int>(std::min<std::int64_t>(kMostThreads, std::max<std::int64_t>(64, (work + 63) / 64 * 64)));

@@ -466,7 +466,7 @@ class KvPlan(C.Structure):
     _fields_ = [(f, C.c_int) for f in ("streams", "pages", "page_size", "tokens", "window", "sinks")] + [
         ("table", C.c_void_p), ("table_stride", C.c_int)] + [
         (f, C.c_void_p) for f in ("held", "free_pages", "free_count", "past", "fresh", "seen", "lengths", "starts", "slots",
-                                  "positions", "lacking")]
+                                  "positions", "lacking", "placed")]
 
 
 class WindowAttention(C.Structure):
@@ -480,14 +480,14 @@ class DraftAttention(C.Structure):
         ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("starts", C.c_void_p),
         ("seen", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int), ("lengths", C.c_void_p)] + [
         (f, C.c_int) for f in ("longest", "window", "sinks")] + [
-        ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+        ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("placed", C.c_void_p)]
 
 
 class KvKeep(C.Structure):
     """mlvc_hip_kv_keep_desc; keep the KvCache that `cache` points to."""
     _fields_ = [("cache", C.POINTER(KvCache)), ("streams", C.c_int), ("table", C.c_void_p), ("table_stride", C.c_int),
                 ("starts", C.c_void_p), ("lengths", C.c_void_p), ("kept", C.c_void_p), ("kept_stride", C.c_int),
-                ("lengths_out", C.c_void_p)]
+                ("lengths_out", C.c_void_p), ("placed", C.c_void_p)]
 
 
 def _bind_attention(lib) -> None:

@@ -96,3 +96,13 @@ def test_nothing_to_do(call):
 def test_workspace_of_refused_descriptor_is_zero():
     c = cache(kind=7)
     assert mlvc_hip.attention_drafts_workspace_bytes(mlvc_hip.DraftAttention(cache=C.pointer(c), streams=1, q_heads=2, longest_q=1)) == 0
+
+
+@pytest.mark.parametrize("call,message", [
+    (plan(placed=A), "placed must not be"), (plan(placed=A + 64), "placed must not be"), (plan(placed=A + 128), "placed must not be"),
+    (plan(placed=A + 258), "aligned"), (drafts(placed=A + 2), "aligned"), (keep(placed=A + 2), "aligned"),
+    (keep(placed=A + 128), "lengths_out must not be"),
+])
+def test_refused_placed(call, message):
+    with pytest.raises(mlvc_hip.MlvcError, match=message):
+        call()

@@ -1,13 +1,16 @@
 """Drafts where a context, a list or a number ends: cuts, drafts that do not
 count, pages that ran out, the last lengths and the largest scores."""
 
+import ctypes as C
+
 import numpy as np
 import pytest
 
+import mlvc_hip
 from devmem import Dev
-from drafts import Contexts, Drafts, drafts_seen, masked64, tops_of, tree
+from drafts import Contexts, Drafts, Plan, drafts_seen, masked64, tops_of, tree
 from mlvc_hip import KV_E4M3, KV_F16, KV_INT8
-from tokens import Cache, f64, stored64, within
+from tokens import Cache, Padded, f64, stored64, within
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +72,169 @@ def test_tokens_past_longest_are_not_seen(dev, rng, kind, q_heads, heads, dim, c
                 seen = drafts_seen(n, trees[i], window, 4)[:, :cut]
                 check(got[at:at + count], q[at:at + count], ctx.k[i][:cut], ctx.v[i][:cut], kind, dim ** -0.5, seen, f"stream {i} cut at {cut}")
             at += count
+
+
+# ------------------------------------------------------------ pages that ran out
+
+@pytest.mark.parametrize("streams", [1, 64, 70, 1100])
+def test_plan_tells_what_is_placed(dev, rng, streams):
+    """Of a short pool and of short rows, also where the streams take several turns."""
+    plan = Plan(dev, streams, 2 * streams, 16, 3, order=rng.permutation(2 * streams))
+    placed = dev.put(np.full(streams + 1, 77, np.int32))
+    length = np.zeros(streams, int)
+    short = 0
+    for _ in range(5):
+        fresh = rng.integers(-1, 30, streams)
+        total = int(fresh.clip(0).sum())
+        desc = plan.desc(length.tolist(), fresh.tolist(), total)
+        desc.placed = placed
+        mlvc_hip.kv_plan(desc)
+        want = plan.host(length.tolist(), fresh.tolist(), total)
+        plan.compare(want, total)
+        got = dev.get(placed, (streams + 1,), np.int32)
+        past = np.where(fresh < 0, 0, length)
+        assert got[-1] == 77 and np.array_equal(got[:-1], np.array(want["lengths"]) - past)
+        short += want["lacking"]
+        length = np.array(want["lengths"])
+    assert short or streams == 1
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 96, 264])
+def test_first_drafts_alone_are_placed(dev, rng, kind, dim):
+    """`placed` below the drafts of starts: those behind are not computed; above: no more than there are."""
+    counts, placed, lengths = [7, 70, 3, 5, 4], [3, 66, 0, 9, -2], [40, 100, 41, 5, 1300]
+    ctx = Contexts(dev, rng, Cache, kind, 1, dim, 16, lengths)
+    here = [min(max(p, 0), n) for p, n in zip(placed, counts)]
+    trees = [tree(rng, min(n, 64)) + [0] * max(n - 64, 0) for n in counts]
+    q = normal(rng, sum(counts), 2, dim)
+    d = Drafts(ctx.cache, q, counts, [m for t in trees for m in t], ctx.table, lengths, 0.1, longest_q=64)
+    d.desc.placed = dev.put(np.array(placed, np.int32))
+    got, at = d.run(), 0
+    for i, (count, n) in enumerate(zip(counts, lengths)):
+        done = min(here[i], 64)
+        seen = np.zeros((done, n), bool)
+        for r in range(done):
+            for j in range(n):
+                e = j - (n - here[i])
+                seen[r, j] = e < 0 or (e < 64 and trees[i][r] >> e & 1)
+        check(got[at:at + done], q[at:at + done], ctx.k[i], ctx.v[i], kind, 0.1, seen, f"stream {i}")
+        assert np.isnan(got[at + done:at + count]).all()
+        at += count
+    new = dev.put(np.full(6, 77, np.int32))
+    kept = np.array([[2, 3], [65, 66], [0, 1], [1, 4], [0, 1]], np.int32)
+    mlvc_hip.kv_keep(mlvc_hip.KvKeep(cache=C.pointer(ctx.cache.desc), streams=5, table=d.desc.table, table_stride=d.desc.table_stride,
+                                     starts=d.desc.starts, lengths=d.lengths, kept=dev.put(kept), kept_stride=2, lengths_out=new,
+                                     placed=d.desc.placed))
+    assert dev.get(new, (6,), np.int32).tolist() == [38, 35, 41, 2, 1300, 77]
+    moved = [{37: 39}, {34: 99}, {}, {0: 1, 1: 4}, {}]
+    for i, n in enumerate(lengths):
+        order = np.array([moved[i].get(j, j) for j in range(n)])
+        for g, x in zip(ctx.cache.read(ctx.slots(i, np.arange(n))), (ctx.k[i], ctx.v[i])):
+            want = stored64(x, kind)[order]
+            within(g, want, np.abs(want) * (2.0 ** -11 + 2.0 ** -23) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("pages,width,window,sinks", [
+    (7, 40, 0, 0),      # a pool for fewer tokens than the streams take
+    (9, 40, 40, 5),     # the same behind a window
+    (40, 3, 0, 0),      # rows of 48 tokens, pages enough
+])
+def test_loop_that_runs_out_of_pages(dev, rng, kind, pages, width, window, sinks):
+    """Plan, write, attend to and keep drafts, captured once and replayed: a stream that gets no pages keeps its
+    rows, its length and its rows of out, and goes on once pages are there again."""
+    streams, heads, q_heads, dim, page, most = 4, 2, 4, 64, 16, 8
+    plan = Plan(dev, streams, pages, page, width, window, sinks, rng.permutation(pages))
+    cache = Cache(dev, kind, pages, page, heads, dim)
+    put = lambda shape, t: dev.put(np.zeros(shape, t))  # noqa: E731
+    tokens = streams * most
+    past, fresh, kept, seen, placed = put(streams, np.int32), put(streams, np.int32), put((streams, most), np.int32), put(tokens, np.uint64), put(streams, np.int32)
+    x = np.zeros((tokens, heads, dim), np.float16)
+    q, k, v = Padded(dev, np.zeros((tokens, q_heads, dim), np.float16)), Padded(dev, x), Padded(dev, x)
+    out = Padded(dev, np.full((tokens, q_heads, dim), np.nan, np.float16))
+    pd = plan.desc(past, fresh, tokens, seen)
+    pd.placed = placed
+    rows = mlvc_hip.KvRows(tokens=tokens, k=k.at, v=v.at, k_stride=k.stride, v_stride=v.stride, slots=plan.slots)
+    ad = mlvc_hip.DraftAttention(cache=C.pointer(cache.desc), streams=streams, q_heads=q_heads, q_tokens=tokens, longest_q=most,
+                                 q=q.at, out=out.at, q_stride=q.stride, out_stride=out.stride, starts=plan.d_starts, seen=seen,
+                                 table=plan.d_table, table_stride=width, lengths=plan.d_lengths, longest=width * page,
+                                 window=window, sinks=sinks, scale=0.125, placed=placed)
+    ad.workspace_bytes = mlvc_hip.attention_drafts_workspace_bytes(ad)
+    if ad.workspace_bytes:
+        ad.workspace = dev.put(np.full(ad.workspace_bytes, 0xFF, np.uint8))
+    kd = mlvc_hip.KvKeep(cache=C.pointer(cache.desc), streams=streams, table=plan.d_table, table_stride=width, starts=plan.d_starts,
+                         lengths=plan.d_lengths, kept=kept, kept_stride=most, lengths_out=past, placed=placed)
+    stream, graph = C.c_void_p(), C.c_void_p()
+    dev.check(dev.lib.mlvc_hip_stream_synchronize(None))
+    dev.check(dev.lib.mlvc_hip_stream_create(C.byref(stream)))
+    dev.check(dev.lib.mlvc_hip_capture_begin(stream))
+    mlvc_hip.kv_plan(pd, stream)
+    mlvc_hip.kv_write(cache.desc, rows, stream)
+    mlvc_hip.attention_drafts(ad, stream)
+    mlvc_hip.kv_keep(kd, stream)
+    dev.check(dev.lib.mlvc_hip_capture_end(stream, C.byref(graph)))
+
+    def set_(at, a):
+        a = np.ascontiguousarray(a)
+        dev.check(dev.lib.mlvc_hip_memcpy_h2d(at, a.ctypes.data, a.nbytes, stream))
+        dev.check(dev.lib.mlvc_hip_stream_synchronize(stream))
+
+    length, refused, again, waits = [0] * streams, 0, 0, set()
+    held_k, held_v = [np.zeros((0, heads, dim), np.float16) for _ in range(streams)], [np.zeros((0, heads, dim), np.float16) for _ in range(streams)]
+    for step in range(40):
+        counts = [int(rng.integers(1, most + 1)) for _ in range(streams)]
+        if step % 9 == 8:                       # one ends, its pages go to those that wait
+            i = int(np.argmax(length))
+            counts[i], length[i] = -1, 0
+            held_k[i] = held_v[i] = held_k[i][:0]
+            waits.discard(i)
+        trees = [tree(rng, max(n, 0), 3) for n in counts]
+        n_new = sum(max(n, 0) for n in counts)
+        qn, kn, vn = normal(rng, tokens, q_heads, dim), normal(rng, tokens, heads, dim), normal(rng, tokens, heads, dim)
+        paths = np.full((streams, most), -1, np.int32)
+        for i, t in enumerate(trees):
+            if t:
+                leaf = int(rng.integers(0, len(t)))
+                path = [j for j in range(len(t)) if t[leaf] >> j & 1]
+                paths[i, :len(path)] = path
+        masks = np.array([m for t in trees for m in t] + [0] * (tokens - n_new), np.uint64)
+        set_(fresh, np.array(counts, np.int32))
+        set_(kept, paths)
+        set_(seen, masks)
+        for p, a in ((q, qn), (k, kn), (v, vn)):
+            set_(p.base, np.concatenate([a.reshape(-1).view(np.uint16), np.full(8, 0x7E00, np.uint16)]))
+        set_(out.base, np.full(out.n, 0x7E00, np.uint16))
+        dev.check(dev.lib.mlvc_hip_graph_launch(graph, stream))
+        dev.check(dev.lib.mlvc_hip_stream_synchronize(stream))
+        want = plan.host(length, counts, tokens, masks)
+        plan.compare(want, tokens)
+        got, at = out.get(), 0
+        for i, t in enumerate(trees):
+            n = len(t)
+            if n and want["lengths"][i] == length[i]:
+                assert np.isnan(got[at:at + n]).all()
+                refused += 1
+                waits.add(i)
+            elif n:
+                again += i in waits
+                waits.discard(i)
+                kk, vv = np.concatenate([held_k[i], kn[at:at + n]]), np.concatenate([held_v[i], vn[at:at + n]])
+                check(got[at:at + n], qn[at:at + n], kk, vv, kind, 0.125, drafts_seen(length[i] + n, t, window, sinks), f"step {step}, stream {i}")
+                path = [d for d in paths[i] if d >= 0]
+                held_k[i], held_v[i] = np.concatenate([held_k[i], kn[at:at + n][path]]), np.concatenate([held_v[i], vn[at:at + n][path]])
+                length[i] += len(path)
+            at += n
+            places = np.arange(length[i])
+            if window:
+                places = places[(places < sinks) | (places > length[i] - window)]
+            if places.size:
+                slots = np.array(plan.table[i])[places // page] * page + places % page
+                for g, a in zip(cache.read(slots), (held_k[i], held_v[i])):
+                    stored = stored64(a, kind)[places]
+                    within(g, stored, np.abs(stored) * (2.0 ** -11 + 2.0 ** -23) + 2.0 ** -25, f"rows of stream {i} after step {step}")
+        assert np.isnan(got[n_new:]).all()
+        assert dev.get(past, (streams,), np.int32).tolist() == length
+    assert refused and again
+    dev.check(dev.lib.mlvc_hip_graph_destroy(graph))
+    dev.check(dev.lib.mlvc_hip_stream_destroy(stream))
