@@ -104,7 +104,8 @@ struct Sight {
 // Masks and depths of a stream's drafts, one a lane.
 __device__ __forceinline__ unsigned long long mask_of(const DraftArgs& a, const View& w, int draft)
 {
-    const unsigned long long there = w.drafts < 64 ? (1ull << w.drafts) - 1 : ~0ull;
+    const int count = min(w.drafts, a.longest_q);  // those behind are seen by none
+    const unsigned long long there = count < 64 ? (1ull << count) - 1 : ~0ull;
     if (!a.seen || w.start + draft >= a.q_tokens || draft >= w.drafts) return there & (2ull << draft) - 1;
     return a.seen[w.start + draft] & there;
 }

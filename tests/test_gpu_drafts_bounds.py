@@ -8,7 +8,7 @@ import pytest
 
 import mlvc_hip
 from devmem import Dev
-from drafts import Contexts, Drafts, Plan, drafts_seen, masked64, tops_of, tree
+from drafts import ALL, Contexts, Drafts, Plan, depths, drafts_seen, masked64, tops_of, tree
 from mlvc_hip import KV_E4M3, KV_F16, KV_INT8
 from tokens import Cache, Padded, f64, stored64, within
 
@@ -238,3 +238,34 @@ def test_loop_that_runs_out_of_pages(dev, rng, kind, pages, width, window, sinks
     assert refused and again
     dev.check(dev.lib.mlvc_hip_graph_destroy(graph))
     dev.check(dev.lib.mlvc_hip_stream_destroy(stream))
+
+
+# ------------------------------------------------------------ drafts that do not count
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("q_heads,heads,dim", [(4, 2, 64), (12, 1, 128), (40, 2, 64), (4, 2, 96), (2, 1, 264)])
+@pytest.mark.parametrize("window", [0, 3, 40])
+def test_drafts_past_longest_q_are_not_seen(dev, rng, kind, q_heads, heads, dim, window):
+    """Masks that are no tree, with bits of drafts at longest_q and behind it: these add neither keys nor depth."""
+    counts, lengths, longest_q = [9, 70, 3, 5], [60, 100, 41, 5], 3
+    ctx = Contexts(dev, rng, Cache, kind, heads, dim, 16, lengths)
+    masks = [0b010000001, 0b111, 0b101100100, 1 << 7, ALL, ALL] + [ALL] * (sum(counts) - 6)
+    q = normal(rng, sum(counts), q_heads, dim)
+    got = Drafts(ctx.cache, q, counts, masks, ctx.table, lengths, dim ** -0.5, window, 2, longest_q=longest_q).run()
+    at = 0
+    for i, (count, n) in enumerate(zip(counts, lengths)):
+        past, here = n - count, [m & (1 << min(count, longest_q)) - 1 for m in masks[at:at + min(count, longest_q)]]
+        depth = depths(here, longest_q)
+        seen = np.zeros((len(here), n), bool)
+        for r, m in enumerate(here):
+            place = past + depth[r]
+            for j in range(n):
+                d = j - past
+                if d < 0:
+                    seen[r, j] = not window or place - j < window or j < 2
+                elif d < len(here):
+                    seen[r, j] = m >> d & 1 and (not window or depth[r] - depth[d] < window or past + depth[d] < 2)
+        done = len(here)
+        check(got[at:at + done], q[at:at + done], ctx.k[i], ctx.v[i], kind, dim ** -0.5, seen, f"stream {i}")
+        assert np.isnan(got[at + done:at + count]).all()
+        at += count
