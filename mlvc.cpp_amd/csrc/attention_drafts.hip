@@ -101,6 +101,17 @@ struct Sight {
     }
 };
 
+// A score and the logarithm of its row's scale, for the base. FP32 numbers of 2^28
+// and more are 32 and more apart: a sum that falls so far below the exact one that
+// the weight, 2^(score - sum) scale, would not fit FP16 gives way to the score, which
+// is above the exact one (scales of 2^15 and more do not come from FP16 rows).
+__device__ __forceinline__ float with_scale(float score, float scale)
+{
+#pragma clang fp contract(off) reassociate(off)
+    const float log = __builtin_amdgcn_logf(scale), sum = score + log;
+    return score - sum + log > kMost ? score : sum;
+}
+
 // Masks and depths of a stream's drafts, one a lane.
 __device__ __forceinline__ unsigned long long mask_of(const DraftArgs& a, const View& w, int draft)
 {
@@ -535,7 +546,7 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
             if (__any(top > 0x1p15f)) {
                 top = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, KIND == MLVC_KV_F16 ? x[e] : x[e] + __builtin_amdgcn_logf(scale[e]));
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, KIND == MLVC_KV_F16 ? x[e] : with_scale(x[e], scale[e]));
                 const float now = fmaxf(base[b], lifted(column_max(top))), keep = __builtin_amdgcn_exp2f(base[b] - now);
                 l[b] *= keep;
 #pragma unroll
@@ -850,7 +861,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
         if (__any(top > 0x1p15f)) {
             top = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, KIND == MLVC_KV_F16 ? x[r] : x[r] + __builtin_amdgcn_logf(scale[r]));
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, KIND == MLVC_KV_F16 ? x[r] : with_scale(x[r], scale[r]));
             const float now = fmaxf(base, lifted(both_max(top))), keep = __builtin_amdgcn_exp2f(base - now);
             l *= keep;
 #pragma unroll

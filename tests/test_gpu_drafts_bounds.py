@@ -269,3 +269,39 @@ def test_drafts_past_longest_q_are_not_seen(dev, rng, kind, q_heads, heads, dim,
         check(got[at:at + done], q[at:at + done], ctx.k[i], ctx.v[i], kind, dim ** -0.5, seen, f"stream {i}")
         assert np.isnan(got[at + done:at + count]).all()
         at += count
+
+
+# ------------------------------------------------------------ the largest scores
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("q_heads,drafts,dim", [(2, 3, 64), (4, 8, 128), (6, 40, 128), (4, 64, 64), (3, 9, 96), (2, 40, 256), (2, 9, 512)])
+@pytest.mark.parametrize("power", [8, 10, 11, 12, 13, 14])
+def test_drafts_of_small_values_at_large_scores(dev, rng, kind, q_heads, drafts, dim, power):
+    """Scores of 2^24 to 2^30, one key far above the others, on rows of V that are zero or far smaller than the others'.
+
+    The best keys weigh 1 / count each and the others nothing (scores are 2^16 apart and more), so the result is the
+    best rows' mean: a weight times its row's scale is rounded to FP16 (2^-11 of it, the scales 2^-16 are exact; scales
+    below 2^-30 may be lost, with values up to 2^-24), the output once more."""
+    n = 260
+    level = {KV_E4M3: 448.0, KV_INT8: 127.0}.get(kind, 127.0)
+    ctx = Contexts(dev, rng, Cache, kind, 1, dim, 16, [n])
+    k = np.zeros((n, 1, dim), np.float16)
+    k[:, 0, 0] = rng.permutation(n) + 1
+    k[:, 0, 1] = n
+    q = np.zeros((drafts, q_heads, dim), np.float16)
+    q[..., 0] = 256 - np.arange(q_heads)
+    masks, sk = tree(rng, drafts), stored64(k, kind)
+    seen = drafts_seen(n, masks, 0, 0)
+    order = np.argsort(k[:, 0, 0].astype(np.float64))
+    for small in (0.0, 2.0 ** -24, level * 2.0 ** -16):
+        v = ctx.v[0].copy()
+        v[order[n // 2:]] = np.sign(v[order[n // 2:]]) * np.float16(small)
+        ctx.cache.write(k, v, ctx.slots(0, np.arange(n)))
+        got = Drafts(ctx.cache, q, [drafts], masks, ctx.table, [n], 2.0 ** power).run()
+        sv = stored64(v, kind)
+        for i in range(drafts):
+            see = np.flatnonzero(seen[i])
+            best = see[sk[see, 0, 0] == sk[see, 0, 0].max()]
+            tol = np.abs(sv[best, 0]).max(0) * 2.0 ** -9 + 2.0 ** -23
+            for h in range(q_heads):
+                within(got[i, h], sv[best, 0].mean(0), tol, f"draft {i}, values of {small}")
