@@ -8,6 +8,9 @@ namespace mlvc_hip {
 
 constexpr int kStep = 32;  // tokens of a step
 
+// Steps of so many tokens; a context may have 2^31 - 1.
+__device__ __forceinline__ int steps_for(int tokens) { return tokens / kStep + (tokens % kStep != 0); }
+
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
 // The shares of a key head's steps: `shares` large ones, all on the GPU at

@@ -71,8 +71,8 @@ struct View {
         length = static_cast<int>(min(static_cast<std::int64_t>(min(tokens, a.longest)), held));
         const int first = a.window ? first_seen(past, a.window) / kStep : 0;
         sinks = a.window ? min(a.sinks, length) : 0;
-        sink_steps = (sinks + kStep - 1) / kStep;
-        const int all = (length + kStep - 1) / kStep;
+        sink_steps = steps_for(sinks);
+        const int all = steps_for(length);
         skipped = max(min(first, all) - sink_steps, 0);
         steps = queries > 0 ? all - skipped : 0;
     }
@@ -80,7 +80,7 @@ struct View {
     __device__ int token(int step) const { return (step < sink_steps ? step : step + skipped) * kStep; }
     // Whether no draft sees a part only of the step at token j, whose tiles are there: it ends before the drafts,
     // before the context is cut, and not across the window's edge, behind which all drafts see from clear_from on.
-    __device__ bool whole(int j, int clear_from) const { return j + kStep <= min(past, length) && (j >= clear_from || j + kStep <= sinks); }
+    __device__ bool whole(int j, int clear_from) const { return min(past, length) - j >= kStep && (j >= clear_from || sinks - j >= kStep); }
 };
 
 // What a draft sees.
@@ -294,8 +294,8 @@ struct Tiles {
         const int tile = token / 16;
         if (static_cast<unsigned>(tile - first) >= 64u) {
             first = tile;
-            const int at = token + 16 * static_cast<int>(threadIdx.x & 63);
-            mine = at < w.length ? token_row(a, stream, head, at) : -1;
+            const int ahead = 16 * static_cast<int>(threadIdx.x & 63);
+            mine = ahead < w.length - token ? token_row(a, stream, head, token + ahead) : -1;
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {

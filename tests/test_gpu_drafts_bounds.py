@@ -305,3 +305,52 @@ def test_drafts_of_small_values_at_large_scores(dev, rng, kind, q_heads, drafts,
             tol = np.abs(sv[best, 0]).max(0) * 2.0 ** -9 + 2.0 ** -23
             for h in range(q_heads):
                 within(got[i, h], sv[best, 0].mean(0), tol, f"draft {i}, values of {small}")
+
+
+# ------------------------------------------------------------ the last lengths
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("q_heads,dim,most,longest,window,sinks", [
+    (4, 64, 4, (1 << 31) - 1, 50, 20),      # whole contexts: 16 rows, 64, padded, value by value
+    (4, 128, 30, (1 << 31) - 1, 300, 0),
+    (2, 96, 9, (1 << 31) - 1, 50, 20),
+    (2, 264, 3, (1 << 31) - 1, 50, 20),
+    (4, 64, 4, (1 << 31) - 1, 2500, 70),    # cut over workgroups
+    (4, 128, 40, (1 << 31) - 1, 2500, 70),
+    (2, 96, 9, (1 << 31) - 1, 2500, 70),
+    (2, 264, 3, (1 << 31) - 1, 2100, 7),
+    (4, 64, 4, (1 << 31) - 40, 300, 20),    # a cut before the last of them
+])
+def test_drafts_of_lengths_at_31_bits(dev, rng, kind, q_heads, dim, most, longest, window, sinks):
+    """Contexts that end at 2^31 - 1 and a little before it, on pages of 2^16 tokens; what the window does not reach is on no page."""
+    last, page, width = (1 << 31) - 1, 1 << 16, 1 << 15
+    lengths, counts = [last, last - 20, 300, last - 31, last - 32, last - 1000], [most, 1, 2, 3, most, 2]
+    cache = Cache(dev, kind, 3, page, 1, dim)
+    table = np.full((len(lengths), width), -1, np.int32)
+    table[:, 0], table[:, -1] = 1, 2        # sinks and the last tokens, the same for all streams
+    k, v = normal(rng, 4096, 1, dim), normal(rng, 4096, 1, dim)
+    at_end = np.arange(last - 4000, last)   # places of rows 96 ..
+    cache.write(k[:96], v[:96], page + np.arange(96))
+    cache.write(k[96:], v[96:], 2 * page + at_end % page)
+    table[2, 0] = 2                         # the short one: the first rows of the last page's end, none of its window
+    q = normal(rng, sum(counts), q_heads, dim)
+    trees = [tree(rng, n) for n in counts]
+    d = Drafts(cache, q, counts, [m for t in trees for m in t], table, lengths, dim ** -0.5, window, sinks, longest=longest)
+    got, at = d.run(), 0
+    for i, (count, n) in enumerate(zip(counts, lengths)):
+        if i == 2:                          # rows that were never written
+            at += count
+            continue
+        past, depth = n - count, depths(trees[i], count)
+        places = np.concatenate([np.arange(sinks), np.arange(max(n - window - 100, last - 4000), min(n, longest))])
+        rows = np.concatenate([np.arange(sinks), places[sinks:] - (last - 4000) + 96])
+        seen = np.zeros((count, len(places)), bool)
+        for r in range(count):
+            place = past + depth[r]
+            e = places - past
+            other = past + np.array(depth)[np.clip(e, 0, count - 1)]
+            at_place = np.where(e >= 0, other, places)
+            mask = np.array([trees[i][r] >> b & 1 for b in range(count)], bool)[np.clip(e, 0, count - 1)]
+            seen[r] = ((e < 0) | mask) & ((place - at_place < window) | (at_place < sinks))
+        check(got[at:at + count], q[at:at + count], k[rows], v[rows], kind, dim ** -0.5, seen, f"stream {i}")
+        at += count
