@@ -46,7 +46,7 @@ __device__ __forceinline__ int context(const TokenArgs& a, int stream)
 
 __device__ __forceinline__ int steps_of(const TokenArgs& a, int stream)
 {
-    return stream < a.streams ? (context(a, stream) + kStep - 1) / kStep : 0;
+    return stream < a.streams ? steps_for(context(a, stream)) : 0;
 }
 
 // Calls fn(stream, first, last, whole, slot) for each piece [first, last) of a
@@ -58,10 +58,9 @@ __device__ __forceinline__ void each_piece(const TokenArgs& a, int share, F&& fn
     const int lane = threadIdx.x & 63;
     // 64 streams at a time, one a lane: tokens, and steps up to its end.
     auto tokens = [&](int b) { return b + lane < a.streams ? context(a, b + lane) : 0; };
-    auto steps = [](int n) { return (n + kStep - 1) / kStep; };
-    int block = 0, n = tokens(0), upto = wave_scan(steps(n));
+    int block = 0, n = tokens(0), upto = wave_scan(steps_for(n));
     int total = __builtin_amdgcn_readlane(upto, 63);
-    for (int b = 64; b < a.streams; b += 64) total += wave_sum(steps(tokens(b)));
+    for (int b = 64; b < a.streams; b += 64) total += wave_sum(steps_for(tokens(b)));
     total = __builtin_amdgcn_readfirstlane(total);
     const Shares shares(a.shares, total);
     if (share >= 2 * shares.count || (share >= shares.count && shares.large == total)) return;
@@ -72,15 +71,15 @@ __device__ __forceinline__ void each_piece(const TokenArgs& a, int share, F&& fn
         const int before = __builtin_amdgcn_readlane(upto, 63);
         block += 64;
         n = tokens(block);
-        upto = before + wave_scan(steps(n));
+        upto = before + wave_scan(steps_for(n));
     };
     unsigned long long past;
     while (!(past = __ballot(upto > at))) next_block();  // at < total: some stream holds it
     int i = __builtin_ctzll(past);
     for (;;) {
-        const int mine = __builtin_amdgcn_readlane(n, i), stop = __builtin_amdgcn_readlane(upto, i), start = stop - steps(mine);
+        const int mine = __builtin_amdgcn_readlane(n, i), stop = __builtin_amdgcn_readlane(upto, i), start = stop - steps_for(mine);
         const int to = min(end, stop);
-        if (to > at) fn(block + i, (at - start) * kStep, min(mine, (to - start) * kStep), to - at == stop - start, share + block + i);
+        if (to > at) fn(block + i, (at - start) * kStep, to == stop ? mine : (to - start) * kStep, to - at == stop - start, share + block + i);
         at = max(at, to);
         if (at >= end) return;
         if (++i == 64) next_block(), i = 0;
@@ -128,9 +127,8 @@ __global__ __launch_bounds__(64) void token_any_kernel(TokenArgs a)
         for (int d = lane; d < a.dim; d += 64) qs[d] = h2f(q[d]) * a.scale2;
         __syncthreads();
         float acc[kColumns] = {}, m = -INFINITY, l = 0.0f;
-        for (int j0 = first; j0 < last; j0 += 64) {
-            const int j = j0 + lane;
-            const long long row = j < last ? token_row(a, stream, head / a.group, j) : -1;
+        for (int left = last - first; left > 0; left -= 64) {
+            const long long row = lane < left ? token_row(a, stream, head / a.group, last - left + lane) : -1;
             float s = -INFINITY;
             if (row >= 0) {
                 s = 0.0f;
@@ -146,7 +144,7 @@ __global__ __launch_bounds__(64) void token_any_kernel(TokenArgs a)
             ps[lane] = p;
             at[lane] = row;
             __syncthreads();
-            const int count = min(64, last - j0);
+            const int count = min(64, left);
 #pragma unroll
             for (int c = 0; c < kColumns; ++c) {
                 const int d = c * 64 + lane;
@@ -250,10 +248,10 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
     // A share's piece is cut into a run of steps for each wave. A whole context
     // is dealt step by step, so that a wave's first step does not depend on the
     // length: its rows are asked for while the length is still on its way.
-    const int steps = (max(last - first, 0) + kStep - 1) / kStep;
+    const int steps = steps_for(max(last - first, 0));
     constexpr int kStride = SHARES ? kStep : C::WAVES * kStep;
     const int from = first + (SHARES ? steps * wave / C::WAVES : wave) * kStep;
-    const int to = SHARES ? min(last, first + steps * (wave + 1) / C::WAVES * kStep) : last;
+    const int to = SHARES && wave + 1 < C::WAVES ? first + steps * (wave + 1) / C::WAVES * kStep : last;
     typedef const __attribute__((address_space(4))) std::int32_t* scalar_table;
     const scalar_table table = (scalar_table)(a.table + static_cast<std::int64_t>(stream) * a.table_stride);
 
@@ -330,7 +328,7 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
     }
     // K of the next step is asked for as soon as this step's has been used, V
     // likewise, so a wave always has about a step of the cache in flight.
-    for (int j = from; j < to; j += kStride) {
+    for (int left = to - from; left > 0; left -= kStride) {
 #pragma clang fp contract(off)  // a score less the base: of the score as it was when the base was taken
         floatx4 dot[2];
 #pragma unroll
@@ -351,16 +349,16 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
                 y[e] = __builtin_amdgcn_logf(vs[e >> 2][e & 3]);
             }
         }
-        const bool ragged = j + kStep > to || !there[0] || !there[1];
+        const bool ragged = left < kStep || !there[0] || !there[1];
         const bool seen[2] = {there[0], there[1]};
-        if (j + kStride < to) {
-            locate(j + kStride);
+        if (left > kStride) {
+            locate(to - left + kStride);
             fetch_k();
         }
         if (ragged) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (!seen[e >> 2] || j + 16 * (e >> 2) + 4 * g + (e & 3) >= to) {
+                if (!seen[e >> 2] || 16 * (e >> 2) + 4 * g + (e & 3) >= left) {
                     // Not seen: weight zero, and a value that is finite whatever lies there.
                     x[e] = -INFINITY, y[e] = 0.0f;
 #pragma unroll
@@ -423,7 +421,7 @@ __device__ __forceinline__ void token_piece(const TokenArgs& a, float* joint, in
                 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, lo, o, 0, 0, 0);
             }
         }
-        if (j + kStride < to) fetch_v(row);
+        if (left > kStride) fetch_v(row);
     }
     l = column_sum(l);
 

@@ -329,3 +329,26 @@ def test_prompt_many_sequences_of_one_tile(dev, rng, sequences, heads, most, dim
         within(got[a, -1:], want, tol, f"{nq} on {nk}") if nq else None
         i, j = i + nq, j + nk
     assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 24])
+def test_tokens_of_lengths_at_31_bits(dev, rng, kind, dim):
+    """Contexts that end at 2^31 - 1 tokens and a little before it, on one page of zero keys that repeats and a last
+    one with two keys that weigh e^40 times the others: what 2^31 of those add is below 2^-25."""
+    last, page, width = (1 << 31) - 1, 1 << 16, 1 << 15
+    cache = Cache(dev, kind, 2, page, 1, dim)
+    k, v = np.zeros((page, 1, dim), np.float16), rng.standard_normal((page, 1, dim)).astype(np.float16)
+    cache.write(k, v, np.arange(page))
+    k[[-22, -2], 0, 0] = 40                 # places last - 21 and last - 1
+    cache.write(k[:-1], v[:-1], np.arange(page, 2 * page - 1))
+    table = np.zeros((3, width), np.int32)
+    table[:, -1] = 1
+    q = np.zeros((3, 2, dim), np.float16)
+    q[..., 0] = 1
+    got = Token(cache, q, table, [last, last - 20, 40], 1.0).run()
+    sv = stored64(v, kind)[:, 0]
+    for stream, (want, size) in enumerate((((sv[-22] + sv[-2]) / 2, np.maximum(abs(sv[-22]), abs(sv[-2]))), (sv[-22], abs(sv[-22])),
+                                           (sv[:40].mean(0), np.abs(sv[:40]).max(0)))):
+        # The weights' rounding and the output's, and the other tokens.
+        within(got[stream], np.broadcast_to(want, (2, dim)), size * 2.0 ** -10 + 2.0 ** -20, f"stream {stream}")
