@@ -101,15 +101,28 @@ struct Sight {
     }
 };
 
-// A score and the logarithm of its row's scale, for the base. FP32 numbers of 2^28
-// and more are 32 and more apart: a sum that falls so far below the exact one that
-// the weight, 2^(score - sum) scale, would not fit FP16 gives way to the score, which
-// is above the exact one (scales of 2^15 and more do not come from FP16 rows).
-__device__ __forceinline__ float with_scale(float score, float scale)
+// Largest score and logarithm of its row's scale of a lane's N, for the base. FP32
+// numbers of 2^28 and more are 32 and more apart: there a sum that falls so far below
+// the exact one that the weight, 2^(score - sum) scale, would not fit FP16 gives way to
+// the score, which is above the exact one (scales of 2^15 and more do not come from
+// FP16 rows).
+template <int KIND, int N>
+__device__ __forceinline__ float largest(const float (&x)[N], const float (&scale)[N])
 {
 #pragma clang fp contract(off) reassociate(off)
-    const float log = __builtin_amdgcn_logf(scale), sum = score + log;
-    return score - sum + log > kMost ? score : sum;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, KIND == MLVC_KV_F16 ? x[i] : x[i] + __builtin_amdgcn_logf(scale[i]));
+    if constexpr (KIND != MLVC_KV_F16)
+        if (__any(fabsf(top) >= 0x1p28f && is_finite(top))) {
+            top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float log = __builtin_amdgcn_logf(scale[i]), sum = x[i] + log;
+                top = fmaxf(top, x[i] - sum + log > kMost ? x[i] : sum);
+            }
+        }
+    return top;
 }
 
 // Masks and depths of a stream's drafts, one a lane.
@@ -544,10 +557,7 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
 #pragma unroll
             for (int e = 2; e < 8; ++e) top = fmaxf(top, wt[e]);
             if (__any(top > 0x1p15f)) {
-                top = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, KIND == MLVC_KV_F16 ? x[e] : with_scale(x[e], scale[e]));
-                const float now = fmaxf(base[b], lifted(column_max(top))), keep = __builtin_amdgcn_exp2f(base[b] - now);
+                const float now = fmaxf(base[b], lifted(column_max(largest<KIND>(x, scale)))), keep = __builtin_amdgcn_exp2f(base[b] - now);
                 l[b] *= keep;
 #pragma unroll
                 for (int i = 0; i < C::DT; ++i)
@@ -859,10 +869,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
         for (int r = 1; r < 15; r += 2) top = fmaxf(fmaxf(top, wt[r]), wt[r + 1]);
         top = fmaxf(top, wt[15]);
         if (__any(top > 0x1p15f)) {
-            top = -INFINITY;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, KIND == MLVC_KV_F16 ? x[r] : with_scale(x[r], scale[r]));
-            const float now = fmaxf(base, lifted(both_max(top))), keep = __builtin_amdgcn_exp2f(base - now);
+            const float now = fmaxf(base, lifted(both_max(largest<KIND>(x, scale)))), keep = __builtin_amdgcn_exp2f(base - now);
             l *= keep;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
