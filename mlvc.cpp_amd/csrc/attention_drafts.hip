@@ -37,7 +37,8 @@ struct DraftArgs {
     const unsigned long long* seen;
     const std::int32_t* table;
     const std::int32_t* lengths;
-    const std::int32_t* placed;
+    const std::int32_t* placed;  // drafts of a stream in the cache; any array where all are
+    int all_placed;              // INT_MAX: all are; 0
     int table_stride, pages, page, heads, q_heads, group, dim, longest, longest_q, q_tokens, streams, window, sinks;
     float scale2;
     float* part;    // [heads][rows][places][dim], a row for each draft and query head of a group
@@ -60,11 +61,11 @@ struct View {
     __device__ View(const DraftArgs& a, int stream)
     {
         const int begin = a.starts[stream], end = a.starts[stream + 1];
+        const int placed = max(a.placed[stream], a.all_placed);  // no branch: the four are asked for together
         int tokens = a.lengths[stream];
         const std::int64_t held = static_cast<std::int64_t>(a.table_stride) * a.page;
         start = min(max(begin, 0), a.q_tokens);
-        drafts = max(end - begin, 0);
-        if (a.placed) drafts = min(drafts, max(a.placed[stream], 0));
+        drafts = min(max(end - begin, 0), placed);
         queries = min(min(drafts, a.longest_q), a.q_tokens - start);
         tokens = max(tokens, 0);
         past = tokens - drafts;
@@ -78,9 +79,9 @@ struct View {
     }
     // First token of a step.
     __device__ int token(int step) const { return (step < sink_steps ? step : step + skipped) * kStep; }
-    // Whether no draft sees a part only of the step at token j, whose tiles are there: it ends before the drafts,
-    // before the context is cut, and not across the window's edge, behind which all drafts see from clear_from on.
-    __device__ bool whole(int j, int clear_from) const { return min(past, length) - j >= kStep && (j >= clear_from || sinks - j >= kStep); }
+    // Whether all drafts see all of the step at token j, if its tiles are there: context before the drafts and the
+    // cut (clear_to), from the window's edge on (clear_from) or among the sinks.
+    __device__ bool clear(int j, int clear_from, int clear_to) const { return clear_to - j >= kStep && (j >= clear_from || sinks - j >= kStep); }
 };
 
 // What a draft sees.
@@ -114,7 +115,7 @@ __device__ __forceinline__ float largest(const float (&x)[N], const float (&scal
 #pragma unroll
     for (int i = 0; i < N; ++i) top = fmaxf(top, KIND == MLVC_KV_F16 ? x[i] : x[i] + __builtin_amdgcn_logf(scale[i]));
     if constexpr (KIND != MLVC_KV_F16)
-        if (__any(fabsf(top) >= 0x1p28f && is_finite(top))) {
+        if (__builtin_expect(__any(fabsf(top) >= 0x1p28f && is_finite(top)), false)) {
             top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -463,8 +464,8 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
 #pragma unroll
     for (int b = 0; b < NB; ++b) draft[b] = static_cast<int>(static_cast<unsigned>(row0 + min(b * 16 + col, mine - 1)) / static_cast<unsigned>(a.group));
     __syncthreads();
-    // Context that all drafts see, from here to `past`.
-    const int clear_from = a.window ? max(w.past + min(w.drafts, kMostDrafts) - a.window, 0) : 0;
+    // Context that all drafts see.
+    const int clear_to = min(w.past, w.length), clear_from = a.window ? max(w.past + min(w.drafts, kMostDrafts) - a.window, 0) : 0;
 
     floatx4 acc[NB][C::DT];
     float base[NB], l[NB];
@@ -504,7 +505,7 @@ __device__ __forceinline__ void draft_piece(const DraftArgs& a, char* lds, Sight
             factor[e] = KIND == MLVC_KV_F16 ? a.scale2 : ks[e >> 2][e & 3] * a.scale2;
             scale[e] = KIND == MLVC_KV_F16 ? 1.0f : __builtin_elementwise_maximum(vs[e >> 2][e & 3], 0x1p-40f);
         }
-        const bool masked = !there[0] || !there[1] || !w.whole(j, clear_from);
+        const bool masked = !there[0] || !there[1] || !w.clear(j, clear_from, clear_to);
         const bool here[2] = {there[0], there[1]};
         // The last step asks for itself again: so that there are always as many loads,
         // and the wait for K leaves V on its way.
@@ -771,7 +772,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
             }
         }
     }
-    const int clear_from = a.window ? max(w.past + min(w.drafts, kMostDrafts) - a.window, 0) : 0;
+    const int clear_to = min(w.past, w.length), clear_from = a.window ? max(w.past + min(w.drafts, kMostDrafts) - a.window, 0) : 0;
 
     // Places of this lane's pieces: of K, pieces 2 ks + hi of row lane & 31; of V,
     // the transposing read of 16 lanes takes 4 halves of each of 4 rows (4 hi + 8 e
@@ -900,7 +901,7 @@ __device__ __forceinline__ void tile_piece(const DraftArgs& a, char* lds, Sight*
     auto take_turn = [&](int turn, Coming& c) {
         const int step = first + turn * KG + kg, buffer = turn & 1, j = c.j;
         const bool here0 = c.there[0], here1 = c.there[1];
-        const bool masked = !here0 || !here1 || !w.whole(j, clear_from);
+        const bool masked = !here0 || !here1 || !w.clear(j, clear_from, clear_to);
         unpack(c, buffer, masked);
         fetch(min(step + C::DEPTH * KG, last - 1), c);
         __syncthreads();
@@ -1281,7 +1282,8 @@ void attention_drafts(const mlvc_hip_attention_drafts_desc* d, hipStream_t s)
     a.k_scale = c->k_scale, a.v_scale = c->v_scale;
     a.q = static_cast<const std::uint16_t*>(d->q), a.out = static_cast<std::uint16_t*>(d->out);
     a.q_stride = d->q_stride, a.out_stride = d->out_stride;
-    a.starts = d->starts, a.seen = reinterpret_cast<const unsigned long long*>(d->seen), a.table = d->table, a.lengths = d->lengths, a.placed = d->placed;
+    a.starts = d->starts, a.seen = reinterpret_cast<const unsigned long long*>(d->seen), a.table = d->table, a.lengths = d->lengths;
+    a.placed = d->placed ? d->placed : d->lengths, a.all_placed = d->placed ? 0 : INT_MAX;
     a.table_stride = d->table_stride, a.pages = c->pages, a.page = c->page_size, a.heads = c->heads;
     a.q_heads = d->q_heads, a.group = d->q_heads / c->heads, a.dim = c->head_dim;
     a.longest = c->pages ? d->longest : 0, a.longest_q = d->longest_q, a.q_tokens = d->q_tokens, a.streams = d->streams;
