@@ -557,9 +557,9 @@ int mlvc_hip_attention_token(const mlvc_hip_attention_token_desc* desc, mlvc_hip
  *   2. streams take the pages that their new tokens need beyond what they hold,
  *      stream by stream, from the top of the stack free_pages; the first one
  *      that the pool does not suffice for and those behind it that need a page
- *      get none (lacking counts them), nor does a stream whose tokens go beyond
- *      its table row or 2^31 - 1; placed[n] is the number of a stream's new
- *      tokens that have slots, fresh[n] or for one that got no pages 0;
+ *      get none, nor does a stream whose tokens go beyond its table row or
+ *      2^31 - 1 (lacking counts both); placed[n] is the number of its new tokens,
+ *      or 0 for a stream that got no pages;
  *   3. lengths[n] = past[n] + fresh[n] (past[n] for a stream that got no pages),
  *      starts = 0, then the sums of fresh; token t, the i-th new one of stream
  *      n, has slots[t], the slot of place past[n] + i, and positions[t] = past[n]
@@ -613,10 +613,10 @@ int mlvc_hip_attention_window(const mlvc_hip_attention_window_desc* desc, mlvc_h
  * ordinary step under a window. Drafts past `longest_q` or the 64th are not
  * computed, and seen by none; their rows of out stay as they are, as do those
  * past the last stream's. With `placed` only the first placed[n] of a stream's
- * drafts are in the cache, and the others' rows of out stay as they are. A draft that sees nothing gives zeros. Pages, lengths,
- * infinities, the workspace and the order of sums are as in
- * mlvc_hip_attention_token; a weight of the softmax is off by at most 2^-11 of
- * itself or 2^-37 of the largest. */
+ * drafts are in the cache, and the others' rows of out stay as they are. A draft
+ * that sees nothing gives zeros. Pages, lengths, infinities, the workspace and the
+ * order of sums are as in mlvc_hip_attention_token; for scores below 2^22 a weight
+ * of the softmax is off by at most 2^-11 of itself or 2^-37 of the largest. */
 typedef struct mlvc_hip_attention_drafts_desc {
     const mlvc_hip_kv_cache* cache;
     int streams, q_heads;          /* q_heads a multiple of the cache's heads */
@@ -645,9 +645,9 @@ int mlvc_hip_attention_drafts(const mlvc_hip_attention_drafts_desc* desc, mlvc_h
 /* Keeps a path of each stream's drafts: draft kept[n][i] moves to the i-th place
  * behind the context, its stored values and scales as they are, and
  * lengths_out[n] becomes the context's length with the kept drafts. A number
- * that is no draft of the stream (-1) ends its list; with `placed` only the first
- * placed[n] of its drafts are there, as the last of its tokens. The same draft may stand
- * twice. Rows whose page is not in the cache are not moved. */
+ * that is no draft of the stream (-1) ends its list. The same draft may stand
+ * twice. Rows whose page is not in the cache are not moved. With `placed` only the
+ * first placed[n] of a stream's drafts are there, as the last of its tokens. */
 typedef struct mlvc_hip_kv_keep_desc {
     const mlvc_hip_kv_cache* cache;
     int streams;

@@ -267,8 +267,8 @@ __device__ __forceinline__ bool choose(const PromptArgs& a, int rank, int tiles,
 // [from, to), and of the latter those that all of them see whole, [clear_from,
 // clear_to). They are taken in the order clear, sinks, before, behind.
 //
-// 32640 tokens, 16 / 4 heads of 128, a window of 1024 and 4 sinks: 371 to 381 us,
-// box to box, 714 to 733 TFLOP/s of what is seen. Of the 19 tiles of a workgroup
+// 32640 tokens, 16 / 4 heads of 128, a window of 1024 and 4 sinks: 362 to 381 us,
+// box to box, 714 to 749 TFLOP/s of what is seen. Of the 19 tiles of a workgroup
 // five need masks and are half seen on average, and a workgroup's start and end
 // (6 us of 48) come eight times in a row.
 struct WindowTiles {
@@ -817,27 +817,28 @@ void launch_prompt(const PromptArgs& a, hipStream_t s)
 // Under a window a workgroup's keys are few and as many in each, so that 256
 // queries gain nothing, and key groups less: two beside 64 queries while those
 // workgroups fit the GPU at once, four beside 32 or 64 while they fit the CUs.
-// us, a window of w (16 query heads, 4 sinks, causal; each is 3 to 6% less since
-// masks come from a word of bits):
-//   heads of 128              (1,4,32) (2,4,32) (2,2,32) (4,2,64) (4,1,64) (8,1,64)
-//     10 on 1500, w 700         12.1     13.3     14.9     17.6     21.6     24.8
-//     240, w 80                  9.2     10.7     10.0     12.6     13.3     16.0
-//     920, w 256                19.9     13.0     12.6     17.0     18.4     27.8
-//     2040, w 512               45.6     29.7     21.0     21.8     24.5     34.4
-//     8160, w 64                 110     81.1     46.0     54.1     37.8     46.2
-//     8160, w 1024               237      144      104      110     94.2      103
-//     8160, w 4080               490      299      252      237      229      252
-//     32640, w 1024              998      588      433      437      371      414
-//   heads of 64               (1,4,64) (1,4,32) (2,4,64) (2,2,32) (4,2,64) (4,1,64)
-//     240, w 80                  6.3      6.6      7.4      7.7      9.1     10.4
-//     10 on 1500, w 700         10.0      8.4     10.9     11.5     13.4     16.1
-//     920, w 300                15.4      8.5      9.8     10.6     12.5     15.6
+// us, a window of w (16 query heads, 4 sinks, causal), of one box and with masks by
+// each key's place; taken: the shape that the rule takes, with masks from a word of
+// bits, on another box:
+//   heads of 128              (1,4,32) (2,4,32) (2,2,32) (4,2,64) (4,1,64) (8,1,64)  taken
+//     10 on 1500, w 700         12.1     13.3     14.9     17.6     21.6     24.8     12.0
+//     240, w 80                  9.2     10.7     10.0     12.6     13.3     16.0      9.0
+//     920, w 256                19.9     13.0     12.6     17.0     18.4     27.8     13.2
+//     2040, w 512               45.6     29.7     21.0     21.8     24.5     34.4     22.4
+//     8160, w 64                 110     81.1     46.0     54.1     37.8     46.2     37.2
+//     8160, w 1024               237      144      104      110     94.2      103     95.8
+//     8160, w 4080               490      299      252      237      229      252      234
+//     32640, w 1024              998      588      433      437      371      414      363
+//   heads of 64               (1,4,64) (1,4,32) (2,4,64) (2,2,32) (4,2,64) (4,1,64)  taken
+//     240, w 80                  6.3      6.6      7.4      7.7      9.1     10.4      6.0
+//     10 on 1500, w 700         10.0      8.4     10.9     11.5     13.4     16.1      8.2
+//     920, w 300                15.4      8.5      9.8     10.6     12.5     15.6      8.9
 //     700 and 600, w 100 both ways
-//                               21.1     14.5     16.0     10.6     11.7     14.5
-//     2040, w 300               29.6     15.6     18.6     12.9     12.9     15.9
+//                               21.1     14.5     16.0     10.6     11.7     14.5     10.4
+//     2040, w 300               29.6     15.6     18.6     12.9     12.9     15.9     12.9
 //     1..2040 packed, w 240 both ways
-//                               99.4     53.9     61.1     31.3     38.8     30.1
-//     8160, w 500                133     68.8     78.0     39.8     57.3     41.4
+//                               99.4     53.9     61.1     31.3     38.8     30.1     30.0
+//     8160, w 500                133     68.8     78.0     39.8     57.3     41.4     41.6
 template <int D>
 void launch_window(const PromptArgs& a, hipStream_t s)
 {
