@@ -73,9 +73,10 @@ __global__ __launch_bounds__(64) void prompt_any_kernel(PromptArgs a)
     constexpr int kColumns = kMaxHeadDim / 64;
     float acc[kColumns] = {}, m = -INFINITY, l = 0.0f;
     for (int range = 0; range < 2; ++range)
-        for (int j0 = from[range], seen = to[range]; j0 < seen; j0 += 64) {
+        for (int left = to[range] - from[range]; left > 0; left -= 64) {
+            const int j0 = to[range] - left;
             float s = -INFINITY;
-            if (j0 + lane < seen) {
+            if (lane < left) {
                 const std::uint16_t* k = a.k + static_cast<std::int64_t>(sk.first + j0 + lane) * a.k_stride + column;
                 s = 0.0f;
                 for (int d = 0; d < a.dim; ++d) s = fmaf(qs[d], h2f(k[d]), s);
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(64) void prompt_any_kernel(PromptArgs a)
             l = l * keep + group_sum<64>(p);
             ps[lane] = p;
             __syncthreads();
-            const int n = min(64, seen - j0);
+            const int n = min(64, left);
             const std::uint16_t* v = a.v + static_cast<std::int64_t>(sk.first + j0) * a.v_stride + column;
 #pragma unroll
             for (int c = 0; c < kColumns; ++c) {
@@ -901,11 +902,14 @@ void attention_prompt(const mlvc_hip_attention_prompt_desc* d, int window, int s
     a.scale2 = std::fabs(d->scale) * 1.4426950408889634f, a.negate = d->scale < 0.0f;
     // A window that reaches from end to end is none.
     a.window = window < static_cast<std::int64_t>(d->q_tokens) + d->k_tokens ? window : 0, a.sinks = sinks;
-    // The matrix-core kernel addresses a tile's rows by 32-bit byte offsets,
-    // and scales masked scores (-inf) by the factor, which must not be 0.
+    // The matrix-core kernel addresses a tile's rows by 32-bit byte offsets, counts
+    // whole tiles in 32 bits, and scales masked scores (-inf) by the factor, which
+    // must not be 0.
     constexpr std::int64_t kFarthest = std::int64_t{1} << 23;
+    constexpr int kMostTokens = INT_MAX - 1024;
     const bool rows = vector_rows(d->q, d->q_stride) && vector_rows(d->out, d->out_stride) && vector_rows(d->k, d->k_stride) &&
-                      vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f;
+                      vector_rows(d->v, d->v_stride) && d->k_stride < kFarthest && d->v_stride < kFarthest && a.scale2 > 1e-30f &&
+                      d->q_tokens <= kMostTokens && d->k_tokens <= kMostTokens;
     // The kernel under a window counts places in 32 bits.
     const std::int64_t tokens = static_cast<std::int64_t>(d->q_tokens) + d->k_tokens;
     const bool fast = rows && (!a.window || tokens < (std::int64_t{1} << 30));

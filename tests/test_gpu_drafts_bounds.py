@@ -8,9 +8,9 @@ import pytest
 
 import mlvc_hip
 from devmem import Dev
-from drafts import ALL, Contexts, Drafts, Plan, depths, drafts_seen, masked64, tops_of, tree
+from drafts import ALL, Contexts, Drafts, Plan, Window, depths, drafts_seen, masked64, tops_of, tree, window_seen
 from mlvc_hip import KV_E4M3, KV_F16, KV_INT8
-from tokens import Cache, Padded, f64, stored64, within
+from tokens import Cache, Padded, Prompt, f64, stored64, within
 
 pytestmark = pytest.mark.gpu
 
@@ -354,3 +354,22 @@ def test_drafts_of_lengths_at_31_bits(dev, rng, kind, q_heads, dim, most, longes
             seen[r] = ((e < 0) | mask) & ((place - at_place < window) | (at_place < sinks))
         check(got[at:at + count], q[at:at + count], k[rows], v[rows], kind, dim ** -0.5, seen, f"stream {i}")
         at += count
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("behind", [0, 30, 63, 64, 200])
+def test_window_of_keys_at_31_bits(dev, rng, causal, behind):
+    """A sequence of 2^31 - 1 keys and a little fewer, of which the window sees the last and the sinks the first."""
+    dim, n, tail, window, sinks = 1, (1 << 31) - 1 - behind, 1000, 100, 3
+    base = dev.alloc(2 * ((1 << 31) + 8))
+    rows = normal(rng, tail, 1, dim)
+    for at, part in ((0, rows[:sinks]), (n - tail + sinks, rows[sinks:])):
+        part = np.ascontiguousarray(part)
+        dev.check(dev.lib.mlvc_hip_memcpy_h2d(base.value + 2 * at, part.ctypes.data, part.nbytes, None))
+    q = normal(rng, 3, 2, dim)
+    p = Prompt(dev, q, rows, rows, [3], [n], causal, 0.5)
+    p.desc.k = p.desc.v = base.value
+    p.desc.k_tokens = n
+    seen = window_seen(3, tail, causal, window, sinks)
+    want, tol = masked64(f64(q), f64(rows), f64(rows), 0.5, seen)
+    within(Window(p, window, sinks).run(), want, tol)
